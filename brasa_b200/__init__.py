@@ -96,6 +96,15 @@ class _PagedKv(C.Structure):
                 ("num_pages", C.c_uint32), ("kv", C.c_int32)]
 
 
+class _PackedRun(C.Structure):
+    _fields_ = [("starts", _Arg), ("tokens", C.c_uint32), ("longest", C.c_uint32)]
+
+
+class _PagePool(C.Structure):
+    _fields_ = ([(n, _Arg) for n in ("kpool", "vpool", "table", "lens", "pinned")] +
+                [(n, C.c_uint32) for n in ("rows", "max_pages", "num_pages", "layers", "hkv")] + [("kv", C.c_int32)])
+
+
 class _Linear(C.Structure):
     _fields_ = ([(n, _Arg) for n in ("w", "x", "w2", "x2", "y", "bias", "resid")] +
                 [(n, C.c_uint32) for n in ("cols", "ldw", "ldx", "cols2", "ldw2", "ldx2", "rows", "tokens", "ldy")] +
@@ -561,6 +570,39 @@ class Kernels:
     def decode_attention_paged(self, cmd, q, paged: _PagedKv, partials, o, hq: int, hkv: int):
         self._k(self.L.brasa_k_decode_attention_paged(cmd._h, _arg(q), paged, _arg(partials), C.c_uint64(partials.nbytes // 4), _arg(o),
                                                       C.c_uint32(hq), C.c_uint32(hkv)))
+
+    @staticmethod
+    def packed_run(starts, tokens: int, longest: int) -> _PackedRun:
+        """New tokens of several sequences behind one another: starts u32 [seqs + 1] on the device, rows of the buffers, the most tokens of one sequence."""
+        return _PackedRun(_arg(starts), tokens, longest)
+
+    def qk_norm_rope_store_packed(self, cmd, q, k, v, q_norm, k_norm, eps, table: RopeTable, paged: _PagedKv, run: _PackedRun, q_out, hq: int, hkv: int):
+        """Norm and RoPE of q into q_out (may be q), of k into the pages; v into the pages: any number of new tokens per sequence."""
+        self._k(self.L.brasa_k_qk_norm_rope_store_packed(cmd._h, _arg(q), _arg(k), _arg(v), _arg(q_norm), _arg(k_norm), _arg(table.cos), _arg(table.sin),
+                                                         C.c_float(eps), paged, run, _arg(q_out), C.c_uint32(hq), C.c_uint32(hkv)))
+
+    def attention_packed(self, cmd, q, paged: _PagedKv, run: _PackedRun, o, hq: int, hkv: int, precision=PrefillPrecision.F32):
+        """Causal attention of a run's tokens over their sequences' pages; o f16 (precision F16) or f32."""
+        self._k(self.L.brasa_k_attention_packed(cmd._h, _arg(q), paged, run, _arg(o), C.c_uint32(hq), C.c_uint32(hkv), C.c_int32(int(precision))))
+
+    def verify_drafts(self, cmd, p, q, drafts, u, starts, seqs: int, rows: int, vocab: int, tokens, accepted):
+        """Accepts drafted tokens against the target's probabilities p and draws one more per sequence; q None: the drafts were not drawn but given."""
+        self._k(self.L.brasa_k_verify_drafts(cmd._h, _arg(p), _arg(q), _arg(drafts), _arg(u), _arg(starts), C.c_uint32(seqs), C.c_uint32(rows),
+                                             C.c_uint32(vocab), _arg(tokens), _arg(accepted)))
+
+    @staticmethod
+    def page_pool(kpool, vpool, table, lens, pinned, rows: int, max_pages: int, num_pages: int, layers: int, hkv: int, kv) -> _PagePool:
+        """All layers' pages, the rows' tables and lengths, and the pages that others hold too (pinned, may be None)."""
+        return _PagePool(_arg(kpool), _arg(vpool), _arg(table), _arg(lens), _arg(pinned), rows, max_pages, num_pages, layers, hkv, int(kv))
+
+    def pages_reassign(self, cmd, pool: _PagePool, source, keep, room, table_out, lens_out, result, accepted=None):
+        """Every row anew from `keep` positions of an old row (None: all, with those that `accepted` adds) and pages for `room` more: forks, reorders,
+        rolls back, frees, reserves."""
+        self._k(self.L.brasa_k_pages_reassign(cmd._h, pool, _arg(source), _arg(keep), _arg(accepted), _arg(room), _arg(table_out), _arg(lens_out), _arg(result)))
+
+    def pages_compact(self, cmd, pool: _PagePool, table_out, moved, result):
+        """Moves the pages in use to the front of the pool."""
+        self._k(self.L.brasa_k_pages_compact(cmd._h, pool, _arg(table_out), _arg(moved), _arg(result)))
 
     def store_kv(self, cmd, kv, src, dst, n):
         self._k(self.L.brasa_k_store_kv(cmd._h, C.c_int32(int(kv)), _arg(src), _arg(dst), C.c_uint64(n)))

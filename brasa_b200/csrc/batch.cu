@@ -726,9 +726,7 @@ int32_t encode_step(brasa_batch *b, brasa_cmd *cmd, uint32_t n) {
 
 }  // namespace
 
-extern "C" {
-
-static int32_t check_paged(brasa_ctx *ctx, const brasa_paged_kv &pg, uint32_t hq, uint32_t hkv) {
+int32_t brasa_check_paged(brasa_ctx *ctx, const brasa_paged_kv &pg, uint32_t hq, uint32_t hkv) {
     BRASA_REQUIRE(ctx, pg.kv >= BRASA_KV_F32 && pg.kv <= BRASA_KV_Q8_0, "paged kv: unknown KV type %d", pg.kv);
     BRASA_REQUIRE(ctx, hkv > 0 && hq % hkv == 0 && hq / hkv <= 8, "paged kv: GQA group must divide and be <= 8");
     BRASA_REQUIRE(ctx, pg.seqs >= 1 && pg.max_pages >= 1 && pg.num_pages >= 1, "paged kv: empty batch or pool");
@@ -739,11 +737,13 @@ static int32_t check_paged(brasa_ctx *ctx, const brasa_paged_kv &pg, uint32_t hq
     return BRASA_OK;
 }
 
+extern "C" {
+
 int32_t brasa_k_qk_norm_rope_store_paged(brasa_cmd *cmd, brasa_arg q, brasa_arg k, brasa_arg v, brasa_arg q_norm, brasa_arg k_norm, brasa_arg rope_cos,
                                          brasa_arg rope_sin, float eps, brasa_paged_kv pg, uint32_t hq, uint32_t hkv) {
     if (!cmd) return BRASA_EINVAL;
     brasa_ctx *ctx = cmd->ctx;
-    BRASA_TRY(check_paged(ctx, pg, hq, hkv));
+    BRASA_TRY(brasa_check_paged(ctx, pg, hq, hkv));
     BRASA_REQUIRE(ctx, arg_fits(q, (uint64_t)pg.seqs * hq * 512) && arg_fits(k, (uint64_t)pg.seqs * hkv * 512) && arg_fits(v, (uint64_t)pg.seqs * hkv * 512),
                   "qk_norm_rope_store_paged: q, k or v too small");
     BRASA_REQUIRE(ctx, arg_fits(q_norm, 512) && arg_fits(k_norm, 512), "qk_norm_rope_store_paged: norm weights too small");
@@ -770,7 +770,7 @@ int32_t brasa_k_decode_attention_paged(brasa_cmd *cmd, brasa_arg q, brasa_paged_
                                        uint32_t hkv) {
     if (!cmd) return BRASA_EINVAL;
     brasa_ctx *ctx = cmd->ctx;
-    BRASA_TRY(check_paged(ctx, pg, hq, hkv));
+    BRASA_TRY(brasa_check_paged(ctx, pg, hq, hkv));
     const uint32_t max_chunks = (uint32_t)(((uint64_t)pg.max_pages * PAGE + 127) / 128);
     const uint64_t need = (uint64_t)pg.seqs * hq * max_chunks * 130;
     BRASA_REQUIRE(ctx, partials_len >= need && arg_fits(partials, partials_len * 4), "decode_attention_paged: scratch of %llu floats needed",

@@ -50,6 +50,8 @@ struct brasa_ctx {
     float *gemm_part = nullptr;      // partial output tiles of the split-K tensor-core GEMM
     size_t gemm_part_bytes = 0;
     uint32_t *gemm_counters = nullptr;  // arrivals per output tile of that GEMM (GEMM_TC_COUNTERS words, zero between launches)
+    uint8_t *page_work = nullptr;       // flags, free list and copy list of the page operators
+    size_t page_work_bytes = 0;
     bool recorded = false;              // a graph has been recorded: its kernels may hold the address of any workspace there was
     std::mutex events_lock;
     std::vector<std::pair<cudaEvent_t, cudaEvent_t>> events;  // timing events of finished commands for the next ones, at most 16 pairs
@@ -188,6 +190,9 @@ static inline bool qm_fits(const brasa_qmatrix &m) {
 }
 
 int32_t brasa_post_launch(brasa_cmd *cmd, const char *name);
+
+// What every operator over a paged pool asks of it: known type, a group of at most 8, buffers large enough and aligned (batch.cu).
+int32_t brasa_check_paged(brasa_ctx *ctx, const brasa_paged_kv &pg, uint32_t hq, uint32_t hkv);
 
 // ops.cu. out[i] = layer norm of row x[rows ? rows[r] : r] times w[i] plus b[i], i < n_out (1 or 2), [n_rows][ldo] in f32 or bf16
 int32_t brasa_layer_norm_launch(brasa_cmd *cmd, const float *x, const uint32_t *rows, uint32_t n_rows, uint32_t n, float eps, const float *const *w,

@@ -1,0 +1,185 @@
+// Verification of drafted tokens against the target model's probabilities. With p the target's and q the draft's distribution, a draft x
+// drawn from q is accepted with probability min(1, p(x) / q(x)); at the first refusal a token is drawn from max(p - q, 0), normalised, and
+// behind the last accepted draft one from p. Whatever q is, the tokens are then distributed as p alone would have drawn them.
+//
+// One row of p (and of q) per sequence is all that has to be read: 2 x 0.6 MB for a vocabulary of 151 936, so a cluster of eight blocks
+// takes a sequence, each with an eighth of the ids. Masses and their sums are 64-bit: p - q of two f32 numbers is exact up to the last
+// bits, and where the running sum passes the drawn point is decided far below the smallest mass. The sums' order depends on the vocabulary alone.
+#include "brasa_internal.h"
+
+namespace {
+
+constexpr uint32_t THREADS = 512, WARPS = THREADS / 32, CLUSTER = 8;
+
+struct VerifyParams {
+    const float *p, *q, *u;
+    const uint32_t *drafts, *starts;
+    uint32_t *tokens, *accepted;
+    uint32_t seqs, rows, vocab;
+    uint64_t ndrafts;  // entries of drafts (and rows of q) that there are
+};
+
+// the same shared variable of block `rank` of the cluster
+__device__ __forceinline__ double cluster_double(const double *local, uint32_t rank) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(remote) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t cluster_word(const uint32_t *local, uint32_t rank) {
+    uint32_t remote, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) verify_drafts_kernel(VerifyParams a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (launched as a programmatic dependent: see brasa_launch_dependent)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ double block_sum[2], warp_sum[WARPS];
+    __shared__ uint32_t stop_s, token_s, last_s;
+    const uint32_t s = blockIdx.x / CLUSTER, me = blockIdx.x % CLUSTER, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t first = min(a.starts[s], a.rows), end = max(first, min(a.starts[s + 1], a.rows));
+    // ---- drafts lie without the sequences' last rows: as many fewer as sequences before this one have rows ----
+    uint32_t before = 0;
+    for (uint32_t i = tid; i - tid < s; i += THREADS) before += __syncthreads_count(i < s && min(a.starts[i + 1], a.rows) > min(a.starts[i], a.rows));
+    if (end == first) {  // (the same for the whole cluster)
+        if (me == 0 && tid == 0) a.accepted[s] = 0;
+        return;
+    }
+    const uint32_t n = end - first - 1;  // drafts
+    const size_t draft0 = (size_t)first - min(before, first);
+    if (tid == 0) {
+        stop_s = n;
+        last_s = 0;
+        token_s = UINT32_MAX;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += THREADS) {
+        bool take = false;
+        const uint32_t x = draft0 + i < a.ndrafts ? a.drafts[draft0 + i] : UINT32_MAX;
+        if (x < a.vocab) {
+            const double px = a.p[(size_t)(first + i) * a.vocab + x], qx = a.q ? a.q[(draft0 + i) * a.vocab + x] : 1.0;
+            take = (double)a.u[first + i] * qx < px;
+        }
+        if (!take) atomicMin(&stop_s, i);
+    }
+    __syncthreads();
+    const uint32_t stop = stop_s;
+    const bool drafted = stop < n && draft0 + stop < a.ndrafts;
+    const float *p = a.p + (size_t)(first + stop) * a.vocab, *q = drafted && a.q ? a.q + (draft0 + stop) * a.vocab : nullptr;
+    uint32_t gone = drafted && !a.q ? a.drafts[draft0 + stop] : UINT32_MAX;  // (a given draft: its own probability was 1)
+    // ---- masses of this block's ids, warp by warp; the second time round nothing is subtracted, when nothing was left ----
+    const uint32_t per_block = (a.vocab + CLUSTER - 1) / CLUSTER, b0 = min(me * per_block, a.vocab), b1 = min(b0 + per_block, a.vocab);
+    const uint32_t per_warp = (b1 - b0 + WARPS - 1) / WARPS, w0 = min(b0 + warp * per_warp, b1), w1 = min(w0 + per_warp, b1);
+    auto mass = [&](uint32_t i) -> double {
+        if (i == gone) return 0.0;
+        const double m = q ? (double)p[i] - (double)q[i] : (double)p[i];
+        return m > 0.0 && m < INFINITY ? m : 0.0;
+    };
+    double total = 0.0, start = 0.0;
+    uint32_t last = 0;  // the last of this thread's ids that has mass
+    int round = 0;
+    for (;; ++round) {
+        double m = 0.0;
+        for (uint32_t i = w0 + lane; i < w1; i += 32) {
+            const double x = mass(i);
+            if (x > 0.0) last = i;
+            m += x;
+        }
+        for (int x = 16; x > 0; x >>= 1) m += __shfl_xor_sync(0xffffffffu, m, x);
+        if (lane == 0) warp_sum[warp] = m;
+        __syncthreads();
+        if (tid == 0) {
+            double sum = 0.0;
+            for (uint32_t w = 0; w < WARPS; ++w) sum += warp_sum[w];
+            block_sum[round] = sum;
+        }
+        cluster_sync();
+        total = start = 0.0;
+        for (uint32_t r = 0; r < CLUSTER; ++r) {
+            const double b = cluster_double(&block_sum[round], r);
+            if (r < me) start += b;
+            total += b;
+        }
+        if (total > 0.0 || round == 1) break;
+        q = nullptr;
+        gone = UINT32_MAX;
+    }
+    // ---- the first id at which the running sum exceeds the point. A warp's piece of [0, total) ends where the next one's begins, in the very
+    // same sums, so one warp holds the point; two can only where rounding moved a block's end by a bit, and then the lower id counts ----
+    const double point = (double)a.u[end - 1] * total, block_end = start + block_sum[round];
+    for (uint32_t w = 0; w < warp; ++w) start += warp_sum[w];
+    const double piece_end = warp + 1 < WARPS ? start + warp_sum[warp] : block_end;
+    if (start <= point && point < piece_end) {
+        uint32_t id = UINT32_MAX;
+        for (uint32_t i0 = w0; i0 < w1 && id == UINT32_MAX; i0 += 256) {  // eight ids per lane
+            double m[8], sum = 0.0;
+            for (uint32_t k = 0; k < 8; ++k) {
+                const uint32_t i = i0 + 8 * lane + k;
+                m[k] = i < w1 ? mass(i) : 0.0;
+                sum += m[k];
+            }
+            double upto = sum;
+            for (uint32_t x = 1; x < 32; x <<= 1) {
+                const double v = __shfl_up_sync(0xffffffffu, upto, x);
+                if (lane >= x) upto += v;
+            }
+            uint32_t mine = UINT32_MAX;
+            double run = start + (upto - sum);
+            for (uint32_t k = 0; k < 8; ++k) {
+                run += m[k];
+                if (mine == UINT32_MAX && m[k] > 0.0 && run > point) mine = i0 + 8 * lane + k;
+            }
+            id = __reduce_min_sync(0xffffffffu, mine);
+            start += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (id == UINT32_MAX) id = __reduce_max_sync(0xffffffffu, last);  // (rounding: the piece's last mass)
+        if (lane == 0) atomicMin(&token_s, id);
+    }
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0) atomicMax(&last_s, last);
+    cluster_sync();
+    if (me == 0 && warp == 0) {
+        uint32_t token = UINT32_MAX, final = 0;
+        for (uint32_t r = 0; r < CLUSTER; ++r) {
+            token = min(token, cluster_word(&token_s, r));
+            final = max(final, cluster_word(&last_s, r));
+        }
+        if (token == UINT32_MAX) token = final;  // (a point behind every sum: the last id that has mass; none has: 0)
+        if (lane == 0) {
+            a.accepted[s] = stop;
+            a.tokens[first + stop] = token;
+        }
+        for (uint32_t i = lane; i <= n; i += 32)
+            if (i != stop) a.tokens[first + i] = i < stop ? a.drafts[draft0 + i] : 0u;
+    }
+    cluster_sync();  // (no block leaves while another reads its words)
+}
+
+}  // namespace
+
+extern "C" int32_t brasa_k_verify_drafts(brasa_cmd *cmd, brasa_arg p, brasa_arg q, brasa_arg drafts, brasa_arg u, brasa_arg starts, uint32_t seqs, uint32_t rows,
+                                         uint32_t vocab, brasa_arg tokens, brasa_arg accepted) {
+    if (!cmd) return BRASA_EINVAL;
+    brasa_ctx *ctx = cmd->ctx;
+    BRASA_REQUIRE(ctx, seqs >= 1 && rows >= 1 && vocab >= 1, "verify_drafts: no sequences, rows or vocabulary");
+    BRASA_REQUIRE(ctx, seqs <= (1u << 31) / CLUSTER - 1 && vocab <= 1u << 31, "verify_drafts: more than 2^28 sequences or 2^31 ids");
+    // at least so many drafts: a sequence without rows makes it more, which the kernel holds against what there is
+    const uint64_t nd = rows > seqs ? rows - seqs : 0;
+    BRASA_REQUIRE(ctx, arg_fits(p, (uint64_t)rows * vocab * 4) && arg_fits(u, (uint64_t)rows * 4) && arg_fits(starts, ((uint64_t)seqs + 1) * 4),
+                  "verify_drafts: p, u or starts too small");
+    BRASA_REQUIRE(ctx, arg_fits(drafts, nd * 4) && (!q.buf || arg_fits(q, nd * vocab * 4)), "verify_drafts: drafts or q too small");
+    BRASA_REQUIRE(ctx, arg_fits(tokens, (uint64_t)rows * 4) && arg_fits(accepted, (uint64_t)seqs * 4), "verify_drafts: tokens or accepted too small");
+    for (const brasa_arg *a : {&p, &q, &drafts, &u, &starts, &tokens, &accepted}) BRASA_REQUIRE(ctx, a->offset % 4 == 0, "verify_drafts: misaligned buffer");
+    VerifyParams a{(const float *)arg_ptr(p), (const float *)arg_ptr(q), (const float *)arg_ptr(u), (const uint32_t *)arg_ptr(drafts), (const uint32_t *)arg_ptr(starts),
+                   (uint32_t *)arg_ptr(tokens), (uint32_t *)arg_ptr(accepted), seqs, rows, vocab, drafts.buf ? (drafts.buf->bytes - drafts.offset) / 4 : 0};
+    if (q.buf) a.ndrafts = std::min(a.ndrafts, (q.buf->bytes - q.offset) / 4 / vocab);
+    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, verify_drafts_kernel, dim3(seqs * CLUSTER), dim3(THREADS), 0, a));
+    return brasa_post_launch(cmd, "verify_drafts");
+}

@@ -431,6 +431,69 @@ int32_t brasa_k_qk_norm_rope_store_paged(brasa_cmd *cmd, brasa_arg q, brasa_arg 
 int32_t brasa_k_decode_attention_paged(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv paged, brasa_arg partials, uint64_t partials_len, brasa_arg o,
                                        uint32_t hq, uint32_t hkv);
 
+/* ---- several new tokens per sequence over the paged pool (no counterpart in the reference, which decodes one sequence and one token
+ * at a time): prompts of different lengths packed behind one another, drafted tokens to be verified, a prompt's next portion beside
+ * decoding sequences. The tokens of all sequences lie behind one another: sequence s of the brasa_paged_kv has rows
+ * starts[s] .. starts[s + 1] - 1 of q, k, v and o (starts: u32 [seqs + 1] on the device, not falling; none is a sequence without new
+ * tokens) at its positions lens[s], lens[s] + 1, ... Rows behind starts[seqs] are left alone. lens stays as it is: a step advances it
+ * behind its last layer. Whatever the device data says, nothing outside the buffers is touched: rows from `tokens` on, a
+ * sequence's tokens from `longest` on and positions from max_pages * 16 on are left alone, and a page number that is negative or not
+ * below num_pages stands for sixteen positions that hold nothing: none is stored there, none is attended to. */
+typedef struct brasa_packed_run {
+    brasa_arg starts;
+    uint32_t tokens;  /* rows of the buffers, at least starts[seqs] */
+    uint32_t longest; /* the most tokens one sequence has in this run */
+} brasa_packed_run;
+/* brasa_k_qk_norm_rope_store_paged for such a run: q f32 [tokens][hq][128] is normalised and rotated into q_out (which may be q), k and
+ * v f32 [tokens][hkv][128] are read: normalised and rotated k, and v, are rounded to the cache type and stored into the pages. No two
+ * tokens may share a place of the pool. Tables as for the paged call: every position that max_pages pages reach. */
+int32_t brasa_k_qk_norm_rope_store_packed(brasa_cmd *cmd, brasa_arg q, brasa_arg k, brasa_arg v, brasa_arg q_norm, brasa_arg k_norm, brasa_arg rope_cos,
+                                          brasa_arg rope_sin, float eps, brasa_paged_kv paged, brasa_packed_run run, brasa_arg q_out, uint32_t hq, uint32_t hkv);
+/* Causal attention of the run's tokens: a token attends to the positions of its sequence up to its own, which the call before it has
+ * stored. q f32 [tokens][hq][128]; precision F16: o f16 [tokens][hq][128], q * scale rounded to f16, as brasa_k_flash_attention; F32:
+ * o f32, nothing rounded but the sums. Cache rows that a sequence has not reached may hold anything, infinities and NaN included. A token
+ * that sees no position gives zeros. */
+int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv paged, brasa_packed_run run, brasa_arg o, uint32_t hq, uint32_t hkv, int32_t precision);
+/* Verification of drafted tokens. Sequence s has rows starts[s] .. starts[s + 1] - 1 (u32 [seqs + 1], not falling, at most `rows`) of p
+ * f32 [rows][vocab], the target model's probabilities behind its last token and behind each of its drafted ones, so one row more
+ * than drafted tokens. drafts u32 and q f32 [.][vocab], the probabilities that each draft was drawn from, have no entry for a sequence's
+ * last row and lie without gaps. u f32 [rows]: one number of [0, 1) for every row. Draft i is accepted while all before it are and
+ * u * q(draft) < p(draft). accepted[s] (u32) is their number, tokens[starts[s] + i] (u32) the accepted drafts, behind them one token
+ * more, behind that zeros. That token is drawn with the u of the sequence's last row: from max(p - q, 0) of the refused draft's row, or
+ * from p of the last row when none was refused: the first id at which the running sum, from id 0 on and in 64 bits, exceeds u times the
+ * whole. q.buf NULL: the drafts were not drawn but given, q is 1 at the draft and 0 elsewhere. Entries that are no positive finite
+ * numbers count as 0, a draft that is not below vocab is refused; where max(p - q, 0) holds nothing p takes its place, and
+ * where p does not either the token is 0. Rows of no sequence are left alone, one without rows gets accepted 0. */
+int32_t brasa_k_verify_drafts(brasa_cmd *cmd, brasa_arg p, brasa_arg q, brasa_arg drafts, brasa_arg u, brasa_arg starts, uint32_t seqs, uint32_t rows,
+                              uint32_t vocab, brasa_arg tokens, brasa_arg accepted);
+/* Pages of all layers and who holds them, for a caller that keeps its own page tables: kpool, vpool [layers][num_pages]
+ * [BRASA_KV_PAGE positions][hkv][128] in the cache type; table i32 [rows][max_pages], row r the pages of its positions in order, -1 where it
+ * has none; lens u32 [rows], the positions it holds; pinned u32 [num_pages], pages that are not 0 there belong to someone else as well and are
+ * neither handed out nor moved nor given away for writing (buf NULL: none). Rows may share pages. Up to 2^19 pages and 65 536 rows. */
+typedef struct brasa_page_pool {
+    brasa_arg kpool, vpool, table, lens, pinned;
+    uint32_t rows, max_pages, num_pages, layers, hkv;
+    int32_t kv; /* brasa_kv_type */
+} brasa_page_pool;
+/* Every row anew: row r takes over the first positions of the old row source[r] (i32; outside the rows: nothing), keep[r] (u32; buf NULL:
+ * all) of the lens[source[r]] that it holds, and gets pages for room[r] (u32) positions more, as far as max_pages reach. With accepted
+ * (u32 [rows], buf NULL: none), as brasa_k_verify_drafts leaves it, an old row s holds accepted[s] + 1 positions more than lens[s]: the token
+ * that the step began with and the drafts that stood. One call forks (several rows with one source), reorders,
+ * rolls back, frees (source -1 or keep 0, room 0) and reserves. Whole pages that are kept are shared. The last page of a row, when it is not
+ * full, becomes its own to write into: the first row that ends in it keeps it, unless it is pinned or held as a whole page too, the
+ * others get copies of it in all layers. Pages that no new row holds are free at once; free ones are handed out from the lowest
+ * on, to the rows in order (a copy's page ahead of those for new positions). Table entries that name no page are kept as -1.
+ * table_out i32 [rows][max_pages] and lens_out u32 [rows] must not overlap table and lens. result u32[4]: pages in use (pinned ones among them), pages
+ * copied, pages free, pages missing; when pages are missing nothing is copied and table_out and lens_out are table and lens (entries
+ * that name no page are -1). */
+int32_t brasa_k_pages_reassign(brasa_cmd *cmd, brasa_page_pool pool, brasa_arg source, brasa_arg keep, brasa_arg accepted, brasa_arg room, brasa_arg table_out,
+                               brasa_arg lens_out, brasa_arg result);
+/* Moves pages to the front of the pool: the highest page in use that is not pinned to the lowest free one, until none lies behind a free
+ * one. In use is what the table names or pinned holds. table_out i32 [rows][max_pages] (which may be table) names the new places, moved
+ * i32 [num_pages] where every page went (itself if it stayed, -1 if it was not in use). result u32[4]: pages in use, pages moved, one more
+ * than the highest page now in use, 0. */
+int32_t brasa_k_pages_compact(brasa_cmd *cmd, brasa_page_pool pool, brasa_arg table_out, brasa_arg moved, brasa_arg result);
+
 /* Memory of a batch before it is created (crates/memory/src/planner.rs:57-95 for the paged pool): the same sums
  * brasa_batch_create allocates, buffer by buffer. head_rows: the model's lm_head rows (its vocabulary unless it is a
  * tensor-parallel shard). */

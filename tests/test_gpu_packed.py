@@ -1,0 +1,548 @@
+"""Operators over packed runs (several new tokens per sequence of a paged cache), verification of drafted tokens, pages that are handed on:
+each against a plain 64-bit computation, and all of them together as one decoding loop."""
+import numpy as np
+import pytest
+
+import packed_cases as R
+
+pytestmark = pytest.mark.gpu
+
+KV = {"f32": 0, "f16": 1, "q8_0": 2}
+EPS, THETA = 1e-6, 1e6
+
+
+@pytest.fixture(scope="module")
+def B():
+    import brasa_b200
+    return brasa_b200
+
+
+@pytest.fixture(scope="module")
+def ctx(B):
+    c = B.Context(0)
+    yield c
+    c.close()
+
+
+@pytest.fixture(scope="module")
+def K(B, ctx):
+    return B.Kernels(ctx)
+
+
+def go(ctx, f):
+    cmd = ctx.command()
+    try:
+        f(cmd)
+    finally:
+        cmd.wait()
+
+
+class OnDevice:
+    """A Run in device buffers."""
+
+    def __init__(self, ctx, K, run, longest=None, tokens=None, starts=None):
+        self.run = run
+        self.bufs = [ctx.buffer_from(x) for x in (run.k, run.v, run.table, run.lens, run.starts if starts is None else np.array(starts, np.uint32), run.q)]
+        k, v, t, n, s, self.q = self.bufs
+        self.kpool, self.vpool = k, v
+        self.paged = K.paged_kv(k, v, t, n, len(run.seqs), run.max_pages, run.num_pages, KV[run.kv])
+        self.packed = K.packed_run(s, tokens or run.tokens, longest or run.longest)
+
+    def free(self):
+        for b in self.bufs:
+            b.free()
+
+
+def attend(ctx, K, run, half, **kw):
+    dev = OnDevice(ctx, K, run, **kw)
+    n = run.tokens * run.hq * 128
+    o = ctx.buffer(n * (2 if half else 4))
+    o.fill(0x3C)
+    go(ctx, lambda c: K.attention_packed(c, dev.q, dev.paged, dev.packed, o, run.hq, run.hkv, 0 if half else 1))
+    got = o.download(np.float16 if half else np.float32).astype(np.float64).reshape(run.tokens, run.hq, 128)
+    untouched = np.frombuffer(b"\x3c" * 4, np.float16 if half else np.float32)[0].astype(np.float64)
+    o.free()
+    dev.free()
+    return got, untouched
+
+
+def check(got, want, tol):
+    off = np.abs(got - want)
+    assert np.isfinite(got).all()
+    worst = np.unravel_index(np.argmax(off - tol), off.shape)
+    assert (off <= tol).all(), (worst, got[worst], want[worst], tol[worst])
+
+
+SHAPES = {
+    "one": [(1, 0)],
+    "one-deep": [(1, 700)],
+    "page-ends": [(1, 15), (1, 16), (1, 17), (2, 14), (16, 0), (17, 0), (15, 1), (1, 127), (1, 128), (129, 0)],
+    "drafts": [(5, 130), (1, 63), (3, 300), (0, 40), (4, 0), (5, 511), (2, 64)],
+    "prompts": [(70, 0), (1, 0), (200, 33), (0, 0), (129, 250)],
+    "mixed": [(150, 100), (1, 400), (3, 90), (260, 0), (1, 0)],
+}
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("q8_0", False), ("f32", False), ("f32", True)])
+def test_attention(ctx, K, kv, half, shape):
+    run = R.Run(SHAPES[shape], 8, 2, kv, seed=len(shape), spare_tokens=3)
+    got, untouched = attend(ctx, K, run, half)
+    want, tol = run.attention(half)
+    n = int(run.starts[-1])
+    check(got[:n], want[:n], tol[:n])
+    assert (got[n:] == untouched).all()  # rows behind the last sequence
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 1), (5, 1), (8, 1), (6, 2), (7, 7), (14, 2), (16, 8)])
+@pytest.mark.parametrize("kv,half", [("f16", True), ("q8_0", False), ("q8_0", True), ("f32", False)])
+def test_attention_head_layouts(ctx, K, kv, half, hq, hkv):
+    run = R.Run([(3, 70), (75, 20), (1, 200), (18, 0)], hq, hkv, kv, seed=hq)
+    want, tol = run.attention(half)
+    check(attend(ctx, K, run, half)[0], want, tol)
+
+
+@pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("f32", False)])
+def test_attention_large_scores(ctx, K, kv, half):
+    """Scores far apart: the running maximum moves often, and what it leaves underflows."""
+    run = R.Run([(2, 500), (140, 90)], 4, 2, kv, seed=9, scale=12.0)
+    want, tol = run.attention(half)
+    check(attend(ctx, K, run, half)[0], want, tol)
+
+
+@pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("f32", False)])
+def test_attention_positions_without_pages(ctx, K, kv, half):
+    """Pages that are none stand for positions that hold nothing; a row that sees nothing gives zeros."""
+    run = R.Run([(4, 60), (100, 150), (2, 20), (140, 0)], 4, 2, kv, seed=3)
+    run.table[0, 1], run.table[1, 0], run.table[1, 9], run.table[1, 15] = -1, run.num_pages, -7, 2 ** 31 - 1
+    run.table[2, :] = -1
+    run.table[3, :8] = -1
+    want, tol = run.attention(half)
+    got, _ = attend(ctx, K, run, half)
+    check(got, want, tol)
+    a, b = int(run.starts[2]), int(run.starts[3])
+    assert (got[a:b] == 0).all() and (got[b:b + 128] == 0).all()
+
+
+def test_attention_keeps_to_what_the_call_says(ctx, K):
+    """`longest` and `tokens` below what starts say, starts that fall, positions behind the table: such rows are left alone."""
+    run = R.Run([(3, 40), (150, 20), (2, 30)], 4, 2, "f16", seed=5)
+    want, tol = run.attention(True)
+    got, untouched = attend(ctx, K, run, True, longest=20)
+    check(got[:23], want[:23], tol[:23])
+    assert (got[23:153] == untouched).all()
+    check(got[153:], want[153:], tol[153:])
+    got, _ = attend(ctx, K, run, True, tokens=10)
+    check(got[:10], want[:10], tol[:10])
+    assert (got[10:] == untouched).all()
+    got, _ = attend(ctx, K, run, True, starts=[0, 3, 1, 155])
+    check(got[:1], want[:1], tol[:1])
+    run = R.Run([(20, 10)], 4, 2, "f16", seed=6)
+    want, tol = run.attention(True)
+    run.table, run.max_pages = np.ascontiguousarray(run.table[:, :1]), 1
+    got, _ = attend(ctx, K, run, True)
+    check(got[:6], want[:6], tol[:6])
+    assert (got[6:] == untouched).all()
+
+
+def test_attention_of_a_single_token_is_the_paged_one(ctx, K):
+    """One token per sequence: what brasa_k_decode_attention_paged gives, to the rounding of its sums."""
+    import brasa_b200 as B
+    run = R.Run([(1, 90), (1, 300), (1, 0)], 8, 2, "f16", seed=8)
+    dev = OnDevice(ctx, K, run)
+    o, o2 = ctx.buffer(3 * 8 * 512), ctx.buffer(3 * 8 * 512)
+    part = ctx.buffer(B.decode_partials_len(8, run.max_pages * 16) * 3 * 4)
+    go(ctx, lambda c: (K.attention_packed(c, dev.q, dev.paged, dev.packed, o, 8, 2, 1), K.decode_attention_paged(c, dev.q, dev.paged, part, o2, 8, 2)))
+    want, tol = run.attention(False)
+    check(o.download(np.float32).reshape(3, 8, 128).astype(np.float64), want, tol)
+    check(o2.download(np.float32).reshape(3, 8, 128).astype(np.float64), want, tol)
+    dev.free()
+
+
+def test_attention_long_cache(ctx, K):
+    """One drafting sequence behind 20 000 positions, and two short ones: work of one item over many blocks."""
+    run = R.Run([(4, 20000), (1, 3), (2, 500)], 4, 1, "f16", seed=10)
+    for half in (True, False):
+        want, tol = run.attention(half)
+        check(attend(ctx, K, run, half)[0], want, tol)
+
+
+def test_attention_many_sequences(ctx, K):
+    """More sequences than a warp has lanes, most without new tokens."""
+    g = np.random.default_rng(2)
+    seqs = [(int(n), int(p)) for n, p in zip(g.integers(0, 3, 1100) * (g.random(1100) < 0.2), g.integers(0, 40, 1100))]
+    seqs[0], seqs[500], seqs[-1] = (0, 5), (90, 7), (3, 2)
+    run = R.Run(seqs, 2, 1, "f16", seed=11, spare_tokens=1)
+    want, tol = run.attention(True)
+    got, untouched = attend(ctx, K, run, True)
+    check(got[:-1], want[:-1], tol[:-1])
+    assert (got[-1] == untouched).all()
+
+
+def test_attention_repeats_and_replays(B, ctx, K):
+    """The same bits again, and out of a recorded graph with new lengths and tables behind it."""
+    run, other = R.Run([(130, 40), (2, 300), (5, 90)], 8, 2, "f16", seed=12), R.Run([(100, 70), (30, 272), (7, 88)], 8, 2, "f16", seed=13)
+    assert run.tokens == other.tokens and run.max_pages >= other.max_pages
+    dev = OnDevice(ctx, K, run)
+    o = ctx.buffer(run.tokens * 8 * 256)
+    go(ctx, lambda c: K.attention_packed(c, dev.q, dev.paged, dev.packed, o, 8, 2, 0))
+    first = o.download(np.uint16)
+    graph = ctx.capture(lambda c: K.attention_packed(c, dev.q, dev.paged, dev.packed, o, 8, 2, 0))
+    for _ in range(2):
+        o.fill(0)
+        go(ctx, lambda c: graph.launch(c))
+        assert (o.download(np.uint16) == first).all()
+    table = np.zeros_like(run.table)
+    table[:, :other.max_pages] = other.table
+    big = other.num_pages <= run.num_pages
+    assert big
+    for buf, x in zip(dev.bufs, (other.k, other.v, table, other.lens, other.starts, other.q)):
+        buf.upload(x)
+    go(ctx, lambda c: graph.launch(c))
+    want, tol = other.attention(True)
+    check(o.download(np.float16).astype(np.float64).reshape(run.tokens, 8, 128), want, tol)
+    graph.free()
+    dev.free()
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (3, 1), (7, 7), (10, 2)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_store(B, ctx, K, kv, hq, hkv, in_place):
+    run = R.Run([(5, 30), (1, 0), (0, 9), (33, 15), (2, 4000)], hq, hkv, kv, seed=20, spare_tokens=2)
+    run.table[3, 1] = -1  # positions 16 to 31 of that sequence have no place
+    g = np.random.default_rng(21)
+    k, v = (g.standard_normal((run.tokens, hkv, 128)).astype(np.float32) * 3 for _ in range(2))
+    k[2], v[2] = 0, 0
+    qn, kn = (1 + 0.2 * g.standard_normal(128).astype(np.float32) for _ in range(2))
+    dev = OnDevice(ctx, K, run)
+    gk, gv, gqn, gkn = (ctx.buffer_from(x) for x in (k, v, qn, kn))
+    out = dev.q if in_place else ctx.buffer_from(np.full_like(run.q, 7.0))
+    table = B.RopeTable(ctx, THETA, 128, run.max_pages * 16)
+    go(ctx, lambda c: K.qk_norm_rope_store_packed(c, dev.q, gk, gv, gqn, gkn, EPS, table, dev.paged, dev.packed, out, hq, hkv))
+    got_q = out.download(np.float32).reshape(run.q.shape)
+    pools = [p.download(np.uint8).reshape(run.k.shape) for p in (dev.kpool, dev.vpool)]
+    want = [run.k.copy(), run.v.copy()]
+    written = np.zeros(run.k.shape[:2], bool)
+    for s, (n, past) in enumerate(run.seqs):
+        for j in range(n):
+            t, pos = int(run.starts[s]) + j, past + j
+            # 32-bit sums of 128 squares, a root, a product and two of the rotation, whose table is rounded to 2^-24: within 2^-20 of the row's largest
+            wq, wk = R.norm_rope(run.q[t], qn, EPS, THETA, pos), R.norm_rope(k[t], kn, EPS, THETA, pos)
+            assert np.abs(got_q[t] - wq).max() <= 2.0 ** -20 * np.abs(wq).max()
+            page = run.table[s, pos // 16]
+            if page < 0:
+                continue
+            written[page, pos % 16] = True
+            gotk, gotv = (R.from_bytes(p[page, pos % 16], kv) for p in pools)
+            # a rounding to the cache's type: half a step of the value, in 8 bits of the block's largest / 127 (and its scale's own rounding, 2^-11 of 127 steps)
+            for got, w, exact in ((gotk, wk, False), (gotv, v[t].astype(np.float64), True)):
+                block = np.repeat(np.abs(w).reshape(hkv, 4, 32).max(-1), 32, -1).reshape(hkv, 128)
+                step = {"f32": 2.0 ** -24 * np.abs(w), "f16": 2.0 ** -11 * np.abs(w) + 2.0 ** -25, "q8_0": (0.5 / 127 + 2.0 ** -11) * block + 2.0 ** -24}[kv]
+                assert (np.abs(got - w) <= step + (0 if exact else 2.0 ** -20) * block).all()
+    for got, was in zip(pools, want):
+        assert (got[~written] == was[~written]).all()
+    n = int(run.starts[-1])
+    assert (got_q[n:] == (run.q[n:] if in_place else 7.0)).all()
+
+
+def random_verify(g, seqs, drafts, vocab, q_given, empty=0.0):
+    n = [0 if g.random() < empty else int(g.integers(0, drafts + 1)) + 1 for _ in range(seqs)]
+    starts = np.concatenate([[0], np.cumsum(n)]).astype(np.uint32)
+    rows, nd = int(starts[-1]), int(sum(max(0, x - 1) for x in n))
+    p = g.dirichlet(np.full(vocab, 0.3), rows).astype(np.float32) if rows else np.zeros((0, vocab), np.float32)
+    q = g.dirichlet(np.full(vocab, 0.3), max(nd, 1)).astype(np.float32)
+    d = np.array([g.integers(0, vocab) if not q_given else np.argmax(np.cumsum(q[i]) > g.random() * 0.999) for i in range(nd)], np.uint32)
+    return p, q[:nd] if q_given else None, d, g.random(rows).astype(np.float32), starts
+
+
+def run_verify(ctx, K, p, q, d, u, starts, spare=2):
+    seqs, vocab, rows = len(starts) - 1, p.shape[1], len(p)
+    bufs = [ctx.buffer_from(x) if x is not None and x.size else ctx.buffer(16) for x in (p, q, d, u, starts)]
+    out, acc = ctx.buffer_from(np.full(rows + spare, 77, np.uint32)), ctx.buffer_from(np.full(seqs + 1, 77, np.uint32))
+    go(ctx, lambda c: K.verify_drafts(c, bufs[0], bufs[1] if q is not None else None, bufs[2], bufs[3], bufs[4], seqs, rows, vocab, out, acc))
+    got = out.download(np.uint32), acc.download(np.uint32)
+    for b in bufs + [out, acc]:
+        b.free()
+    want_t, want_a = np.full(rows + spare, 77, np.uint32), np.full(seqs + 1, 77, np.uint32)
+    R.verify(p, q, d, u, starts, want_t, want_a[:-1])
+    return got, (want_t, want_a)
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 31, 127, 1000, 4099, 40003])
+@pytest.mark.parametrize("given", [True, False])
+def test_verify(ctx, K, vocab, given):
+    g = np.random.default_rng(vocab)
+    for seqs, drafts, empty in ((1, 0, 0), (1, 5, 0), (9, 4, 0.3), (40 if vocab < 5000 else 5, 7, 0)):
+        case = random_verify(g, seqs, drafts, vocab, given, empty)
+        if len(case[0]):
+            got, want = run_verify(ctx, K, *case)
+            assert (got[1] == want[1]).all() and (got[0] == want[0]).all()
+
+
+def test_verify_odd_numbers(ctx, K):
+    """Entries that are no positive finite numbers, drafts outside the vocabulary, u at both ends, nothing left of p - q, nothing in p."""
+    V = 700
+    g = np.random.default_rng(1)
+    p, q = (g.dirichlet(np.full(V, 0.5), 14).astype(np.float32) for _ in range(2))
+    starts = np.array([0, 2, 4, 6, 8, 10, 12, 14], np.uint32)
+    d = g.integers(0, V, 7).astype(np.uint32)
+    u = g.random(14).astype(np.float32)
+    p[0, :50], p[0, 60], p[0, 61], p[0, 62] = np.nan, np.inf, -1.0, 0.0
+    u[0] = 0.9999999
+    d[1] = V
+    d[2] = 2 ** 32 - 1
+    q = q[:7].copy()
+    q[3] = 1.0  # more than p everywhere: refused, and nothing is left
+    u[6] = 0.9999999
+    p[8], p[9] = 0.0, 0.0
+    u[11], u[13] = 0.0, 0.99999994
+    p[12, d[6]] = 1.0
+    for qq in (q, None):
+        got, want = run_verify(ctx, K, p, qq, d, u, starts)
+        assert (got[1] == want[1]).all() and (got[0] == want[0]).all()
+    u[9], p[9, 5:9] = 1.0, 0.1  # a u that is no number below 1: the last id that has any mass
+    got, want = run_verify(ctx, K, p, None, d, u, starts)
+    assert (got[0] == want[0]).all()
+
+
+def test_verify_draws_as_the_target_does(ctx, K):
+    """First tokens of 20 000 verified drafts are distributed as p: each frequency within five standard deviations."""
+    g = np.random.default_rng(4)
+    n, V = 20000, 6
+    p1, q1 = np.array([0.35, 0.05, 0.2, 0.3, 0.1, 0.0], np.float32), np.array([0.1, 0.3, 0.2, 0.05, 0.15, 0.2], np.float32)
+    p, q = np.tile(p1, (2 * n, 1)), np.tile(q1, (n, 1))
+    d = g.choice(V, n, p=q1 / q1.sum()).astype(np.uint32)
+    (tokens, acc), want = run_verify(ctx, K, p, q, d, g.random(2 * n).astype(np.float32), np.arange(0, 2 * n + 1, 2).astype(np.uint32))
+    assert (tokens == want[0]).all() and (acc == want[1]).all()
+    share = np.bincount(tokens[0:2 * n:2], minlength=V) / n
+    assert (np.abs(share - p1) <= 5 * np.sqrt(p1 * (1 - p1) / n) + 1e-9).all()
+
+
+class Pages:
+    def __init__(self, g, rows, max_pages, num_pages, layers, hkv, kv, fill):
+        self.layers, self.hkv, self.kv = layers, hkv, kv
+        self.num_pages = num_pages
+        self.table = np.full((rows, max_pages), -1, np.int32)
+        self.lens = np.zeros(rows, np.uint32)
+        free = list(g.permutation(num_pages))
+        for r in range(rows):
+            n = int(g.integers(0, max_pages * 16 + 1) * fill)
+            c = -(-n // 16)
+            if c <= len(free):
+                self.table[r, :c] = [free.pop() for _ in range(c)]
+                self.lens[r] = n
+        self.pinned = (g.random(num_pages) < 0.05).astype(np.uint32)
+        shape = (layers, num_pages, 16, hkv, R.ROW[kv])
+        self.k, self.v = (g.integers(0, 256, shape, dtype=np.uint8) for _ in range(2))
+
+    def device(self, ctx, K, pinned=True):
+        self.bufs = [ctx.buffer_from(x) for x in (self.k, self.v, self.table, self.lens, self.pinned)]
+        return K.page_pool(*self.bufs[:4], self.bufs[4] if pinned else None, *self.table.shape, self.num_pages, self.layers, self.hkv, KV[self.kv])
+
+
+def run_reassign(ctx, K, P, source, keep, room, pinned=True, accepted=None):
+    pool = P.device(ctx, K, pinned)
+    ins = [None if x is None else ctx.buffer_from(np.array(x, t)) for x, t in ((source, np.int32), (keep, np.uint32), (room, np.uint32), (accepted, np.uint32))]
+    outs = [ctx.buffer_from(np.full_like(P.table, 99)), ctx.buffer_from(np.full_like(P.lens, 99)), ctx.buffer(16)]
+    go(ctx, lambda c: K.pages_reassign(c, pool, *ins[:3], *outs, accepted=ins[3]))
+    got = outs[0].download(np.int32).reshape(P.table.shape), outs[1].download(np.uint32), outs[2].download(np.uint32)
+    pools = [b.download(np.uint8).reshape(P.k.shape) for b in P.bufs[:2]]
+    for b in P.bufs + [x for x in ins if x] + outs:
+        b.free()
+    table, lens, result, copies = R.reassign(P.table, P.lens, P.pinned if pinned else None, P.num_pages, source, keep, room, accepted)
+    assert list(got[2]) == result
+    assert (got[1] == lens).all() and (got[0] == table).all()
+    for have, was in zip(pools, (P.k, P.v)):
+        want = was.copy()
+        for a, b in copies:
+            want[:, b] = was[:, a]
+        assert (have == want).all()
+    return table, lens, result
+
+
+@pytest.mark.parametrize("rows,max_pages,num_pages,layers,hkv,kv", [(1, 1, 1, 1, 1, "f16"), (4, 5, 40, 2, 2, "q8_0"), (33, 9, 700, 1, 1, "f32"), (7, 40, 900, 3, 1, "f16"),
+                                                                  (70, 3, 60, 1, 3, "q8_0"), (1500, 2, 5000, 1, 1, "q8_0")])
+def test_reassign(ctx, K, rows, max_pages, num_pages, layers, hkv, kv):
+    g = np.random.default_rng(rows)
+    P = Pages(g, rows, max_pages, num_pages, layers, hkv, kv, 0.6)
+    most = max_pages * 16
+    same = np.arange(rows)
+    seen_short = False
+    for source, keep, room in (
+            (same, P.lens, np.zeros(rows)),                                          # nothing changes
+            (same, P.lens, g.integers(0, 40, rows)),                                 # room to go on
+            (same, g.integers(0, most + 1, rows), np.full(rows, 3)),                 # rolled back
+            (g.integers(0, rows, rows), np.full(rows, most), np.full(rows, 1)),      # beams: rows of any row
+            (np.zeros(rows), np.full(rows, P.lens[0]), g.integers(0, 20, rows)),     # all of the first
+            (g.integers(-2, rows + 2, rows), g.integers(0, most + 1, rows), g.integers(0, most, rows)),
+            (np.full(rows, -1), np.full(rows, most), np.zeros(rows)),                # all given back
+            (same, np.full(rows, 2 ** 32 - 1), np.full(rows, 2 ** 32 - 1))):         # as much as the table holds
+        result = run_reassign(ctx, K, P, source.astype(np.int64), keep.astype(np.int64), room.astype(np.int64), pinned=rows != 7)[2]
+        seen_short |= result[3] > 0
+    assert seen_short or rows != 70
+    got = g.integers(0, 9, rows)
+    run_reassign(ctx, K, P, same, None, np.full(rows, 4), accepted=got)
+    run_reassign(ctx, K, P, same[::-1], P.lens.astype(np.int64) + 3, np.full(rows, 4), accepted=got)
+    run_reassign(ctx, K, P, same, None, np.zeros(rows), pinned=False)
+
+
+def test_reassign_pages_held_more_than_once(ctx, K):
+    """Rows that share pages already: the last page of one row is a whole page of another, or pinned, or named twice; entries that are no pages."""
+    g = np.random.default_rng(0)
+    P = Pages(g, 6, 4, 30, 2, 1, "f16", 0)
+    P.table[:] = [[3, 4, 5, -1], [3, 4, -1, -1], [3, 9, -1, -1], [7, -5, 8, -1], [2, 2, -1, -1], [40, 6, 11, -1]]
+    P.lens[:] = [40, 24, 20, 41, 30, 40]
+    P.pinned[:] = 0
+    P.pinned[9] = 1
+    run_reassign(ctx, K, P, np.arange(6), P.lens.astype(np.int64), np.full(6, 7))
+    run_reassign(ctx, K, P, [0, 0, 2, 2, 3, 5], [40, 33, 20, 17, 20, 5], [0, 30, 1, 0, 5, 17])
+
+
+@pytest.mark.parametrize("rows,max_pages,num_pages,layers,hkv,kv", [(1, 1, 1, 1, 1, "f16"), (4, 5, 40, 2, 2, "q8_0"), (33, 9, 1500, 1, 1, "f32"), (7, 40, 200, 3, 1, "f16"),
+                                                                  (20, 300, 40000, 1, 1, "q8_0")])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_compact(ctx, K, rows, max_pages, num_pages, layers, hkv, kv, in_place):
+    g = np.random.default_rng(rows + 1)
+    P = Pages(g, rows, max_pages, num_pages, layers, hkv, kv, 0.4)
+    P.table[rows // 2] = P.table[0]  # shared pages
+    P.table[0, -1] = num_pages + 3
+    for pinned in (True, False):
+        pool = P.device(ctx, K, pinned)
+        out, moved, result = ctx.buffer(P.table.nbytes), ctx.buffer(num_pages * 4), ctx.buffer(16)
+        go(ctx, lambda c: K.pages_compact(c, pool, P.bufs[2] if in_place else out, moved, result))
+        table, want_moved, want_result, moves = R.compact(P.table, P.pinned if pinned else None, num_pages)
+        assert list(result.download(np.uint32)) == want_result
+        assert (moved.download(np.int32) == want_moved).all()
+        assert ((P.bufs[2] if in_place else out).download(np.int32).reshape(table.shape) == table).all()
+        for b, was in zip(P.bufs[:2], (P.k, P.v)):
+            want = was.copy()
+            for a, to in moves:
+                want[:, to] = was[:, a]
+            assert (b.download(np.uint8).reshape(was.shape) == want).all()
+        for b in P.bufs + [out, moved, result]:
+            b.free()
+
+
+def test_refusals(B, ctx, K):
+    """Every precondition comes back as EINVAL, with nothing launched."""
+    run = R.Run([(2, 20), (1, 3)], 4, 2, "f16")
+    dev = OnDevice(ctx, K, run)
+    k, v, t, n, s, q = dev.bufs
+    o, small, w = ctx.buffer(run.tokens * 4 * 512), ctx.buffer(16), ctx.buffer(512)
+    rope = B.RopeTable(ctx, THETA, 128, run.max_pages * 16)
+    kv2, run2 = ctx.buffer(run.tokens * 2 * 512), dev.packed
+
+    def paged(**kw):
+        a = dict(kpool=k, vpool=v, table=t, lens=n, seqs=2, max_pages=run.max_pages, num_pages=run.num_pages, kv=1) | kw
+        return K.paged_kv(*a.values())
+
+    def store(c, paged=dev.paged, packed=run2, q=q, k=kv2, out=o, norm=w, rope=rope, hq=4, hkv=2):
+        K.qk_norm_rope_store_packed(c, q, k, kv2, norm, w, EPS, rope, paged, packed, out, hq, hkv)
+
+    def att(c, paged=dev.paged, packed=run2, q=q, o=o, hq=4, hkv=2, precision=0):
+        K.attention_packed(c, q, paged, packed, o, hq, hkv, precision)
+    short = B.RopeTable(ctx, THETA, 128, 16)
+    f = {x: ctx.buffer(4096) for x in "pquds"}
+
+    def ver(c, p=f["p"], q=f["q"], d=f["d"], u=f["u"], st=f["s"], seqs=2, rows=4, vocab=100, out=f["d"], acc=f["u"]):
+        K.verify_drafts(c, p, q, d, u, st, seqs, rows, vocab, out, acc)
+    kp = ctx.buffer(2 * 8 * 16 * 256)
+    tb, tb2, ln, ln2, pins = ctx.buffer(4 * 3 * 4), ctx.buffer(4 * 3 * 4), ctx.buffer(16), ctx.buffer(16), ctx.buffer(32)
+
+    def pool(**kw):
+        a = dict(kpool=kp, vpool=kp, table=tb, lens=ln, pinned=pins, rows=4, max_pages=3, num_pages=8, layers=2, hkv=1, kv=1) | kw
+        return K.page_pool(*a.values())
+    src, keep, room, res, moved = (ctx.buffer(32) for _ in range(5))
+
+    def rea(c, pool=pool(), source=src, keep=keep, acc=None, out=tb2, lens_out=ln2, result=res):
+        K.pages_reassign(c, pool, source, keep, room, out, lens_out, result, accepted=acc)
+
+    def com(c, pool=pool(), out=tb2, moved=moved, result=res):
+        K.pages_compact(c, pool, out, moved, result)
+    for f_ok in (store, att, ver, rea, com):
+        go(ctx, f_ok)
+    before = ctx.launch_count()
+    bad = [(store, dict(paged=paged(num_pages=run.num_pages + 1))), (store, dict(paged=paged(kv=3))), (store, dict(paged=paged(seqs=0))), (store, dict(paged=paged(table=small))),
+           (store, dict(packed=K.packed_run(s, 0, 2))), (store, dict(packed=K.packed_run(s, run.tokens, 0))),
+           (store, dict(packed=K.packed_run(s.at(8), run.tokens, 2))), (store, dict(packed=K.packed_run(s.at(2), run.tokens, 2))), (store, dict(packed=K.packed_run(s, run.tokens + 1, 2))),
+           (store, dict(q=small)), (store, dict(q=None)), (store, dict(k=small)), (store, dict(out=small)), (store, dict(out=o.at(4))), (store, dict(norm=small)), (store, dict(rope=short)),
+           (store, dict(hq=0)), (store, dict(hkv=0)), (store, dict(hq=5)), (store, dict(hq=18, hkv=2)),
+           (att, dict(paged=paged(lens=small.at(12)))), (att, dict(packed=K.packed_run(s, run.tokens + 9, 2))), (att, dict(q=small)), (att, dict(o=small)), (att, dict(o=o.at(8))),
+           (att, dict(precision=2)), (att, dict(precision=-1)), (att, dict(hq=0)), (att, dict(hq=3)),
+           (ver, dict(seqs=0)), (ver, dict(rows=0)), (ver, dict(vocab=0)), (ver, dict(rows=12)), (ver, dict(vocab=300)), (ver, dict(d=small.at(12))), (ver, dict(u=small.at(4))),
+           (ver, dict(st=small.at(8))), (ver, dict(out=small.at(4))), (ver, dict(acc=small.at(12))), (ver, dict(p=f["p"].at(2))), (ver, dict(p=None)), (ver, dict(seqs=2 ** 30)),
+           (rea, dict(pool=pool(kv=3))), (rea, dict(pool=pool(rows=0))), (rea, dict(pool=pool(layers=3))), (rea, dict(pool=pool(max_pages=4))), (rea, dict(pool=pool(num_pages=2 ** 19 + 1))),
+           (rea, dict(pool=pool(rows=65537))), (rea, dict(pool=pool(pinned=small))), (rea, dict(pool=pool(kpool=kp.at(8)))), (rea, dict(source=small.at(4))), (rea, dict(source=None)), (rea, dict(acc=small.at(4))), (rea, dict(keep=small.at(4))),
+           (rea, dict(out=tb)), (rea, dict(out=tb2.at(4))), (rea, dict(lens_out=ln)), (rea, dict(result=ln)), (rea, dict(result=small.at(4))),
+           (com, dict(pool=pool(hkv=0))), (com, dict(moved=small)), (com, dict(moved=tb)), (com, dict(moved=pins)), (com, dict(out=small)), (com, dict(result=pins)), (com, dict(out=pins))]
+    for call, kw in bad:
+        with pytest.raises(B.BrasaError) as e:
+            go(ctx, lambda c: call(c, **kw))
+        assert e.value.code == B.EINVAL, (call.__name__, kw)
+    assert ctx.launch_count() == before
+
+
+@pytest.mark.parametrize("kv", ["f16", "q8_0"])
+def test_a_decoding_loop_with_drafts(B, ctx, K, kv):
+    """Two layers' caches through steps of drafting, verification, rollback and forks, as a program drives them; every attention against a cache that is
+    kept densely on the host, in the values that the pool gives back."""
+    g = np.random.default_rng(30)
+    rows, max_pages, num_pages, layers, hq, hkv, V = 5, 12, 70, 2, 8, 2, 300
+    half = True
+    shape = (layers, num_pages, 16, hkv, R.ROW[kv])
+    pools = [ctx.buffer_from(np.full(shape, 0xFF, np.uint8)) for _ in range(2)]
+    layer_bytes = int(np.prod(shape[1:]))
+    tables, lens = [ctx.buffer_from(np.full((rows, max_pages), -1, np.int32)) for _ in range(2)], [ctx.buffer(rows * 4) for _ in range(2)]
+    rope = B.RopeTable(ctx, THETA, 128, max_pages * 16)
+    norm = ctx.buffer_from(np.ones(128, np.float32))
+    result = ctx.buffer(16)
+    dense = [[[np.zeros((0, hkv, 128)) for _ in range(2)] for _ in range(layers)] for _ in range(rows)]  # [row][layer][k, v]
+    source, keep, acc, now = np.arange(rows), np.zeros(rows, int), np.zeros(rows, int), 0
+    for step in range(7):
+        new = [int(g.integers(1, 6)) if step else int(g.integers(10, 60)) for _ in range(rows)]
+        if step == 3:
+            source = np.array([0, 0, 2, 2, 2])
+            keep = keep[source]
+        ins = [ctx.buffer_from(np.array(x, t)) for x, t in ((source, np.int32), (new, np.uint32), (acc, np.uint32))]
+        pool = K.page_pool(*pools, tables[now], lens[now], None, rows, max_pages, num_pages, layers, hkv, KV[kv])
+        go(ctx, lambda c: K.pages_reassign(c, pool, ins[0], None, ins[1], tables[1 - now], lens[1 - now], result, accepted=ins[2] if step else None))
+        now = 1 - now
+        assert result.download(np.uint32)[3] == 0 and (lens[now].download(np.uint32) == keep).all()
+        dense = [[[x[:keep[r]] for x in dense[source[r]][li]] for li in range(layers)] for r in range(rows)]
+        starts = np.concatenate([[0], np.cumsum(new)]).astype(np.uint32)
+        T = int(starts[-1])
+        run = K.packed_run(ctx.buffer_from(starts), T, max(new))
+        table = tables[now].download(np.int32).reshape(rows, max_pages)
+        for li in range(layers):
+            paged = K.paged_kv(pools[0].at(li * layer_bytes), pools[1].at(li * layer_bytes), tables[now], lens[now], rows, max_pages, num_pages, KV[kv])
+            q, k, v = (g.standard_normal((T, h, 128)).astype(np.float32) for h in (hq, hkv, hkv))
+            gq, gk, gv, o = ctx.buffer_from(q), ctx.buffer_from(k), ctx.buffer_from(v), ctx.buffer(T * hq * 256)
+
+            def layer(c):
+                K.qk_norm_rope_store_packed(c, gq, gk, gv, norm, norm, EPS, rope, paged, run, gq, hq, hkv)
+                K.attention_packed(c, gq, paged, run, o, hq, hkv, 0)
+            go(ctx, layer)
+            got = o.download(np.float16).astype(np.float64).reshape(T, hq, 128)
+            raw = [p.download(np.uint8, layer_bytes, li * layer_bytes).reshape(shape[1:]) for p in pools]
+            for r in range(rows):
+                at = [(table[r, i // 16], i % 16) for i in range(keep[r] + new[r])]
+                for w, pool_rows in enumerate(raw):
+                    have = np.stack([R.from_bytes(pool_rows[a], kv) for a in at])
+                    assert (have[:keep[r]] == dense[r][li][w]).all(), (step, li, r)  # what is kept is what was there
+                    dense[r][li][w] = have
+                ref = R.Run([(new[r], int(keep[r]))], hq, hkv, "f32")
+                ref.q = np.stack([R.norm_rope(q[starts[r] + j], np.ones(128), EPS, THETA, keep[r] + j) for j in range(new[r])])
+                pages = [R.to_bytes(np.concatenate([x, np.zeros((-len(x) % 16, hkv, 128))]).reshape(-1, 16, hkv, 128).astype(np.float32), "f32") for x in dense[r][li]]
+                ref.k, ref.v, ref.num_pages = *pages, len(pages[0])
+                ref.table[0, :len(pages[0])] = np.arange(len(pages[0]))
+                want, tol = ref.attention(half)
+                check(got[starts[r]:starts[r + 1]], want, tol + 2.0 ** -18)  # (and q's own rounding to 32 bits)
+        p = g.dirichlet(np.full(V, 0.2), T).astype(np.float32)
+        nd = T - rows
+        drafts = np.array([np.argmax(p[i]) for r in range(rows) for i in range(starts[r], starts[r + 1] - 1)], np.uint32)
+        (tokens, taken), want = run_verify(ctx, K, p, None, drafts, (0.3 * g.random(T)).astype(np.float32), starts, spare=0)
+        assert (tokens == want[0]).all() and (taken == want[1]).all() and len(drafts) == nd
+        acc = taken[:rows].astype(int)
+        source, keep = np.arange(rows), keep + acc + 1
+    assert keep.max() <= max_pages * 16
