@@ -50,6 +50,8 @@ struct brasa_ctx {
     float *gemm_part = nullptr;      // partial output tiles of the split-K tensor-core GEMM
     size_t gemm_part_bytes = 0;
     uint32_t *gemm_counters = nullptr;  // arrivals per output tile of that GEMM (GEMM_TC_COUNTERS words, zero between launches)
+    uint8_t *packed_work = nullptr;     // partial results of the packed attention, and what they belong to
+    size_t packed_work_bytes = 0;
     uint8_t *page_work = nullptr;       // flags, free list and copy list of the page operators
     size_t page_work_bytes = 0;
     bool recorded = false;              // a graph has been recorded: its kernels may hold the address of any workspace there was

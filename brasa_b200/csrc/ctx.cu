@@ -96,6 +96,7 @@ void brasa_ctx_destroy(brasa_ctx *ctx) {
     cudaFree(ctx->gemm_part);
     cudaFree(ctx->flash_part);
     cudaFree(ctx->kv_expand);
+    cudaFree(ctx->packed_work);
     cudaFree(ctx->page_work);
     cudaFree(ctx->gemm_counters);
     for (void *p : ctx->outgrown) cudaFree(p);

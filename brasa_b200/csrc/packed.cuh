@@ -44,4 +44,142 @@ __device__ __forceinline__ int32_t packed_page(const PackedView &p, uint32_t seq
     return (uint32_t)page < p.num_pages ? page : -1;
 }
 
+// ---- the work of a run in a line, cut evenly ----
+// An item is up to rows_item rows (token by token, of one token the heads of a key head's group) of one sequence against one key head.
+// In the line an item takes `start` units for its beginning and end and one per `tile` keys that its last row sees. Equal pieces of the line
+// go to the blocks; a block works through the items of its piece, whole ones and parts. A piece's end that falls within `snap` units of an
+// item's ends moves there, since a part costs a way through memory and a merge. Everything is read from device memory, so that a recorded
+// launch follows new lengths.
+struct PackedLine {
+    PackedView v;
+    uint32_t group, rows_item, tile, start, snap, least;  // query heads per key head; ..; fewest units that are worth a block
+    uint32_t min_rows, max_rows;                          // sequences of fewer or more rows are another kernel's
+};
+struct PackedItem {
+    uint64_t first;                // its place in the line
+    uint32_t seq, t0, rows, past;  // sequence, its first row of the run, its rows, the positions before them
+    uint32_t part, kh, tiles;      // which rows_item of its rows, key head, key tiles
+    uint32_t j;                    // the key tile that a piece begins or ends at
+};
+
+__device__ __forceinline__ void line_sequence(const PackedLine &l, uint32_t s, PackedItem &it) {
+    const uint32_t a = min(l.v.starts[s], l.v.tokens), b = min(l.v.starts[s + 1], l.v.tokens);
+    const uint64_t most = (uint64_t)l.v.max_pages * BRASA_KV_PAGE, past = l.v.lens[s];
+    uint64_t n = min(b > a ? b - a : 0u, l.v.longest);
+    n = past >= most ? 0 : min(n, most - past);
+    const uint64_t rows = n * l.group;
+    it.seq = s;
+    it.t0 = a;
+    it.past = (uint32_t)past;
+    it.rows = rows >= l.min_rows && rows <= l.max_rows ? (uint32_t)rows : 0u;
+}
+__device__ __forceinline__ uint32_t line_keys(const PackedLine &l, const PackedItem &it, uint32_t part) {  // that a part's last row sees
+    return it.past + (min((part + 1) * l.rows_item, it.rows) - 1) / l.group + 1;
+}
+__device__ __forceinline__ uint32_t line_tiles(const PackedLine &l, const PackedItem &it, uint32_t part) { return (line_keys(l, it, part) - 1) / l.tile + 1; }
+__device__ __forceinline__ uint64_t line_units(const PackedLine &l, const PackedItem &it) {
+    uint64_t u = 0;
+    for (uint32_t p = 0; p * l.rows_item < it.rows; ++p) u += (uint64_t)l.v.hkv * (l.start + line_tiles(l, it, p));
+    return u;
+}
+
+// What a block leaves of the items at its piece's ends, for the kernel that adds parts up.
+struct PackedNote {
+    uint32_t opens;         // the piece began an item and left it open: the rest of the note is about that item
+    uint32_t closes;        // the piece ended an item that began before it
+    uint32_t t0, g0, rows;  // first row of the run, head of the group at its first row, rows
+    uint32_t kh;
+};
+// floats of a part's slot: O [rows_item][128], m and l by row
+__host__ __device__ constexpr size_t packed_part_floats(uint32_t rows_item) { return (size_t)rows_item * 130; }
+
+struct PackedPieces {
+    uint64_t sums[32], total;
+    PackedItem at[2];  // where this block's piece begins and ends
+    uint32_t pieces;   // how many there are
+};
+// All threads of the block (a multiple of 32). False when this block has no piece.
+template <uint32_t THREADS>
+__device__ bool line_cut(const PackedLine &l, PackedPieces &w) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid >= THREADS) {  // (more threads than take part: they only keep the barriers company)
+        for (int i = 0; i < 3; ++i) __syncthreads();
+        return blockIdx.x < w.pieces;
+    }
+    const uint32_t each = (l.v.seqs + THREADS - 1) / THREADS, s0 = min(tid * each, l.v.seqs), s1 = min(s0 + each, l.v.seqs);
+    PackedItem it;
+    uint64_t mine = 0;
+    for (uint32_t s = s0; s < s1; ++s) {
+        line_sequence(l, s, it);
+        mine += line_units(l, it);
+    }
+    uint64_t upto = mine;
+    for (uint32_t x = 1; x < 32; x <<= 1) {
+        const uint64_t o = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += o;
+    }
+    if (lane == 31) w.sums[warp] = upto;
+    __syncthreads();
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < THREADS / 32; ++i) {
+        if (i == warp) upto += total;
+        total += w.sums[i];
+    }
+    const uint32_t pieces = (uint32_t)min((uint64_t)gridDim.x, (total + l.least - 1) / l.least);
+    if (tid == 0) {
+        w.total = total;
+        w.pieces = pieces;
+        w.at[1].first = total;  // (unless the line goes on there)
+        w.at[1].j = 0;
+    }
+    __syncthreads();
+    if (blockIdx.x < pieces) {
+        for (uint32_t e = 0; e < 2; ++e) {
+            const uint64_t unit = total * (blockIdx.x + e) / pieces;
+            if (unit < upto - mine || unit >= upto) continue;
+            uint64_t first = upto - mine;
+            uint32_t s = s0;
+            for (;; ++s) {  // (ends: the unit lies in one of this thread's sequences)
+                line_sequence(l, s, it);
+                const uint64_t u = line_units(l, it);
+                if (unit < first + u) break;
+                first += u;
+            }
+            it.part = 0;
+            uint32_t tiles = line_tiles(l, it, 0);
+            while (unit >= first + (uint64_t)l.v.hkv * (l.start + tiles)) {
+                first += (uint64_t)l.v.hkv * (l.start + tiles);
+                tiles = line_tiles(l, it, ++it.part);
+            }
+            const uint32_t each_item = l.start + tiles;
+            it.kh = (uint32_t)((unit - first) / each_item);
+            it.first = first + (uint64_t)it.kh * each_item;
+            it.tiles = tiles;
+            const uint32_t off = (uint32_t)(unit - it.first);
+            it.j = off > l.start ? off - l.start : 0u;
+            if (it.j < l.snap) it.j = 0;
+            else if (tiles - it.j < l.snap) it.j = tiles;  // (as far as the item goes: the next piece begins behind it)
+            w.at[e] = it;
+        }
+    }
+    __syncthreads();
+    return blockIdx.x < pieces;
+}
+// The item behind `it`; false at the end of the line.
+__device__ __forceinline__ bool line_next(const PackedLine &l, PackedItem &it) {
+    it.first += l.start + it.tiles;
+    it.j = 0;
+    if (++it.kh < l.v.hkv) return true;
+    it.kh = 0;
+    if (++it.part * l.rows_item >= it.rows) {
+        it.part = 0;
+        do {
+            if (++it.seq >= l.v.seqs) return false;
+            line_sequence(l, it.seq, it);
+        } while (it.rows == 0);
+    }
+    it.tiles = line_tiles(l, it, it.part);
+    return true;
+}
+
 }  // namespace brasa_dev

@@ -450,8 +450,8 @@ typedef struct brasa_packed_run {
 int32_t brasa_k_qk_norm_rope_store_packed(brasa_cmd *cmd, brasa_arg q, brasa_arg k, brasa_arg v, brasa_arg q_norm, brasa_arg k_norm, brasa_arg rope_cos,
                                           brasa_arg rope_sin, float eps, brasa_paged_kv paged, brasa_packed_run run, brasa_arg q_out, uint32_t hq, uint32_t hkv);
 /* Causal attention of the run's tokens: a token attends to the positions of its sequence up to its own, which the call before it has
- * stored. q f32 [tokens][hq][128]; precision F16: o f16 [tokens][hq][128], q * scale rounded to f16, as brasa_k_flash_attention; F32:
- * o f32, nothing rounded but the sums. Cache rows that a sequence has not reached may hold anything, infinities and NaN included. A token
+ * stored. q f32 [tokens][hq][128]; precision F16: o f16 [tokens][hq][128], q * scale, the weights and an 8-bit cache's
+ * values rounded to f16, sums in 32 bits; F32: o f32, 32-bit arithmetic. Cache rows that a sequence has not reached may hold anything, infinities and NaN included. A token
  * that sees no position gives zeros. */
 int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv paged, brasa_packed_run run, brasa_arg o, uint32_t hq, uint32_t hkv, int32_t precision);
 /* Verification of drafted tokens. Sequence s has rows starts[s] .. starts[s + 1] - 1 (u32 [seqs + 1], not falling, at most `rows`) of p

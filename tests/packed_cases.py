@@ -62,9 +62,11 @@ class Run:
                 out[i], there[i] = from_bytes(pool[page, i % PAGE], self.kv), True
         return out, there
 
-    def attention(self, half):
+    def attention(self, half, kv=None):
         """o in 64 bits, and how far a result may be off. With s the scores, o = sum p v: do = sum p ds (v - o) to first order, and
-        half: q rounded to f16, 2^-11 of every factor, independent (six standard deviations of the sum); P to f16, 2^-11 of each; o to f16.
+        kv: the cache that the rows came from, if not this one.
+        half: q rounded to f16, 2^-11 of every factor, independent (six standard deviations of the sum); P to f16, 2^-11 of each; o to f16; an
+        8-bit cache's rows, whose values d * code have up to 19 bits, to f16 as well.
         both: sums of 128 terms in 32 bits, where a tensor core may cut instead of round, and products of terms of 2^-22: 2^-22 * 130 of sum |q k|;
         sums over the keys and the exponentials, 2^-22 * (keys + 8) of sum p |v|."""
         out, tol = np.zeros((self.tokens, self.hq, D)), np.zeros((self.tokens, self.hq, D))
@@ -88,6 +90,8 @@ class Run:
                     e = ds * spread + 2.0 ** -22 * (len(p) + 8) * (p @ np.abs(vv))
                     if half:
                         dq = 6 * 2.0 ** -11 / np.sqrt(3) * np.sqrt((kk ** 2) @ (qq ** 2)).max() / np.sqrt(D)
+                        if (kv or self.kv) == "q8_0":  # k too, independent of q: the root of two; v: 2^-11 of each, sum p |v| of them at most
+                            dq, e = dq * np.sqrt(2), e + 2.0 ** -11 * (p @ np.abs(vv))
                         e = e + (dq + 2.0 ** -11) * spread + 2.0 ** -11 * np.abs(o) + 2.0 ** -24
                     out[t, h], tol[t, h] = o, e
         return out, tol

@@ -536,7 +536,7 @@ def test_a_decoding_loop_with_drafts(B, ctx, K, kv):
                 pages = [R.to_bytes(np.concatenate([x, np.zeros((-len(x) % 16, hkv, 128))]).reshape(-1, 16, hkv, 128).astype(np.float32), "f32") for x in dense[r][li]]
                 ref.k, ref.v, ref.num_pages = *pages, len(pages[0])
                 ref.table[0, :len(pages[0])] = np.arange(len(pages[0]))
-                want, tol = ref.attention(half)
+                want, tol = ref.attention(half, kv)
                 check(got[starts[r]:starts[r + 1]], want, tol + 2.0 ** -18)  # (and q's own rounding to 32 bits)
         p = g.dirichlet(np.full(V, 0.2), T).astype(np.float32)
         nd = T - rows
