@@ -1,7 +1,7 @@
 // Norm, RoPE and store, and attention, of a packed run: any number of new tokens per sequence over the paged pool.
 #include <math.h>
 
-#include "packed.cuh"
+#include "packed_tc.h"
 
 using namespace brasa_dev;
 
@@ -556,20 +556,32 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
     BRASA_REQUIRE(ctx, (uint64_t)run.tokens * (hq / hkv) < 1ull << 31, "attention_packed: more than 2^31 rows of a key head's group");
     const float scale = 1.0f / sqrtf((float)D);
     if (pg.kv == BRASA_KV_F16 || (pg.kv == BRASA_KV_Q8_0 && half)) {
-        const uint32_t per_sm = 2, blocks = ctx->sm_count * per_sm;
-        const size_t parts = 2 * (size_t)blocks * packed_part_floats(FEW_ROWS) * sizeof(float);
-        BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, parts + blocks * sizeof(PackedNote)));
-        FewParams f{{p, hq / hkv, FEW_ROWS, FEW_KEYS, 1, 1, 3, 1, UINT32_MAX}, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), (float *)ctx->packed_work,
-                    (PackedNote *)(ctx->packed_work + parts), hq, scale};
+        // Sequences of many rows go to the tensor-core kernel where there is one (16-bit products of an f16 pool) and the call can have any.
+        const uint32_t G = hq / hkv, sms = ctx->sm_count, blocks = sms * 2;
+        const bool tc = half && pg.kv == BRASA_KV_F16 && (uint64_t)run.longest * G >= PACKED_TC_MIN_ROWS && (uint64_t)pg.num_pages * PAGE < 1ull << 31;
+        // the workspace: parts of either kernel's items, then what they belong to
+        const size_t few_floats = 2 * (size_t)blocks * packed_part_floats(FEW_ROWS), tc_floats = 2 * (size_t)sms * packed_part_floats(PACKED_TC_ROWS);
+        BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, (few_floats + tc_floats) * sizeof(float) + (blocks + sms) * sizeof(PackedNote)));
+        float *few_part = (float *)ctx->packed_work, *tc_part = few_part + few_floats;
+        PackedNote *few_notes = (PackedNote *)(tc_part + tc_floats), *tc_notes = few_notes + blocks;
+        auto merge = [&](const float *part, const PackedNote *notes, uint32_t pieces, uint32_t rows_item) {
+            BRASA_CUDA(ctx, brasa_launch_dependent(ctx, half ? attn_packed_merge_kernel<true> : attn_packed_merge_kernel<false>, dim3(pieces, rows_item / 64), dim3(256), 0, part, notes,
+                                                   (void *)arg_ptr(o), hq, G, rows_item));
+            return brasa_post_launch(cmd, "attn_packed_merge");
+        };
+        if (tc) {
+            BRASA_TRY(brasa_packed_tc_launch(cmd, p, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), tc_part, tc_notes, hq, scale));
+            BRASA_TRY(merge(tc_part, tc_notes, sms, PACKED_TC_ROWS));
+        }
+        FewParams f{{p, G, FEW_ROWS, FEW_KEYS, 1, 1, 3, 1, tc ? PACKED_TC_MIN_ROWS - 1 : UINT32_MAX}, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), few_part,
+                    few_notes, hq, scale};
         void (*const kernel)(FewParams) = pg.kv == BRASA_KV_Q8_0 ? attn_packed_few_kernel<BRASA_KV_Q8_0, true>
                                           : half ? attn_packed_few_kernel<BRASA_KV_F16, true> : attn_packed_few_kernel<BRASA_KV_F16, false>;
         const size_t smem = pg.kv == BRASA_KV_Q8_0 ? FewStage<BRASA_KV_Q8_0>::STAGES * few_stage_bytes<BRASA_KV_Q8_0>() : FewStage<BRASA_KV_F16>::STAGES * few_stage_bytes<BRASA_KV_F16>();
         BRASA_TRY(brasa_smem_optin(ctx, (const void *)kernel, smem));
         BRASA_CUDA(ctx, brasa_launch_dependent(ctx, kernel, dim3(blocks), dim3(128), smem, f));
         BRASA_TRY(brasa_post_launch(cmd, "attn_packed_few"));
-        BRASA_CUDA(ctx, brasa_launch_dependent(ctx, half ? attn_packed_merge_kernel<true> : attn_packed_merge_kernel<false>, dim3(blocks), dim3(256), 0, (const float *)f.part,
-                                               (const PackedNote *)f.notes, f.o, hq, hq / hkv, FEW_ROWS));
-        return brasa_post_launch(cmd, "attn_packed_merge");
+        return merge(few_part, few_notes, blocks, FEW_ROWS);
     }
 #define ATTN_PACKED(KVT)                                                                                                                                  \
     BRASA_CUDA(ctx, brasa_launch_dependent(ctx, half ? attn_packed_rows_kernel<KVT, true> : attn_packed_rows_kernel<KVT, false>, dim3(run.tokens, hkv), dim3(128), 0, \
