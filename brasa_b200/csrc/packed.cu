@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_const
     if (it.j == it.tiles) line_next(p.l, it);
     while (it.first < end_first || (it.first == end_first && it.j < end_j)) {
         const uint32_t j0 = it.j, j1 = it.first == end_first ? end_j : it.tiles;
-        const uint32_t row0 = it.part * FEW_ROWS, rows = min(FEW_ROWS, it.rows - row0), nkeys = line_keys(p.l, it, it.part);
+        const uint32_t token0 = it.part * p.l.item_tokens, t0 = it.t0 + token0, rows = line_tokens(p.l, it) * G, nkeys = line_keys(p.l, it);
         const uint32_t share = rows <= 16 ? 4 : (rows <= 32 ? 2 : 1), kp = warp % share, rt = warp / share;
         const bool active = rt * 16 < rows;
         // ---- copies of 64 keys: pages one chunk ahead, what the item's last row does not see as zeros ----
@@ -270,10 +270,11 @@ __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_const
         uint32_t seen[2];
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
-            const uint32_t r = row0 + rt * 16 + g + 8 * h;
-            const bool live = active && r < it.rows;
-            seen[h] = live ? it.past + r / G + 1 : 0;
-            const float *src = p.q + ((size_t)(it.t0 + (live ? r / G : 0)) * p.hq + it.kh * G + (live ? r % G : 0)) * D;
+            const uint32_t r = rt * 16 + g + 8 * h;
+            const bool live = active && r < rows;
+            const uint32_t token = live ? row_token(p.l, r) : 0, head = live ? r - token * G : 0;
+            seen[h] = live ? it.past + token0 + token + 1 : 0;
+            const float *src = p.q + ((size_t)(t0 + token) * p.hq + it.kh * G + head) * D;
 #pragma unroll
             for (uint32_t ks = 0; ks < 8; ++ks) {
                 float2 a = make_float2(0.0f, 0.0f), b = a;
@@ -439,8 +440,8 @@ __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_const
                 acc = fmaf(reinterpret_cast<float *>(smem)[(w * 16 + x) * FEW_TS + tid], f, acc);
             }
             if (whole) {
-                const uint32_t row = row0 + r;
-                const size_t at = ((size_t)(it.t0 + row / G) * p.hq + it.kh * G + row % G) * D + tid;
+                const uint32_t token = row_token(p.l, r);
+                const size_t at = ((size_t)(t0 + token) * p.hq + it.kh * G + r - token * G) * D + tid;
                 const float v = L == 0.0f ? 0.0f : acc / L;
                 if (HALF) static_cast<__half *>(p.o)[at] = __float2half_rn(v);
                 else static_cast<float *>(p.o)[at] = v;
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_const
                 }
             }
         }
-        if (!whole && j0 == 0) note = PackedNote{1, note.closes, it.t0 + row0 / G, row0 % G, rows, it.kh};
+        if (!whole && j0 == 0) note = PackedNote{1, note.closes, t0, rows, it.kh};
         if (j0 > 0 && j1 == it.tiles) note.closes = 1;
         __syncthreads();  // the ring and the sums are free again
         if (j1 < it.tiles || !line_next(p.l, it)) break;
@@ -463,7 +464,7 @@ __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_const
 // The items that several blocks worked on: block (b, y) takes the one that piece b began and left open, of it every gridDim.y * 8-th row: the sum of
 // 2^(m - M) O over that of 2^(m - M) l, in the order of the keys.
 template <bool HALF>
-__global__ void __launch_bounds__(256) attn_packed_merge_kernel(const float *part, const PackedNote *notes, void *o, uint32_t hq, uint32_t group, uint32_t rows_item) {
+__global__ void __launch_bounds__(256) attn_packed_merge_kernel(const float *part, const PackedNote *notes, void *o, uint32_t hq, PackedLine l, uint32_t rows_item) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const PackedNote n = notes[blockIdx.x];
@@ -492,8 +493,8 @@ __global__ void __launch_bounds__(256) attn_packed_merge_kernel(const float *par
             acc.w = fmaf(v.w, f, acc.w);
         }
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-        const uint32_t row = n.g0 + r;
-        const size_t at = ((size_t)(n.t0 + row / group) * hq + n.kh * group + row % group) * D + 4 * lane;
+        const uint32_t token = row_token(l, r);
+        const size_t at = ((size_t)(n.t0 + token) * hq + n.kh * l.group + r - token * l.group) * D + 4 * lane;
         if (HALF) *reinterpret_cast<uint2 *>(static_cast<__half *>(o) + at) = make_uint2(pack_h2(acc.x * inv, acc.y * inv), pack_h2(acc.z * inv, acc.w * inv));
         else *reinterpret_cast<float4 *>(static_cast<float *>(o) + at) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     }
@@ -566,14 +567,14 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
         PackedNote *few_notes = (PackedNote *)(tc_part + tc_floats), *tc_notes = few_notes + blocks;
         auto merge = [&](const float *part, const PackedNote *notes, uint32_t pieces, uint32_t rows_item) {
             BRASA_CUDA(ctx, brasa_launch_dependent(ctx, half ? attn_packed_merge_kernel<true> : attn_packed_merge_kernel<false>, dim3(pieces, rows_item / 64), dim3(256), 0, part, notes,
-                                                   (void *)arg_ptr(o), hq, G, rows_item));
+                                                   (void *)arg_ptr(o), hq, packed_line(p, G, rows_item, 0, 0, 0, 0, 0, 0), rows_item));
             return brasa_post_launch(cmd, "attn_packed_merge");
         };
         if (tc) {
             BRASA_TRY(brasa_packed_tc_launch(cmd, p, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), tc_part, tc_notes, hq, scale));
             BRASA_TRY(merge(tc_part, tc_notes, sms, PACKED_TC_ROWS));
         }
-        FewParams f{{p, G, FEW_ROWS, FEW_KEYS, 1, 1, 3, 1, tc ? PACKED_TC_MIN_ROWS - 1 : UINT32_MAX}, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), few_part,
+        FewParams f{packed_line(p, G, FEW_ROWS, 6, 1, 1, 3, 1, tc ? PACKED_TC_MIN_ROWS - 1 : UINT32_MAX), (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), few_part,
                     few_notes, hq, scale};
         void (*const kernel)(FewParams) = pg.kv == BRASA_KV_Q8_0 ? attn_packed_few_kernel<BRASA_KV_Q8_0, true>
                                           : half ? attn_packed_few_kernel<BRASA_KV_F16, true> : attn_packed_few_kernel<BRASA_KV_F16, false>;

@@ -45,50 +45,55 @@ __device__ __forceinline__ int32_t packed_page(const PackedView &p, uint32_t seq
 }
 
 // ---- the work of a run in a line, cut evenly ----
-// An item is up to rows_item rows (token by token, of one token the heads of a key head's group) of one sequence against one key head.
-// In the line an item takes `start` units for its beginning and end and one per `tile` keys that its last row sees. Equal pieces of the line
-// go to the blocks; a block works through the items of its piece, whole ones and parts. A piece's end that falls within `snap` units of an
-// item's ends moves there, since a part costs a way through memory and a merge. Everything is read from device memory, so that a recorded
-// launch follows new lengths.
+// An item is up to item_tokens tokens of one sequence, each with the heads of a key head's group, against that key head. In the line an item takes `start`
+// units for its beginning and end and one per 2^tile_log2 keys that its last token sees. Equal pieces of the line go to the blocks; a block works
+// through the items of its piece, whole ones and parts. A piece's end that falls within `snap` units of an item's ends moves there, since a
+// part costs a way through memory and a merge. Everything is read from device memory, so that a recorded launch follows new lengths.
 struct PackedLine {
     PackedView v;
-    uint32_t group, rows_item, tile, start, snap, least;  // query heads per key head; ..; fewest units that are worth a block
-    uint32_t min_rows, max_rows;                          // sequences of fewer or more rows are another kernel's
+    uint32_t group, inv, item_tokens;        // query heads per key head, 65 536 / group rounded up
+    uint32_t tile_log2, start, snap, least;  // ..; fewest units that are worth a block
+    uint32_t min_rows, max_rows;             // sequences of fewer or more rows (tokens times group) are another kernel's
 };
+inline PackedLine packed_line(const PackedView &v, uint32_t group, uint32_t rows_item, uint32_t tile_log2, uint32_t start, uint32_t snap, uint32_t least, uint32_t min_rows, uint32_t max_rows) {
+    return PackedLine{v, group, (65536 + group - 1) / group, rows_item / group, tile_log2, start, snap, least, min_rows, max_rows};
+}
+// token of a row of an item (below 2^10, for groups up to 8)
+__device__ __forceinline__ uint32_t row_token(const PackedLine &l, uint32_t r) { return r * l.inv >> 16; }
 struct PackedItem {
-    uint64_t first;                // its place in the line
-    uint32_t seq, t0, rows, past;  // sequence, its first row of the run, its rows, the positions before them
-    uint32_t part, kh, tiles;      // which rows_item of its rows, key head, key tiles
-    uint32_t j;                    // the key tile that a piece begins or ends at
+    uint64_t first;             // its place in the line
+    uint32_t seq, t0, n, past;  // sequence, its first row of the run, its tokens, the positions before them
+    uint32_t part, kh, tiles;   // which item_tokens of its tokens, key head, key tiles
+    uint32_t j;                 // the key tile that a piece begins or ends at
 };
 
 __device__ __forceinline__ void line_sequence(const PackedLine &l, uint32_t s, PackedItem &it) {
-    const uint32_t a = min(l.v.starts[s], l.v.tokens), b = min(l.v.starts[s + 1], l.v.tokens);
-    const uint64_t most = (uint64_t)l.v.max_pages * BRASA_KV_PAGE, past = l.v.lens[s];
+    const uint32_t a = min(l.v.starts[s], l.v.tokens), b = min(l.v.starts[s + 1], l.v.tokens), past = l.v.lens[s];
+    const uint64_t most = (uint64_t)l.v.max_pages * BRASA_KV_PAGE;
     uint64_t n = min(b > a ? b - a : 0u, l.v.longest);
     n = past >= most ? 0 : min(n, most - past);
     const uint64_t rows = n * l.group;
     it.seq = s;
     it.t0 = a;
-    it.past = (uint32_t)past;
-    it.rows = rows >= l.min_rows && rows <= l.max_rows ? (uint32_t)rows : 0u;
+    it.past = past;
+    it.n = rows >= l.min_rows && rows <= l.max_rows ? (uint32_t)n : 0u;
 }
-__device__ __forceinline__ uint32_t line_keys(const PackedLine &l, const PackedItem &it, uint32_t part) {  // that a part's last row sees
-    return it.past + (min((part + 1) * l.rows_item, it.rows) - 1) / l.group + 1;
-}
-__device__ __forceinline__ uint32_t line_tiles(const PackedLine &l, const PackedItem &it, uint32_t part) { return (line_keys(l, it, part) - 1) / l.tile + 1; }
+__device__ __forceinline__ uint32_t line_keys(const PackedLine &l, const PackedItem &it) { return it.past + min((it.part + 1) * l.item_tokens, it.n); }  // that its last token sees
+__device__ __forceinline__ uint32_t line_tokens(const PackedLine &l, const PackedItem &it) { return min(l.item_tokens, it.n - it.part * l.item_tokens); }
+__device__ __forceinline__ uint32_t line_tiles(const PackedLine &l, const PackedItem &it) { return ((line_keys(l, it) - 1) >> l.tile_log2) + 1; }
+// units of all items of a sequence, for one key head
 __device__ __forceinline__ uint64_t line_units(const PackedLine &l, const PackedItem &it) {
     uint64_t u = 0;
-    for (uint32_t p = 0; p * l.rows_item < it.rows; ++p) u += (uint64_t)l.v.hkv * (l.start + line_tiles(l, it, p));
-    return u;
+#pragma unroll 4
+    for (uint32_t t = l.item_tokens; t < it.n; t += l.item_tokens) u += l.start + 1 + ((it.past + t - 1) >> l.tile_log2);
+    return it.n ? u + l.start + 1 + ((it.past + it.n - 1) >> l.tile_log2) : 0;
 }
 
 // What a block leaves of the items at its piece's ends, for the kernel that adds parts up.
 struct PackedNote {
-    uint32_t opens;         // the piece began an item and left it open: the rest of the note is about that item
-    uint32_t closes;        // the piece ended an item that began before it
-    uint32_t t0, g0, rows;  // first row of the run, head of the group at its first row, rows
-    uint32_t kh;
+    uint32_t opens;   // the piece began an item and left it open: the rest of the note is about that item
+    uint32_t closes;  // the piece ended an item that began before it
+    uint32_t t0, rows, kh;  // its first row of the run, its rows (tokens times group), key head
 };
 // floats of a part's slot: O [rows_item][128], m and l by row
 __host__ __device__ constexpr size_t packed_part_floats(uint32_t rows_item) { return (size_t)rows_item * 130; }
@@ -111,7 +116,7 @@ __device__ bool line_cut(const PackedLine &l, PackedPieces &w) {
     uint64_t mine = 0;
     for (uint32_t s = s0; s < s1; ++s) {
         line_sequence(l, s, it);
-        mine += line_units(l, it);
+        mine += line_units(l, it) * l.v.hkv;
     }
     uint64_t upto = mine;
     for (uint32_t x = 1; x < 32; x <<= 1) {
@@ -141,20 +146,24 @@ __device__ bool line_cut(const PackedLine &l, PackedPieces &w) {
             uint32_t s = s0;
             for (;; ++s) {  // (ends: the unit lies in one of this thread's sequences)
                 line_sequence(l, s, it);
-                const uint64_t u = line_units(l, it);
+                if (each == 1) break;
+                const uint64_t u = line_units(l, it) * l.v.hkv;
                 if (unit < first + u) break;
                 first += u;
             }
-            it.part = 0;
-            uint32_t tiles = line_tiles(l, it, 0);
-            while (unit >= first + (uint64_t)l.v.hkv * (l.start + tiles)) {
-                first += (uint64_t)l.v.hkv * (l.start + tiles);
-                tiles = line_tiles(l, it, ++it.part);
+            // of the sequence's items, in one key head's units: part by part (their key heads lie behind one another)
+            uint64_t left = unit - first;
+            uint32_t each_item = 0;
+            for (it.part = 0;; ++it.part) {  // (ends: the unit lies in one of them)
+                it.tiles = line_tiles(l, it);
+                each_item = l.start + it.tiles;
+                const uint64_t all = (uint64_t)each_item * l.v.hkv;
+                if (left < all) break;
+                left -= all;
             }
-            const uint32_t each_item = l.start + tiles;
-            it.kh = (uint32_t)((unit - first) / each_item);
-            it.first = first + (uint64_t)it.kh * each_item;
-            it.tiles = tiles;
+            it.kh = (uint32_t)(left / each_item);
+            const uint32_t tiles = it.tiles;
+            it.first = unit - left + (uint64_t)it.kh * each_item;
             const uint32_t off = (uint32_t)(unit - it.first);
             it.j = off > l.start ? off - l.start : 0u;
             if (it.j < l.snap) it.j = 0;
@@ -171,14 +180,14 @@ __device__ __forceinline__ bool line_next(const PackedLine &l, PackedItem &it) {
     it.j = 0;
     if (++it.kh < l.v.hkv) return true;
     it.kh = 0;
-    if (++it.part * l.rows_item >= it.rows) {
+    if (++it.part * l.item_tokens >= it.n) {
         it.part = 0;
         do {
             if (++it.seq >= l.v.seqs) return false;
             line_sequence(l, it.seq, it);
-        } while (it.rows == 0);
+        } while (it.n == 0);
     }
-    it.tiles = line_tiles(l, it, it.part);
+    it.tiles = line_tiles(l, it);
     return true;
 }
 
