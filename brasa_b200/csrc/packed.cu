@@ -180,14 +180,6 @@ __device__ __forceinline__ void terms_h2(float x, float y, uint32_t &hi, uint32_
         lo = pack_h2(x - back.x, y - back.y);
     }
 }
-// two signed bytes of `w` (already without sign bit: +128), chosen by `sel` into the low bytes of two halves, as f16 (exact) times a pair of scales
-__device__ __forceinline__ uint32_t bytes_h2(uint32_t w, uint32_t sel, __half2 scale) {
-    const uint32_t u = __byte_perm(w, 0x64646464u, sel);  // 1024 + byte
-    __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));  // - 1152
-    h = __hmul2(h, scale);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 template <int KV, bool HALF>
 __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_constant__ FewParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");  // (launched as a programmatic dependent: see brasa_launch_dependent)
@@ -557,9 +549,9 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
     BRASA_REQUIRE(ctx, (uint64_t)run.tokens * (hq / hkv) < 1ull << 31, "attention_packed: more than 2^31 rows of a key head's group");
     const float scale = 1.0f / sqrtf((float)D);
     if (pg.kv == BRASA_KV_F16 || (pg.kv == BRASA_KV_Q8_0 && half)) {
-        // Sequences of many rows go to the tensor-core kernel where there is one (16-bit products of an f16 pool) and the call can have any.
+        // Sequences of many rows go to the tensor-core kernel where there is one (16-bit products) and the call can have any.
         const uint32_t G = hq / hkv, sms = ctx->sm_count, blocks = sms * 2;
-        const bool tc = half && pg.kv == BRASA_KV_F16 && (uint64_t)run.longest * G >= PACKED_TC_MIN_ROWS && (uint64_t)pg.num_pages * PAGE < 1ull << 31;
+        const bool tc = half && (uint64_t)run.longest * G >= PACKED_TC_MIN_ROWS && (uint64_t)pg.num_pages * PAGE < 1ull << 31;
         // the workspace: parts of either kernel's items, then what they belong to
         const size_t few_floats = 2 * (size_t)blocks * packed_part_floats(FEW_ROWS), tc_floats = 2 * (size_t)sms * packed_part_floats(PACKED_TC_ROWS);
         BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, (few_floats + tc_floats) * sizeof(float) + (blocks + sms) * sizeof(PackedNote)));
@@ -571,7 +563,7 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
             return brasa_post_launch(cmd, "attn_packed_merge");
         };
         if (tc) {
-            BRASA_TRY(brasa_packed_tc_launch(cmd, p, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), tc_part, tc_notes, hq, scale));
+            BRASA_TRY(brasa_packed_tc_launch(cmd, p, pg.kv, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), tc_part, tc_notes, hq, scale));
             BRASA_TRY(merge(tc_part, tc_notes, sms, PACKED_TC_ROWS));
         }
         FewParams f{packed_line(p, G, FEW_ROWS, 6, 1, 1, 3, 1, tc ? PACKED_TC_MIN_ROWS - 1 : UINT32_MAX), (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), few_part,

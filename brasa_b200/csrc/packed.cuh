@@ -44,6 +44,14 @@ __device__ __forceinline__ int32_t packed_page(const PackedView &p, uint32_t seq
     return (uint32_t)page < p.num_pages ? page : -1;
 }
 
+// two signed bytes of `w` (already without sign bit: +128), chosen by `sel` into the low bytes of two halves, as f16 (exact) times a pair of scales
+__device__ __forceinline__ uint32_t bytes_h2(uint32_t w, uint32_t sel, __half2 scale) {
+    const uint32_t u = __byte_perm(w, 0x64646464u, sel);  // 1024 + byte
+    __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));  // - 1152
+    h = __hmul2(h, scale);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 // ---- the work of a run in a line, cut evenly ----
 // An item is up to item_tokens tokens of one sequence, each with the heads of a key head's group, against that key head. In the line an item takes `start`
 // units for its beginning and end and one per 2^tile_log2 keys that its last token sees. Equal pieces of the line go to the blocks; a block works

@@ -5,11 +5,13 @@
 // 128^3: S = Q K^T into tensor memory, O += P V with P read out of tensor memory, over the columns that S had. Two threads hold a row, 64 scores
 // each: warps 0-7 tile A, 8-15 tile B; warp 16 issues the products, warp 17 the copies. The order on the tensor core is P V of A, S of
 // A's next keys, P V of B, S of B's next, so that one tile's products run while the other's probabilities are formed.
-// K and V tiles are eight pages each, two boxes of 16 positions x 64 dims a page (cp.async.bulk.tensor, 128-byte swizzle), through a ring of four
-// 32 KB slots. Rows of the cache behind the item's last position may hold anything: such scores are replaced before they count, and V's rows,
+// K and V tiles are eight pages each, two boxes of 16 positions x 64 dims a page (cp.async.bulk.tensor, 128-byte swizzle), through two slots of 32 KB each. A
+// warp issues such a copy every 80 cycles, so that K and V have a warp each.
+// Rows of the cache behind the item's last position may hold anything: such scores are replaced before they count, and V's rows,
 // which enter P V with a weight of zero, are written as zeros by the copying warp instead of copied.
 // What bounds it: the tensor core, 2 048 cycles per tile of keys, and as many cycles of exponentials (16 a clock).
 #include <math.h>
+#include <string.h>
 
 #include "packed_tc.h"
 #include "tc_device.cuh"
@@ -18,8 +20,9 @@ using namespace brasa_dev;
 
 namespace {
 
-constexpr uint32_t PAGE = BRASA_KV_PAGE, D = 128, WAIT_LIMIT = 1u << 20, TILE_BYTES = 128 * 128 * 2, SLOTS = 4, ROWS = PACKED_TC_ROWS;
-constexpr uint32_t SOFTMAX_WARPS = 16, MMA_WARP = 16, COPY_WARP = 18, THREADS = 608;  // (one MMA warp for each row tile)
+constexpr uint32_t PAGE = BRASA_KV_PAGE, D = 128, WAIT_LIMIT = 1u << 20, TILE_BYTES = 128 * 128 * 2, ROWS = PACKED_TC_ROWS;
+constexpr uint32_t SOFTMAX_WARPS = 8, MMA_WARP = 8, K_WARP = 10, V_WARP = 11;  // (one MMA warp for each row tile)
+constexpr uint32_t THREADS = 384, THREADS_Q8 = 448;  // an 8-bit pool's K and V have two warps each
 
 struct PackedMaps {
     CUtensorMap k, v;
@@ -27,7 +30,7 @@ struct PackedMaps {
 struct PackedTcParams {
     PackedLine l;
     const float *q;
-    const uint8_t *vpool;
+    const uint8_t *kpool, *vpool;
     __half *o;
     float *part;
     PackedNote *notes;
@@ -35,6 +38,15 @@ struct PackedTcParams {
     float scale;
     uint32_t *status;
 };
+
+// A block's share of an item, as the copying warp hands it on: the other roles keep no place in the line.
+struct PackedShare {
+    uint32_t t0, rows, kh, past;  // its first row of the run, its rows (0: there are no more), key head, positions before its first token
+    uint32_t seq, nkeys;          // sequence, keys that its last token sees
+    uint32_t j0, len, steps;      // first key tile, key tiles, steps of 64 keys as far as any are seen
+    uint32_t whole;               // all of the item's keys
+};
+constexpr uint32_t SHARES = 8;  // (the copies are at most four items ahead of the outputs)
 
 // byte offset of the 16-byte piece of columns [c, c + 8) of row r in a swizzled 128 x 128 tile of 16-bit values
 __device__ __forceinline__ uint32_t tile_piece(uint32_t r, uint32_t c) {
@@ -54,13 +66,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t v[32]) {  // 
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t v[8]) {  // (the caller waits for its stores)
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
                  "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t v[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
-                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                 : "r"(taddr)
                  : "memory");
 }
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t v[8]) {
@@ -84,32 +89,36 @@ __device__ __forceinline__ void add_halves(uint32_t pair, float &a, float &b) {
     asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tadd.rn.f32.f16 %0, x, %0;\n\tadd.rn.f32.f16 %1, y, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(pair));
 }
 
-__global__ void __launch_bounds__(THREADS, 1) attn_packed_tc_kernel(const __grid_constant__ PackedMaps maps, const __grid_constant__ PackedTcParams p) {
+template <bool Q8>
+__global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_kernel(const __grid_constant__ PackedMaps maps, const __grid_constant__ PackedTcParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *ring = smem + 2 * TILE_BYTES;
-    __shared__ uint64_t full[SLOTS], freed[SLOTS], q_full[2], s_ready[2], p_ready[2][2], o_done[2], turn[2];
+    __shared__ uint64_t full[2][2], freed[2][2], q_full[2], s_ready[2][2], p_ready[2][2], pv_done[2], o_done[2], turn[2], share_full[SHARES];
+    __shared__ PackedShare shares[SHARES];
     __shared__ uint32_t tmem_base_s, abort_s, there_s[8];  // (there: of the last key tiles, which of their eight pages are pages)
-    __shared__ float pair[2][2][128];                      // [row tile][half of the keys][row]: largest score; at the end the sum of the weights
     __shared__ PackedPieces pieces;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.l.group, hkv = p.l.v.hkv;
 
     if (tid == 0) {
-        for (uint32_t i = 0; i < SLOTS; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&freed[i], 2);  // by either row tile's products
+        for (uint32_t i = 0; i < 4; ++i) {  // [K or V][slot]
+            mbar_init(&full[i >> 1][i & 1], Q8 ? 2 : 1);
+            mbar_init(&freed[i >> 1][i & 1], 2);  // by either row tile's products
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&q_full[i], 8);  // one arrival per softmax warp of the row tile
-            mbar_init(&s_ready[i], 1);
-            mbar_init(&p_ready[i][0], 8);
-            mbar_init(&p_ready[i][1], 8);
-            mbar_init(&turn[i], 8);  // of the other row tile's warps
+            mbar_init(&q_full[i], 4);  // one arrival per softmax warp of the row tile
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&s_ready[i][b], 1);
+                mbar_init(&p_ready[i][b], 4);
+            }
+            mbar_init(&pv_done[i], 1);
+            mbar_init(&turn[i], 4);  // of the other row tile's warps
             mbar_init(&o_done[i], 1);
         }
+        for (uint32_t i = 0; i < SHARES; ++i) mbar_init(&share_full[i], 1);
         abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == MMA_WARP) {  // tensor memory: S, then P over the first half of either 64 keys, of A in [0, 128), of B in [128, 256); O of A in [256, 384), of B in [384, 512)
+    if (warp == MMA_WARP) {  // tensor memory: S of A, two steps, then P over them, in [0, 128), of B in [128, 256); O of A in [256, 384), of B in [384, 512)
         const uint32_t ncols = 512;
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(ncols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -138,54 +147,108 @@ __global__ void __launch_bounds__(THREADS, 1) attn_packed_tc_kernel(const __grid
         abort_s = 1;
     }
     const bool work = line_cut<256>(p.l, pieces) && !abort_s;
-    // Every role walks through the block's items by itself; they meet at barriers of their own only.
-    PackedItem item = pieces.at[0];
-    const uint64_t end_first = pieces.at[1].first;
-    const uint32_t end_j = pieces.at[1].j;
-    if (work && item.j == item.tiles) line_next(p.l, item);
-    bool more = work && (item.first < end_first || (item.first == end_first && item.j < end_j));
-    auto item_end = [&]() { return item.first == end_first ? end_j : item.tiles; };  // the key tile at which this block's share of the item ends
-    auto next_item = [&](PackedItem &it, uint32_t j1) { return j1 == it.tiles && line_next(p.l, it) && (it.first < end_first || (it.first == end_first && end_j > 0)); };
-    auto has_b = [&](const PackedItem &it) { return line_tokens(p.l, it) * G > 128; };  // rows in both row tiles
-    if (warp == COPY_WARP) {  // ---- K and V, as far ahead of the products as there are slots ----
-        bool ok = true;
-        uint32_t loads = 0;  // tiles copied so far, K and V apart
+    auto share_at = [&](uint32_t i) -> bool { return all_wait(&share_full[i % SHARES], (i / SHARES) & 1); };  // the block's i-th share is handed on
+
+    if (warp >= K_WARP) {  // ---- copies, as far ahead of the products as there are slots; K's warp walks the line and hands the shares on ----
+        const uint32_t is_v = (warp - K_WARP) & 1;
+        const bool walks = warp == K_WARP;
+        PackedItem item = pieces.at[0];
+        const uint64_t end_first = pieces.at[1].first;
+        const uint32_t end_j = pieces.at[1].j;
+        if (work && item.j == item.tiles) line_next(p.l, item);
+        bool more = work && (item.first < end_first || (item.first == end_first && item.j < end_j)), ok = true;
+        PackedNote note{};
+        uint32_t loads = 0;  // tiles copied so far
 #pragma unroll 1
-        while (more && ok) {
-            const uint32_t j0 = item.j, j1 = item_end(), nkeys = line_keys(p.l, item);
-            const int32_t *table = p.l.v.table + (size_t)item.seq * p.l.v.max_pages;
-            auto page_at = [&](uint32_t i) { return (uint64_t)16 * i < nkeys ? table[i] : -1; };  // as the table has it, -1 where nothing is seen
-            int32_t now = page_at(8 * j0 + lane), ahead = page_at(8 * j0 + 32 + lane);           // the pages of four tiles, and of the next four
-            for (uint32_t t = lane; t < line_tokens(p.l, item); t += 32)  // the item's queries on their way into L2
-                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.q + ((size_t)(item.t0 + item.part * p.l.item_tokens + t) * p.hq + item.kh * G) * D), "r"(G * D * 4) : "memory");
-            for (uint32_t j = j0; j < j1 && ok; ++j) {
-                const uint32_t k = (j - j0) & 3, half = lane & 1, i = (lane >> 1) & 7;  // lanes 2 i and 2 i + 1 take the halves of page i
-                if (j > j0 && k == 0) {
-                    now = ahead;
-                    ahead = page_at(8 * j + 32 + lane);
+        for (uint32_t n = 0; ok; ++n) {
+            PackedShare &share = shares[n % SHARES];
+            if (walks) {
+                if (lane == 0) {
+                    share.rows = 0;
+                    if (more) {
+                        const uint32_t j1 = item.first == end_first ? end_j : item.tiles, token0 = item.part * p.l.item_tokens, rows = line_tokens(p.l, item) * G;
+                        share = PackedShare{item.t0 + token0, rows, item.kh, item.past + token0, item.seq, line_keys(p.l, item), item.j, j1 - item.j, min(2 * (j1 - item.j), (line_keys(p.l, item) - 128 * item.j + 63) / 64),
+                                            item.j == 0 && j1 == item.tiles};
+                        if (j1 < item.tiles && item.j == 0) note = PackedNote{1, note.closes, item.t0 + token0, rows, item.kh};
+                        if (item.j > 0 && j1 == item.tiles) note.closes = 1;
+                    } else p.notes[blockIdx.x] = note;
+                    tc_mbar_arrive(&share_full[n % SHARES]);
                 }
-                int32_t page = __shfl_sync(0xffffffffu, now, 8 * k + i);
-                if ((uint32_t)page >= p.l.v.num_pages) page = -1;
-                const uint32_t there = __ballot_sync(0xffffffffu, (uint32_t)now < p.l.v.num_pages) >> (8 * k) & 255;
-                const uint32_t left = nkeys - min(nkeys, 128 * j + 16 * i);  // of the page's positions, those that are seen
-                for (uint32_t is_v = 0; is_v < 2; ++is_v, ++loads) {
-                    const uint32_t s = loads % SLOTS;
-                    if (loads >= SLOTS && !all_wait(&freed[s], ((loads / SLOTS) - 1) & 1)) {
-                        ok = false;
-                        break;
+                __syncwarp();
+            } else ok = share_at(n);
+            if (!ok || share.rows == 0) break;
+            const uint32_t j0 = share.j0, len = share.len, nkeys = share.nkeys, kh = share.kh;
+            const int32_t *table = p.l.v.table + (size_t)share.seq * p.l.v.max_pages;
+            auto page_at = [&](uint32_t i) { return (uint64_t)16 * i < nkeys ? table[i] : -1; };  // as the table has it, -1 where nothing is seen
+            if (warp == V_WARP)  // the queries on their way into L2
+                for (uint32_t t = lane; t * G < share.rows; t += 32)
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.q + ((size_t)(share.t0 + t) * p.hq + kh * G) * D), "r"(G * D * 4) : "memory");
+            if constexpr (Q8) {
+                // Rows are turned into f16(d * code) on the way: this warp has pages 4 w .. 4 w + 3 of a tile, two rows at a time, eight codes a lane; a tile's codes are
+                // fetched while the tile before is turned.
+                const uint32_t w = (warp - K_WARP) >> 1, c = lane & 15, r2 = lane >> 4;
+                const uint8_t *pool = is_v ? p.vpool : p.kpool;
+                uint2 code[32];
+                __half scale[32];
+                uint32_t there = 0;
+                auto fetch = [&](uint32_t j) {  // of tile j0 + j
+                    const int32_t mine = j < len ? page_at(8 * (j0 + j) + (lane & 7)) : -1;
+                    there = __ballot_sync(0xffffffffu, (uint32_t)mine < p.l.v.num_pages) & 255u;
+#pragma unroll
+                    for (uint32_t e = 0; e < 32; ++e) {
+                        const uint32_t i = 4 * w + (e >> 3), r = 2 * (e & 7) + r2;
+                        const int32_t page = __shfl_sync(0xffffffffu, mine, i);
+                        code[e] = make_uint2(0, 0);
+                        scale[e] = __ushort_as_half(0);
+                        if ((there >> i & 1) && 128 * (j0 + j) + 16 * i + r < nkeys) {
+                            const uint8_t *row = pool + (((size_t)page * PAGE + r) * hkv + kh) * 136;
+                            code[e] = reinterpret_cast<const uint2 *>(row)[c];
+                            scale[e] = reinterpret_cast<const __half *>(row + 128)[c >> 2];
+                        }
                     }
-                    uint8_t *slot = ring + (size_t)s * TILE_BYTES;
+                };
+                fetch(0);
+                for (uint32_t j = 0; j < len; ++j, ++loads) {
+                    const uint32_t s = loads & 1;
+                    if (loads >= 2 && !(ok = all_wait(&freed[is_v][s], ((loads >> 1) - 1) & 1))) break;
+                    uint8_t *slot = ring + (size_t)(2 * is_v + s) * TILE_BYTES;
+                    if (walks && lane == 0) there_s[loads & 7] = there;  // (read by whoever sees this tile's scores, four tiles behind at most)
+#pragma unroll
+                    for (uint32_t e = 0; e < 32; ++e) {
+                        const __half2 d = __half2half2(scale[e]);
+                        const uint32_t lo = code[e].x ^ 0x80808080u, hi = code[e].y ^ 0x80808080u;
+                        *reinterpret_cast<uint4 *>(slot + tile_piece(64 * w + 16 * (e >> 3) + 2 * (e & 7) + r2, 8 * c)) =
+                            make_uint4(bytes_h2(lo, 0x4140, d), bytes_h2(lo, 0x4342, d), bytes_h2(hi, 0x4140, d), bytes_h2(hi, 0x4342, d));
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) tc_mbar_arrive(&full[is_v][s]);
+                    fetch(j + 1);
+                }
+            } else {
+                int32_t now = page_at(8 * j0 + lane), ahead = page_at(8 * j0 + 32 + lane);  // the pages of four tiles, and of the next four
+                for (uint32_t j = 0; j < len; ++j, ++loads) {
+                    const uint32_t k = j & 3, s = loads & 1, half = lane & 1, i = (lane >> 1) & 7;  // lanes 2 i and 2 i + 1 take the halves of page i
+                    if (j > 0 && k == 0) {
+                        now = ahead;
+                        ahead = page_at(8 * (j0 + j) + 32 + lane);
+                    }
+                    int32_t page = __shfl_sync(0xffffffffu, now, 8 * k + i);
+                    if ((uint32_t)page >= p.l.v.num_pages) page = -1;
+                    const uint32_t left = nkeys - min(nkeys, 128 * (j0 + j) + 16 * i);  // of the page's positions, those that are seen
+                    if (loads >= 2 && !(ok = all_wait(&freed[is_v][s], ((loads >> 1) - 1) & 1))) break;
+                    uint8_t *slot = ring + (size_t)(2 * is_v + s) * TILE_BYTES;
                     const bool whole = page >= 0 && (!is_v || left >= 16);
-                    const uint32_t odd = is_v ? __ballot_sync(0xffffffffu, !whole) & 0x5555u : 0u;  // bit 2 i: page i is not copied whole
-                    for (uint32_t b = odd; b; b &= b - 1) {  // what is seen of it, and zeros
-                        const uint32_t e = (__ffs(b) - 1) >> 1, seen = __shfl_sync(0xffffffffu, page >= 0 ? left : 0u, 2 * e);
+                    const uint32_t odd = is_v ? __ballot_sync(0xffffffffu, !whole) & 0x5555u : 0u;  // (bit 2 i) pages that are not copied whole
+                    for (uint32_t bits = odd; bits; bits &= bits - 1) {                             // what is seen of such a page, and zeros
+                        const uint32_t e = (__ffs(bits) - 1) >> 1, seen = __shfl_sync(0xffffffffu, page >= 0 ? left : 0u, 2 * e);
                         const int32_t from = __shfl_sync(0xffffffffu, page, 2 * e);
                         uint4 v[8];
 #pragma unroll
                         for (uint32_t u = 0; u < 8; ++u) {
                             const uint32_t r = 2 * u + (lane >> 4);
                             v[u] = make_uint4(0, 0, 0, 0);
-                            if (r < seen) v[u] = reinterpret_cast<const uint4 *>(p.vpool + (((size_t)from * PAGE + r) * hkv + item.kh) * 256)[lane & 15];
+                            if (r < seen) v[u] = reinterpret_cast<const uint4 *>(p.vpool + (((size_t)from * PAGE + r) * hkv + kh) * 256)[lane & 15];
                         }
 #pragma unroll
                         for (uint32_t u = 0; u < 8; ++u) *reinterpret_cast<uint4 *>(slot + tile_piece(16 * e + 2 * u + (lane >> 4), 8 * (lane & 15))) = v[u];
@@ -194,116 +257,120 @@ __global__ void __launch_bounds__(THREADS, 1) attn_packed_tc_kernel(const __grid
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                     }
-                    const uint32_t copies = __popc(__ballot_sync(0xffffffffu, whole) & 0xffffu);
+                    const uint32_t copied = __popc(__ballot_sync(0xffffffffu, whole) & 0xffffu), there = __ballot_sync(0xffffffffu, (uint32_t)now < p.l.v.num_pages) >> (8 * k) & 255u;
                     if (lane == 0) {
-                        if (!is_v) there_s[(loads >> 1) & 7] = there;  // (read by whoever sees this tile's scores; the ring is at most four loads ahead)
-                        mbar_expect_tx(&full[s], copies * 2048);
+                        if (!is_v) there_s[loads & 7] = there;  // (K: which pages are pages; read by whoever sees this tile's scores, four tiles behind at most)
+                        mbar_expect_tx(&full[is_v][s], copied * 2048);
                     }
                     __syncwarp();
-                    if (whole && lane < 16) tma_load_3d(slot + half * 16384 + i * 2048, is_v ? &maps.v : &maps.k, (int)(half * 64), (int)item.kh, page * (int)PAGE, &full[s]);
+                    if (whole && lane < 16) tma_load_3d(slot + half * 16384 + i * 2048, is_v ? &maps.v : &maps.k, (int)(half * 64), (int)kh, page * (int)PAGE, &full[is_v][s]);
                 }
             }
-            more = next_item(item, j1);
+            if (walks && ok) {
+                const uint32_t j1 = item.first == end_first ? end_j : item.tiles;
+                more = j1 == item.tiles && line_next(p.l, item) && (item.first < end_first || (item.first == end_first && end_j > 0));
+            }
         }
-        if (*abort_flag && lane == 0) {  // leaving early: let the copies in flight land before the block's shared memory is handed on
-            for (uint32_t k = loads > SLOTS ? loads - SLOTS : 0; k < loads; ++k)
-                for (uint32_t it = 0; it < WAIT_LIMIT && !tc_mbar_try(&full[k % SLOTS], (k / SLOTS) & 1); ++it) {}
+        if (!Q8 && *abort_flag && lane == 0) {  // leaving early: let the copies in flight land before the block's shared memory is handed on
+            for (uint32_t k = loads > 2 ? loads - 2 : 0; k < loads; ++k)
+                for (uint32_t it = 0; it < WAIT_LIMIT && !tc_mbar_try(&full[is_v][k & 1], (k >> 1) & 1); ++it) {}
         }
     } else if (warp == MMA_WARP || warp == MMA_WARP + 1) {  // ---- products of one row tile: the warp waits, one lane issues ----
-        const uint32_t idesc_s = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24), idesc_o = idesc_s | (1u << 16);  // f16 operands; V is MN-major
+        constexpr uint32_t idesc_s = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);  // f16; V is MN-major
         const uint32_t x = warp - MMA_WARP, st = tmem + 128 * x, ot = tmem + 256 + 128 * x;
-        auto landed = [&](uint32_t m) { return all_wait(&full[m % SLOTS], (m / SLOTS) & 1); };
-        auto slot = [&](uint32_t m) { return smem_u32(ring + (size_t)(m % SLOTS) * TILE_BYTES); };
-        uint32_t loads = 0, done = 0, segs = 0;  // of the items before: tiles copied, key tiles of this row tile, items with this row tile
+        const uint64_t q = tc_desc_kmajor(smem_u32(smem + x * TILE_BYTES));
+        auto landed = [&](uint32_t is_v, uint32_t t) { return all_wait(&full[is_v][t & 1], (t >> 1) & 1); };
+        auto slot = [&](uint32_t is_v, uint32_t t) { return smem_u32(ring + (size_t)(2 * is_v + (t & 1)) * TILE_BYTES); };
+        uint32_t loads = 0, segs = 0, used[2] = {0, 0};  // of the shares before: key tiles, shares with this row tile, uses of either step's columns
         bool ok = true;
 #pragma unroll 1
-        while (more && ok) {
-            const uint32_t j0 = item.j, j1 = item_end(), len = j1 - j0;
-            const bool both = has_b(item);
-            if (x == 1 && !both) {  // no rows: the slots are given back as they come
-                for (uint32_t m = loads; ok && m < loads + 2 * len; ++m) {
-                    ok = landed(m);
-                    if (ok && lane == 0) tc_mbar_arrive(&freed[m % SLOTS]);
-                }
+        for (uint32_t i = 0; ok; ++i) {
+            if (!(ok = share_at(i))) break;
+            const PackedShare &share = shares[i % SHARES];
+            const uint32_t rows = share.rows, len = share.len, steps = share.steps;
+            if (rows == 0) break;
+            if (x == 1 && rows <= 128) {  // no rows: the slots are given back as they come
+                for (uint32_t t = loads; ok && t < loads + len; ++t)
+                    for (uint32_t is_v = 0; is_v < 2 && ok; ++is_v) {
+                        ok = landed(is_v, t);
+                        if (ok && lane == 0) tc_mbar_arrive(&freed[is_v][t & 1]);
+                    }
             } else {
-                const uint32_t q = smem_u32(smem + x * TILE_BYTES);
-                ok = all_wait(&q_full[x], segs & 1);
-                for (uint32_t j = 0; j <= len && ok; ++j) {
-                    const uint32_t mv = loads + 2 * j - 1, mk = loads + 2 * j;
-                    ok = (j == 0 || landed(mv)) && (j == len || landed(mk));
+                auto scores = [&](uint32_t k) {  // S = Q K^T of step k, over the columns of the P that the product before it has read
+                    const uint32_t t = loads + (k >> 1), b = k & 1;
+                    if (tc_elect_one()) {
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint64_t kd = tc_desc_kmajor(slot(0, t) + 8192 * b);
+#pragma unroll
+                        for (uint32_t ks = 0; ks < 8; ++ks) {
+                            const uint32_t off = ((ks >> 2) * 16384 + (ks & 3) * 32) >> 4;
+                            tc_mma(st + 64 * b, q + off, kd + off, idesc_s, ks > 0 ? 1u : 0u);
+                        }
+                        tc_commit(&s_ready[x][b]);
+                        if (b == 1 || k + 1 == steps) tc_commit(&freed[0][t & 1]);
+                    }
+                    __syncwarp();
+                };
+                ok = all_wait(&q_full[x], segs & 1) && landed(0, loads);
+                if (ok) scores(0);
+                if (ok && steps > 1) scores(1);
+                for (uint32_t k = 0; k < steps && ok; ++k) {
+                    const uint32_t t = loads + (k >> 1), b = k & 1;
+                    if (b == 0) ok = landed(1, t) && (k + 2 >= steps || landed(0, t + 1));
+                    ok = ok && all_wait(&p_ready[x][b], (used[b] + (k >> 1)) & 1);
                     if (!ok) break;
-                    if (j > 0) {  // O += P V of the tile before, in two halves as they come
-                        const uint32_t v = slot(mv);
+                    if (tc_elect_one()) {  // O += P V
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint64_t v = tc_desc_mnmajor(slot(1, t) + 8192 * b);
 #pragma unroll
-                        for (uint32_t e = 0; e < 2 && ok; ++e) {
-                            ok = all_wait(&p_ready[x][e], (done + j - 1) & 1);
-                            if (!ok) break;
-                            if (tc_elect_one()) {
-                                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                                for (uint32_t k = 0; k < 4; ++k) {  // 16 keys: 8 columns of P; 32 keys of either half of the tile
-                                    const uint32_t ks = 4 * (k >> 1) + 2 * e + (k & 1);
-                                    tc_mma_ta(ot, st + 64 * (ks >> 2) + 8 * (ks & 3), tc_desc_mnmajor(v + ks * 2048), idesc_o, (j > 1 || e > 0 || k > 0) ? 1u : 0u);
-                                }
-                                if (e == 1) tc_commit(&freed[mv % SLOTS]);
-                                if (e == 1 && j == len) tc_commit(&o_done[x]);
-                            }
-                            __syncwarp();
-                        }
-                        if (!ok) break;
+                        for (uint32_t ks = 0; ks < 4; ++ks) tc_mma_ta(ot, st + 64 * b + 8 * ks, v + ks * (2048 >> 4), idesc_o, (k > 0 || ks > 0) ? 1u : 0u);
+                        tc_commit(&pv_done[x]);
+                        if (b == 1 || k + 1 == steps) tc_commit(&freed[1][t & 1]);
+                        if (k + 1 == steps) tc_commit(&o_done[x]);
                     }
-                    if (j < len) {  // S = Q K^T of this tile, over the columns of the P just read
-                        if (tc_elect_one()) {
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                            const uint32_t k = slot(mk);
-#pragma unroll
-                            for (uint32_t ks = 0; ks < 8; ++ks) {
-                                const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
-                                tc_mma(st, tc_desc_kmajor(q + off), tc_desc_kmajor(k + off), idesc_s, ks > 0 ? 1u : 0u);
-                            }
-                            tc_commit(&s_ready[x]);
-                            tc_commit(&freed[mk % SLOTS]);
-                        }
-                        __syncwarp();
-                    }
+                    __syncwarp();
+                    if (k + 2 < steps) scores(k + 2);
                 }
-                done += len;
+                used[0] += (steps + 1) / 2;
+                used[1] += steps / 2;
                 ++segs;
             }
-            loads += 2 * len;
-            more = next_item(item, j1);
+            loads += len;
         }
         if (*abort_flag) {  // leaving early: the products in flight end before the block's memory is handed on (one commit more to the output's barrier)
             if (tc_elect_one()) tc_commit(&o_done[x]);
             __syncwarp();
             for (uint32_t it = 0; it < 4096 && !tc_mbar_try(&o_done[x], segs & 1); ++it) {}
         }
-    } else if (warp < SOFTMAX_WARPS) {  // ---- softmax: two threads per row, 64 keys of every tile each ----
+    } else if (warp < SOFTMAX_WARPS) {  // ---- softmax: a thread per row ----
         constexpr float LOG2E = 1.4426950408889634f, SLACK = 5.545177444f;  // 8 ln 2
-        const uint32_t x = warp >> 3, h = (warp >> 2) & 1, wrow = (warp & 3) * 32, row = wrow + lane;
-        const uint32_t ts = tmem + 128 * x + 64 * h + (wrow << 16), to = tmem + 256 + 128 * x + 64 * h + (wrow << 16);
-        const uint32_t both = 2 + 4 * x + (warp & 3);       // named barrier of the two warps that hold these rows
-        uint32_t done = 0, segs = 0, turns = 0, tiles0 = 0;  // of the items before: key tiles and items of this row tile, tiles with both; all key tiles
-        PackedNote note{};
-        // The warp's 32 rows and 64 dims of an item's q: fetched, and when `before` has waited for the last scores of the item before, scaled, rounded to f16 and
-        // stored swizzled K-major over that item's (rows past the last are zeros).
-        auto bring_q = [&](const PackedItem &it, auto before) -> bool {
-            const uint32_t rows = line_tokens(p.l, it) * G;
-            const float *q0 = p.q + ((size_t)(it.t0 + it.part * p.l.item_tokens) * p.hq + it.kh * G) * D + 64 * h;
-            float4 f[16];
-#pragma unroll
-            for (uint32_t e = 0; e < 16; ++e) {
-                const uint32_t r = 128 * x + wrow + 2 * e + (lane >> 4), token = row_token(p.l, r);
-                f[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (r < rows) f[e] = reinterpret_cast<const float4 *>(q0 + (token * p.hq + r - token * G) * D)[lane & 15];
-            }
-            const bool fine = before();
+        const uint32_t x = warp >> 2, wrow = (warp & 3) * 32, row = wrow + lane;
+        const uint32_t ts = tmem + 128 * x + (wrow << 16), to = tmem + 256 + 128 * x + (wrow << 16);
+        uint32_t used[2] = {0, 0}, all_steps = 0, segs = 0, tiles0 = 0;  // of the shares before: uses of either step's columns, steps and shares of this row tile; all key tiles
+        uint32_t turns = 0;                                              // steps so far with the other row tile beside
+        // The warp's 32 rows of a share's q: fetched, and when `before` has waited for the last scores of the share before, scaled, rounded to f16 and stored
+        // swizzled K-major over that one's (rows past the last are zeros).
+        auto bring_q = [&](const PackedShare &it, auto before) -> bool {
+            const uint32_t rows = it.rows;
+            const float *q0 = p.q + ((size_t)it.t0 * p.hq + it.kh * G) * D;
             uint8_t *to_q = smem + x * TILE_BYTES;
+            bool fine = true;
 #pragma unroll
-            for (uint32_t e = 0; e < 16; ++e) {
-                const __half2 a = __floats2half2_rn(f[e].x * p.scale, f[e].y * p.scale), b = __floats2half2_rn(f[e].z * p.scale, f[e].w * p.scale);
-                *reinterpret_cast<uint2 *>(to_q + tile_piece(wrow + 2 * e + (lane >> 4), 64 * h + 8 * ((lane & 15) >> 1)) + 8 * (lane & 1)) =
-                    make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+            for (uint32_t e0 = 0; e0 < 32; e0 += 16) {
+                float4 f[16];
+#pragma unroll
+                for (uint32_t e = 0; e < 16; ++e) {
+                    const uint32_t r = 128 * x + wrow + e0 + e, token = row_token(p.l, r);
+                    f[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (r < rows) f[e] = reinterpret_cast<const float4 *>(q0 + (token * p.hq + r - token * G) * D)[lane];
+                }
+                if (e0 == 0) fine = before();
+#pragma unroll
+                for (uint32_t e = 0; e < 16; ++e) {
+                    const __half2 a = __floats2half2_rn(f[e].x * p.scale, f[e].y * p.scale), b = __floats2half2_rn(f[e].z * p.scale, f[e].w * p.scale);
+                    *reinterpret_cast<uint2 *>(to_q + tile_piece(wrow + e0 + e, 8 * (lane >> 1)) + 8 * (lane & 1)) =
+                        make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -311,135 +378,136 @@ __global__ void __launch_bounds__(THREADS, 1) attn_packed_tc_kernel(const __grid
             return fine;
         };
         auto nothing = [] { return true; };
-        bool ok = true;
-        if (more && (x == 0 || has_b(item))) ok = bring_q(item, nothing);
+        bool ok = share_at(0);
+        if (ok && shares[0].rows > 128 * x) ok = bring_q(shares[0], nothing);
 #pragma unroll 1
-        while (more && ok) {
-            const uint32_t j0 = item.j, j1 = item_end(), len = j1 - j0, tiles = item.tiles, kh = item.kh, past = item.past + item.part * p.l.item_tokens;
-            const uint32_t t0 = item.t0 + item.part * p.l.item_tokens, rows = line_tokens(p.l, item) * G, r = 128 * x + row;
-            const bool live = r < rows, pairs = rows > 128, used = x == 0 || pairs;
-            const uint32_t seen_all = live ? past + row_token(p.l, r) + 1 : 0;
-            const uint32_t nfree = (past + row_token(p.l, 128 * x) + 1) / 128;  // tiles [0, nfree) lie wholly at or below every row's own position
-            float m = -INFINITY, mneg = 0.0f, l0 = 0.0f, l1 = 0.0f;
-            more = next_item(item, j1);  // (from here on `item` is the next one)
-            const bool fetch = more && (x == 0 || has_b(item));
-            if (!used) {
-                if (fetch) ok = bring_q(item, nothing);
+        for (uint32_t i = 0; ok; ++i) {
+            const PackedShare &share = shares[i % SHARES], &next = shares[(i + 1) % SHARES];
+            const uint32_t rows = share.rows, steps = share.steps, j0 = share.j0;
+            if (rows == 0) break;
+            const uint32_t seen_all = 128 * x + row < rows ? share.past + row_token(p.l, 128 * x + row) + 1 : 0;
+            const uint32_t nfree = (share.past + row_token(p.l, 128 * x) + 1) / 64;  // steps [0, nfree) of all keys lie wholly at or below every row's own position
+            float m = -INFINITY, mneg = 0.0f, l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (rows <= 128 * x) {
+                ok = share_at(i + 1);
+                if (ok && next.rows > 128 * x) ok = bring_q(next, nothing);
             } else {
 #pragma unroll 1
-                for (uint32_t j = j0; j < j1; ++j) {
-                    auto scores = [&] { return all_wait(&s_ready[x], (done + j - j0) & 1); };  // S of this tile, and with it every product issued before: P V of the tile before
-                    if (j + 1 == j1 && fetch) ok = bring_q(item, scores);  // (the next item's queries on the way)
-                    else ok = scores();
+                for (uint32_t k = 0; k < steps; ++k) {
+                    const uint32_t b = k & 1, at = 2 * j0 + k;
+                    auto scores = [&] { return all_wait(&s_ready[x][b], (used[b] + (k >> 1)) & 1); };  // S of this step, and with it every product issued before
+                    if (k + 1 < steps) ok = scores();
+                    else {  // (the next share's queries on the way)
+                        ok = share_at(i + 1);
+                        if (ok && next.rows > 128 * x) ok = bring_q(next, scores);
+                        else ok = scores() && ok;
+                    }
+                    if (!ok) break;  // (what was read of S would count for nothing)
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     uint32_t v[2][32];
-                    tmem_ld32(ts, v[0]);
-                    tmem_ld32(ts + 32, v[1]);
-                    const uint32_t there = there_s[(tiles0 + j - j0) & 7] >> (4 * h) & 15;  // of the four pages of this thread's keys, those that are pages
+                    tmem_ld32(ts + 64 * b, v[0]);
+                    tmem_ld32(ts + 64 * b + 32, v[1]);
+                    const uint32_t there = there_s[(tiles0 + (k >> 1)) & 7] >> (4 * b) & 15;  // of the step's four pages, those that are pages
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (j >= nfree || there != 15) {
-                        const int seen = (int)min(64u, seen_all - min(seen_all, j * 128 + 64 * h));  // of this thread's keys, those the row sees
+                    if (at >= nfree || there != 15) {
+                        const int seen = (int)min(64u, seen_all - min(seen_all, at * 64));  // of the step's keys, those the row sees
 #pragma unroll
-                        for (int i = 0; i < 64; ++i)
-                            if (i >= seen || !(there >> (i >> 4) & 1)) v[i >> 5][i & 31] = 0xff800000u;  // -inf: exp2 gives 0
+                        for (int e = 0; e < 64; ++e)
+                            if (e >= seen || !(there >> (e >> 4) & 1)) v[e >> 5][e & 31] = 0xff800000u;  // -inf: exp2 gives 0
                     }
                     float t[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) t[i] = fmaxf(__uint_as_float(v[0][2 * i]), __uint_as_float(v[0][2 * i + 1]));
+                    for (int e = 0; e < 4; ++e) t[e] = fmaxf(__uint_as_float(v[0][2 * e]), __uint_as_float(v[0][2 * e + 1]));
 #pragma unroll
-                    for (int i = 8; i < 64; i += 2) t[(i >> 1) & 3] = max3(t[(i >> 1) & 3], __uint_as_float(v[i >> 5][i & 31]), __uint_as_float(v[i >> 5][(i & 31) + 1]));
-                    float tmax = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-                    pair[x][h][row] = tmax;
-                    ok = tc_pair_agree(both, ok);  // (after a wait that gave up, what was read of S counts for nothing)
-                    if (!ok) break;
-                    tmax = fmaxf(tmax, pair[x][h ^ 1][row]);
+                    for (int e = 8; e < 64; e += 2) t[(e >> 1) & 3] = max3(t[(e >> 1) & 3], __uint_as_float(v[e >> 5][e & 31]), __uint_as_float(v[e >> 5][(e & 31) + 1]));
+                    const float tmax = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
                     float rescale = 1.0f;
                     bool move = false;
                     if (tmax > m + SLACK || (m == -INFINITY && tmax != -INFINITY)) {
                         move = m != -INFINITY;
                         rescale = move ? ex2((m - tmax) * LOG2E) : 1.0f;
-                        l0 *= rescale;
-                        l1 *= rescale;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) l[e] *= rescale;
                         m = tmax;
                         mneg = -m * LOG2E;
                     }
-                    if (__any_sync(0xffffffffu, move)) {  // what O holds for the row was accumulated against the old reference
+                    if (__any_sync(0xffffffffu, move)) {  // what O holds for the row was accumulated against the old reference; the last product must have ended
+                        ok = all_wait(&pv_done[x], (all_steps + k - 1) & 1);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                        for (uint32_t c = 0; c < 64; c += 8) {
+                        for (uint32_t c = 0; c < 128; c += 8) {
                             uint32_t o[8];
                             tmem_ld8(to + c, o);
                             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * rescale);
+                            for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * rescale);
                             tmem_st8(to + c, o);
                         }
                     }
-                    // The row tiles take turns with the exponentials, A first: side by side both would end late, and both would wait for the tensor core at once.
-                    if (pairs) {
-                        if (x == 1 || turns > 0) {
-                            ok = wait(&turn[x], (turns - (x ^ 1)) & 1);
-                            ok = __all_sync(0xffffffffu, ok);
-                        }
+                    // The row tiles take turns with the exponentials, A first: side by side, both would hold the exponential unit up and then leave it idle.
+                    if (rows > 128) {
+                        if (x == 1 || turns > 0) ok = all_wait(&turn[x], (turns - (x ^ 1)) & 1);
                         ++turns;
                     }
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {  // 16 keys: 8 columns of P (all of this thread's scores are in registers by now)
+                    for (int c = 0; c < 4; ++c) {  // 16 keys: 8 columns of P (all of the row's scores are in registers by now)
+                        if (c == 3 && rows > 128 && lane == 0) tc_mbar_arrive(&turn[x ^ 1]);
+                        float y[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) y[e] = ex2(fmaf(__uint_as_float(v[c >> 1][(c & 1) * 16 + e]), LOG2E, mneg));
                         uint32_t w[8];
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            const int k = 16 * c + i;
-                            const __half2 e = __floats2half2_rn(ex2(fmaf(__uint_as_float(v[k >> 5][k & 31]), LOG2E, mneg)), ex2(fmaf(__uint_as_float(v[k >> 5][(k & 31) + 1]), LOG2E, mneg)));
-                            w[i >> 1] = *reinterpret_cast<const uint32_t *>(&e);
-                            add_halves(w[i >> 1], l0, l1);
+                        for (int e = 0; e < 8; ++e) {
+                            const __half2 pp = __floats2half2_rn(y[2 * e], y[2 * e + 1]);
+                            w[e] = *reinterpret_cast<const uint32_t *>(&pp);
                         }
-                        tmem_st8(ts + 8 * c, w);
-                        if (c == 3 && pairs && lane == 0) tc_mbar_arrive(&turn[x ^ 1]);
-                        if (c & 1) {  // half of P is there for the product
-                            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                            __syncwarp();
-                            if (lane == 0) tc_mbar_arrive(&p_ready[x][c >> 1]);
-                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) add_halves(w[e], l[2 * e & 3], l[(2 * e & 3) + 1]);
+                        tmem_st8(ts + 64 * b + 8 * c, w);
                     }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) tc_mbar_arrive(&p_ready[x][b]);
                 }
-                done += len;
-                // ---- output: O / l, rounded to f16; a part of the item's keys: O, m and l as they are ----
-                ok = ok && wait(&o_done[x], segs & 1);
-                ok = __all_sync(0xffffffffu, ok);
+                used[0] += (steps + 1) / 2;
+                used[1] += steps / 2;
+                all_steps += steps;
+                // ---- output: O / l, rounded to f16, whole rows by way of shared memory; a part of the item's keys: O, m and l as they are ----
+                ok = ok && all_wait(&o_done[x], segs & 1);
                 ++segs;
-                if (ok) pair[x][h][row] = l0 + l1;
-                ok = tc_pair_agree(both, ok);
                 if (!ok) break;
-                const float l = l0 + l1 + pair[x][h ^ 1][row];
-                tc_pair_agree(both, ok);  // (both have read: the next item's scores come there)
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (len < tiles) {
+                const float sum = (l[0] + l[1]) + (l[2] + l[3]);
+                const uint32_t r = 128 * x + row;
+                const bool live = r < rows;
+                if (!share.whole) {
                     float *dst = p.part + (size_t)(2 * blockIdx.x + (j0 == 0)) * packed_part_floats(ROWS);
-                    if (live && h == 0) {
+                    if (live) {
                         dst[ROWS * D + r] = m * LOG2E;
-                        dst[ROWS * D + ROWS + r] = l;
+                        dst[ROWS * D + ROWS + r] = sum;
                     }
 #pragma unroll 1
                     for (uint32_t c = 0; c < 4; ++c) {
-                        uint32_t o[16];
-                        tmem_ld16(to + 16 * c, o);
+                        uint32_t o[32];
+                        tmem_ld32(to + 32 * c, o);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                        for (int g = 0; g < 4; ++g)
-                            if (live) reinterpret_cast<uint4 *>(dst + (size_t)r * D + 64 * h)[4 * c + g] = make_uint4(o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]);
+                        for (int g = 0; g < 8; ++g)
+                            if (live) reinterpret_cast<uint4 *>(dst + (size_t)r * D)[8 * c + g] = make_uint4(o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]);
                     }
                 } else {
-                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                    uint8_t *stage = ring + SLOTS * TILE_BYTES + warp * 2048;  // 32 rows of 32 dims; a piece of 16 bytes goes where no two meet in a bank
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    uint8_t *stage = ring + 4 * TILE_BYTES + warp * 2048;  // 32 rows of 32 dims; a piece of 16 bytes goes where no two meet in a bank
 #pragma unroll 1
-                    for (uint32_t c = 0; c < 2; ++c) {
+                    for (uint32_t c = 0; c < 4; ++c) {
                         uint32_t o[32], packed[16];
                         tmem_ld32(to + 32 * c, o);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const __half2 hh = __floats2half2_rn(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-                            packed[i >> 1] = *reinterpret_cast<const uint32_t *>(&hh);
+                        for (int e = 0; e < 32; e += 2) {
+                            const __half2 hh = __floats2half2_rn(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+                            packed[e >> 1] = *reinterpret_cast<const uint32_t *>(&hh);
                         }
 #pragma unroll
                         for (uint32_t g = 0; g < 4; ++g)
@@ -449,18 +517,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_packed_tc_kernel(const __grid
                         for (uint32_t g = 0; g < 4; ++g) {  // eight rows at a time, 64 bytes of each
                             const uint32_t e = 8 * g + (lane >> 2), re = 128 * x + wrow + e, tk = row_token(p.l, re);
                             const uint4 w = *reinterpret_cast<const uint4 *>(stage + 64 * e + 16 * ((lane & 3) ^ (e >> 1 & 3)));
-                            if (re < rows) reinterpret_cast<uint4 *>(p.o + ((size_t)(t0 + tk) * p.hq + kh * G + re - tk * G) * D + 64 * h + 32 * c)[lane & 3] = w;
+                            if (re < rows) reinterpret_cast<uint4 *>(p.o + ((size_t)(share.t0 + tk) * p.hq + share.kh * G + re - tk * G) * D + 32 * c)[lane & 3] = w;
                         }
                         __syncwarp();
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             }
-            tiles0 += len;
-            if (len < tiles && j0 == 0) note = PackedNote{1, note.closes, t0, rows, kh};
-            if (j0 > 0 && j1 == tiles) note.closes = 1;
+            tiles0 += share.len;
         }
-        if (tid == 0) p.notes[blockIdx.x] = note;
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -473,17 +538,22 @@ __global__ void __launch_bounds__(THREADS, 1) attn_packed_tc_kernel(const __grid
 
 }  // namespace
 
-int32_t brasa_packed_tc_launch(brasa_cmd *cmd, const PackedView &v, const float *q, const uint8_t *kpool, const uint8_t *vpool, void *o, float *part, PackedNote *notes, uint32_t hq,
-                               float scale) {
+int32_t brasa_packed_tc_launch(brasa_cmd *cmd, const PackedView &v, int32_t kv, const float *q, const uint8_t *kpool, const uint8_t *vpool, void *o, float *part, PackedNote *notes,
+                               uint32_t hq, float scale) {
     brasa_ctx *ctx = cmd->ctx;
+    const bool q8 = kv == BRASA_KV_Q8_0;
     PackedMaps maps;
-    const uint64_t dims[3] = {D, v.hkv, (uint64_t)v.num_pages * PAGE}, strides[2] = {256, (uint64_t)v.hkv * 256};
-    const uint32_t box[3] = {64, 1, PAGE};
-    BRASA_TRY(brasa_tmap_bf16(ctx, &maps.k, 3, kpool, dims, strides, box));  // (16-bit values are copied whatever they are)
-    BRASA_TRY(brasa_tmap_bf16(ctx, &maps.v, 3, vpool, dims, strides, box));
-    const PackedTcParams p{packed_line(v, hq / v.hkv, ROWS, 7, 2, 2, 4, PACKED_TC_MIN_ROWS, UINT32_MAX), q, vpool, (__half *)o, part, notes, hq, scale, ctx->status};
-    const size_t smem = (2 + SLOTS) * TILE_BYTES + SOFTMAX_WARPS * 2048;
-    BRASA_TRY(brasa_smem_optin(ctx, (const void *)attn_packed_tc_kernel, smem));
-    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, attn_packed_tc_kernel, dim3(ctx->sm_count), dim3(THREADS), smem, maps, p));
+    memset(&maps, 0, sizeof maps);
+    if (!q8) {
+        const uint64_t dims[3] = {D, v.hkv, (uint64_t)v.num_pages * PAGE}, strides[2] = {256, (uint64_t)v.hkv * 256};
+        const uint32_t box[3] = {64, 1, PAGE};
+        BRASA_TRY(brasa_tmap_bf16(ctx, &maps.k, 3, kpool, dims, strides, box));  // (16-bit values are copied whatever they are)
+        BRASA_TRY(brasa_tmap_bf16(ctx, &maps.v, 3, vpool, dims, strides, box));
+    }
+    const PackedTcParams p{packed_line(v, hq / v.hkv, ROWS, 7, 2, 2, 4, PACKED_TC_MIN_ROWS, UINT32_MAX), q, kpool, vpool, (__half *)o, part, notes, hq, scale, ctx->status};
+    const size_t smem = (2 + 4) * TILE_BYTES + SOFTMAX_WARPS * 2048;
+    void (*const kernel)(PackedMaps, PackedTcParams) = q8 ? attn_packed_tc_kernel<true> : attn_packed_tc_kernel<false>;
+    BRASA_TRY(brasa_smem_optin(ctx, (const void *)kernel, smem));
+    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, kernel, dim3(ctx->sm_count), dim3(q8 ? THREADS_Q8 : THREADS), smem, maps, p));
     return brasa_post_launch(cmd, "attn_packed_tc");
 }

@@ -1,4 +1,4 @@
-// The tensor-core form of the packed attention (packed_tc.cu) for sequences of many rows of an f16 pool, as packed.cu launches it.
+// The tensor-core form of the packed attention (packed_tc.cu) for sequences of many rows of an f16 or 8-bit pool, as packed.cu launches it.
 #pragma once
 #include "packed.cuh"
 
@@ -6,5 +6,5 @@ constexpr uint32_t PACKED_TC_ROWS = 256;     // rows of an item
 constexpr uint32_t PACKED_TC_MIN_ROWS = 65;  // sequences of fewer rows are the other kernel's
 
 // one block per SM; part: two slots of PACKED_TC_ROWS rows each; notes: one each
-int32_t brasa_packed_tc_launch(brasa_cmd *cmd, const brasa_dev::PackedView &v, const float *q, const uint8_t *kpool, const uint8_t *vpool, void *o, float *part,
-                               brasa_dev::PackedNote *notes, uint32_t hq, float scale);
+int32_t brasa_packed_tc_launch(brasa_cmd *cmd, const brasa_dev::PackedView &v, int32_t kv, const float *q, const uint8_t *kpool, const uint8_t *vpool, void *o,
+                               float *part, brasa_dev::PackedNote *notes, uint32_t hq, float scale);

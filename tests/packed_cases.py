@@ -88,6 +88,8 @@ class Run:
                     spread = p @ np.abs(vv - o)
                     ds = 2.0 ** -22 * 130 * (np.abs(kk) @ np.abs(qq)).max() / np.sqrt(D)
                     e = ds * spread + 2.0 ** -22 * (len(p) + 8) * (p @ np.abs(vv))
+                    if (kv or self.kv) != "f32":  # weights enter a product as f16 terms, whose last step is 2^-24 of the largest weight: at most 2^-25 off, or lost below that
+                        e = e + np.minimum(2.0 ** -25, p) @ np.abs(vv)
                     if half:
                         dq = 6 * 2.0 ** -11 / np.sqrt(3) * np.sqrt((kk ** 2) @ (qq ** 2)).max() / np.sqrt(D)
                         if (kv or self.kv) == "q8_0":  # k too, independent of q: the root of two; v: 2^-11 of each, sum p |v| of them at most
