@@ -135,6 +135,7 @@ struct FewParams {
     PackedNote *notes;
     uint32_t hq;
     float scale;
+    uint32_t late_wait;
 };
 constexpr uint32_t FEW_ROWS = 64, FEW_KEYS = 64;
 template <int KV> struct FewStage;
@@ -182,7 +183,10 @@ __device__ __forceinline__ void terms_h2(float x, float y, uint32_t &hi, uint32_
 }
 template <int KV, bool HALF>
 __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_constant__ FewParams p) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // (launched as a programmatic dependent: see brasa_launch_dependent)
+    // Launched as a programmatic dependent. late_wait: the kernel before this one is the same call's tensor-core form, which has itself waited for what both read
+    // and whose output this one does not touch: the two run side by side, and this one waits for the other at its end, so that whoever waits for it has
+    // waited for both.
+    if (!p.late_wait) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     using S = FewStage<KV>;
     constexpr bool Q8 = KV == BRASA_KV_Q8_0;
@@ -197,6 +201,7 @@ __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_const
     PackedNote note{};
     if (!line_cut<128>(p.l, pieces)) {
         if (tid == 0) p.notes[blockIdx.x] = note;
+        if (p.late_wait) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
     PackedItem it = pieces.at[0];
@@ -451,31 +456,42 @@ __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_const
         if (j1 < it.tiles || !line_next(p.l, it)) break;
     }
     if (tid == 0) p.notes[blockIdx.x] = note;
+    if (p.late_wait) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// The items that several blocks worked on: block (b, y) takes the one that piece b began and left open, of it every gridDim.y * 8-th row: the sum of
-// 2^(m - M) O over that of 2^(m - M) l, in the order of the keys.
+// What either kernel left of the items that several blocks worked on.
+struct PackedParts {
+    const float *part;
+    const PackedNote *notes;
+    uint32_t pieces, rows_item, spread;  // blocks, rows of an item, merging blocks to a piece
+};
+// Such an item is the work of the piece that began and left it open, each of that piece's `spread` blocks with every spread * 8-th row: the sum of 2^(m - M) O over
+// that of 2^(m - M) l, in the order of the keys.
 template <bool HALF>
-__global__ void __launch_bounds__(256) attn_packed_merge_kernel(const float *part, const PackedNote *notes, void *o, uint32_t hq, PackedLine l, uint32_t rows_item) {
+__global__ void __launch_bounds__(256) attn_packed_merge_kernel(PackedParts a, PackedParts b, void *o, uint32_t hq, PackedLine l) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const PackedNote n = notes[blockIdx.x];
-    if (!n.opens || blockIdx.x + 1 == gridDim.x) return;  // (the line ends with a whole item)
+    const bool first = blockIdx.x < a.pieces * a.spread;
+    const PackedParts &p = first ? a : b;
+    const uint32_t at = first ? blockIdx.x : blockIdx.x - a.pieces * a.spread, piece = at / p.spread, share = at % p.spread, rows_item = p.rows_item;
+    const float *part = p.part;
+    const PackedNote *notes = p.notes, n = notes[piece];
+    if (!n.opens || piece + 1 == p.pieces) return;  // (the line ends with a whole item)
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t step = packed_part_floats(rows_item);
-    uint32_t last = blockIdx.x + 1;  // the piece that ends the item
-    while (last + 1 < gridDim.x && !notes[last].closes) ++last;
-    for (uint32_t r = blockIdx.y * 8 + warp; r < n.rows; r += gridDim.y * 8) {
+    uint32_t last = piece + 1;  // the piece that ends the item
+    while (last + 1 < p.pieces && !notes[last].closes) ++last;
+    for (uint32_t r = share * 8 + warp; r < n.rows; r += p.spread * 8) {
         const float *ms = part + rows_item * D + r, *ls = ms + rows_item, *os = part + (size_t)r * D + 4 * lane;
         // (slot 2 b + 1 is what piece b left open, slot 2 k piece k's share of an item that began before it)
-        auto slot = [&](uint32_t k) { return (k == blockIdx.x ? 2 * (size_t)k + 1 : 2 * (size_t)k) * step; };
+        auto slot = [&](uint32_t k) { return (k == piece ? 2 * (size_t)k + 1 : 2 * (size_t)k) * step; };
         float M = -INFINITY;
-        for (uint32_t k = blockIdx.x + lane; k <= last; k += 32) M = fmaxf(M, ms[slot(k)]);
+        for (uint32_t k = piece + lane; k <= last; k += 32) M = fmaxf(M, ms[slot(k)]);
         for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
         float L = 0.0f;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-        for (uint32_t k = blockIdx.x; k <= last; ++k) {
+        for (uint32_t k = piece; k <= last; ++k) {
             const float m = ms[slot(k)], f = m == -INFINITY ? 0.0f : exp2_approx(m - M);
             const float4 v = *reinterpret_cast<const float4 *>(os + slot(k));
             L = fmaf(ls[slot(k)], f, L);
@@ -486,9 +502,9 @@ __global__ void __launch_bounds__(256) attn_packed_merge_kernel(const float *par
         }
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
         const uint32_t token = row_token(l, r);
-        const size_t at = ((size_t)(n.t0 + token) * hq + n.kh * l.group + r - token * l.group) * D + 4 * lane;
-        if (HALF) *reinterpret_cast<uint2 *>(static_cast<__half *>(o) + at) = make_uint2(pack_h2(acc.x * inv, acc.y * inv), pack_h2(acc.z * inv, acc.w * inv));
-        else *reinterpret_cast<float4 *>(static_cast<float *>(o) + at) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        const size_t to = ((size_t)(n.t0 + token) * hq + n.kh * l.group + r - token * l.group) * D + 4 * lane;
+        if (HALF) *reinterpret_cast<uint2 *>(static_cast<__half *>(o) + to) = make_uint2(pack_h2(acc.x * inv, acc.y * inv), pack_h2(acc.z * inv, acc.w * inv));
+        else *reinterpret_cast<float4 *>(static_cast<float *>(o) + to) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     }
 }
 
@@ -557,24 +573,19 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
         BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, (few_floats + tc_floats) * sizeof(float) + (blocks + sms) * sizeof(PackedNote)));
         float *few_part = (float *)ctx->packed_work, *tc_part = few_part + few_floats;
         PackedNote *few_notes = (PackedNote *)(tc_part + tc_floats), *tc_notes = few_notes + blocks;
-        auto merge = [&](const float *part, const PackedNote *notes, uint32_t pieces, uint32_t rows_item) {
-            BRASA_CUDA(ctx, brasa_launch_dependent(ctx, half ? attn_packed_merge_kernel<true> : attn_packed_merge_kernel<false>, dim3(pieces, rows_item / 64), dim3(256), 0, part, notes,
-                                                   (void *)arg_ptr(o), hq, packed_line(p, G, rows_item, 0, 0, 0, 0, 0, 0), rows_item));
-            return brasa_post_launch(cmd, "attn_packed_merge");
-        };
-        if (tc) {
-            BRASA_TRY(brasa_packed_tc_launch(cmd, p, pg.kv, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), tc_part, tc_notes, hq, scale));
-            BRASA_TRY(merge(tc_part, tc_notes, sms, PACKED_TC_ROWS));
-        }
+        if (tc) BRASA_TRY(brasa_packed_tc_launch(cmd, p, pg.kv, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), tc_part, tc_notes, hq, scale));
         FewParams f{packed_line(p, G, FEW_ROWS, 6, 1, 1, 3, 1, tc ? PACKED_TC_MIN_ROWS - 1 : UINT32_MAX), (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), few_part,
-                    few_notes, hq, scale};
+                    few_notes, hq, scale, tc ? 1u : 0u};
         void (*const kernel)(FewParams) = pg.kv == BRASA_KV_Q8_0 ? attn_packed_few_kernel<BRASA_KV_Q8_0, true>
                                           : half ? attn_packed_few_kernel<BRASA_KV_F16, true> : attn_packed_few_kernel<BRASA_KV_F16, false>;
         const size_t smem = pg.kv == BRASA_KV_Q8_0 ? FewStage<BRASA_KV_Q8_0>::STAGES * few_stage_bytes<BRASA_KV_Q8_0>() : FewStage<BRASA_KV_F16>::STAGES * few_stage_bytes<BRASA_KV_F16>();
         BRASA_TRY(brasa_smem_optin(ctx, (const void *)kernel, smem));
         BRASA_CUDA(ctx, brasa_launch_dependent(ctx, kernel, dim3(blocks), dim3(128), smem, f));
         BRASA_TRY(brasa_post_launch(cmd, "attn_packed_few"));
-        return merge(few_part, few_notes, blocks, FEW_ROWS);
+        const PackedParts tc_parts{tc_part, tc_notes, tc ? sms : 0u, PACKED_TC_ROWS, 4}, few_parts{few_part, few_notes, blocks, FEW_ROWS, 1};
+        BRASA_CUDA(ctx, brasa_launch_dependent(ctx, half ? attn_packed_merge_kernel<true> : attn_packed_merge_kernel<false>, dim3((tc ? 4 * sms : 0) + blocks), dim3(256), 0, tc_parts,
+                                               few_parts, (void *)arg_ptr(o), hq, packed_line(p, G, FEW_ROWS, 0, 0, 0, 0, 0, 0)));
+        return brasa_post_launch(cmd, "attn_packed_merge");
     }
 #define ATTN_PACKED(KVT)                                                                                                                                  \
     BRASA_CUDA(ctx, brasa_launch_dependent(ctx, half ? attn_packed_rows_kernel<KVT, true> : attn_packed_rows_kernel<KVT, false>, dim3(run.tokens, hkv), dim3(128), 0, \
