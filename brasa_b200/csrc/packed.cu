@@ -10,36 +10,72 @@ namespace {
 constexpr uint32_t PAGE = BRASA_KV_PAGE;
 constexpr int D = 128, TS = D + 4;
 
-// One warp per row of q, k or v of one token: y = x / sqrt(mean x^2 + eps) * w, rotated by the token's own position.
+// y = x / sqrt(mean x^2 + eps) * w of rows of q and k, rotated by the token's own position (pairs i, i + 64), and the store of k and v. Bound by memory: q read
+// and written, k and v read, the cache's rows written. A warp takes four rows of a token (a lane four dims of each, so that a row is one
+// request and a pair's other half lies sixteen lanes on), asks for all of them first and finds the token's sequence, position and page meanwhile.
+constexpr uint32_t STORE_ROWS = 4;
+
+// four dims a lane of one row, rounded to the cache type
 template <int KV>
-__global__ void __launch_bounds__(128) qk_norm_rope_store_packed_kernel(const float *q, const float *k, const float *v, const float *q_norm, const float *k_norm,
+__device__ __forceinline__ void put_row4(uint8_t *row, const float4 &y, uint32_t lane) {
+    if (KV == BRASA_KV_F32) reinterpret_cast<float4 *>(row)[lane] = y;
+    else if (KV == BRASA_KV_F16) {
+        const __half2 a = __floats2half2_rn(y.x, y.y), b = __floats2half2_rn(y.z, y.w);
+        reinterpret_cast<uint2 *>(row)[lane] = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    } else {  // blocks of 32 dims, eight lanes each: the largest magnitude / 127 as f16, codes against that
+        float top = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
+        for (int x = 4; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const __half dh = __float2half_rn(__fdiv_rn(top, 127.0f));
+        const float d = __half2float(dh);
+        auto code = [&](float v) { return (uint32_t)(uint8_t)(int8_t)(d == 0.0f ? 0.0f : fminf(fmaxf(rintf(__fdiv_rn(v, d)), -127.0f), 127.0f)); };
+        reinterpret_cast<uint32_t *>(row)[lane] = code(y.x) | code(y.y) << 8 | code(y.z) << 16 | code(y.w) << 24;
+        if (lane % 8 == 0) reinterpret_cast<__half *>(row + 128)[lane / 8] = dh;
+    }
+}
+
+template <int KV>
+__global__ void __launch_bounds__(256) qk_norm_rope_store_packed_kernel(const float *q, const float *k, const float *v, const float *q_norm, const float *k_norm,
                                                                         const float *cos_t, const float *sin_t, uint8_t *kpool, uint8_t *vpool, PackedView p,
-                                                                        float *q_out, uint32_t hq, float eps, uint64_t rows) {
+                                                                        float *q_out, uint32_t hq, float eps, uint32_t per_tok, uint64_t warps) {
     asm volatile("griddepcontrol.wait;" ::: "memory");  // (launched as a programmatic dependent: see brasa_launch_dependent)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ __align__(16) uint8_t scratch[4][528];
-    const uint64_t gr = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hkv = p.hkv, per_tok = hq + 2 * hkv;
-    if (gr >= rows) return;
-    const uint32_t t = (uint32_t)(gr / per_tok), r = (uint32_t)(gr % per_tok);
+    const uint64_t w = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const uint32_t lane = threadIdx.x & 31, hkv = p.hkv, rows = hq + 2 * hkv;
+    if (w >= warps) return;
+    const uint32_t t = (uint32_t)(w / per_tok), r0 = (uint32_t)(w % per_tok) * STORE_ROWS;
+    float4 x[STORE_ROWS];
+#pragma unroll
+    for (uint32_t e = 0; e < STORE_ROWS; ++e) {
+        const uint32_t r = min(r0 + e, rows - 1);
+        const float *src = r < hq ? q + ((size_t)t * hq + r) * D : (r < hq + hkv ? k + ((size_t)t * hkv + r - hq) * D : v + ((size_t)t * hkv + r - hq - hkv) * D);
+        x[e] = reinterpret_cast<const float4 *>(src)[lane];
+    }
     uint32_t seq, pos;
     if (!packed_row(p, t, lane, seq, pos) || pos / PAGE >= p.max_pages) return;
     const int32_t page = packed_page(p, seq, pos);
     const size_t slot = (size_t)max(page, 0) * PAGE + pos % PAGE;
-    float y[4];
-    if (r >= hq + hkv) {
-        if (page < 0) return;
-        const uint32_t kh = r - hq - hkv;
-        for (int j = 0; j < 4; ++j) y[j] = v[((size_t)t * hkv + kh) * D + lane + 32 * j];
-        put_row<KV>(vpool + (slot * hkv + kh) * KvRow<KV>::BYTES, scratch[warp], y, lane);
-        return;
-    }
-    if (r < hq) {
-        norm_rope_row(q + ((size_t)t * hq + r) * D, q_norm, cos_t, sin_t, pos, eps, lane, y);
-        for (int j = 0; j < 4; ++j) q_out[((size_t)t * hq + r) * D + lane + 32 * j] = y[j];
-    } else if (page >= 0) {
-        norm_rope_row(k + ((size_t)t * hkv + r - hq) * D, k_norm, cos_t, sin_t, pos, eps, lane, y);
-        put_row<KV>(kpool + (slot * hkv + r - hq) * KvRow<KV>::BYTES, scratch[warp], y, lane);
+    const float4 c = reinterpret_cast<const float4 *>(cos_t + (size_t)pos * (D / 2))[lane & 15], s = reinterpret_cast<const float4 *>(sin_t + (size_t)pos * (D / 2))[lane & 15];
+    const float sign = lane < 16 ? -1.0f : 1.0f;
+#pragma unroll
+    for (uint32_t e = 0; e < STORE_ROWS; ++e) {
+        const uint32_t r = r0 + e;
+        if (r >= rows) break;
+        if (r >= hq + hkv) {
+            if (page >= 0) put_row4<KV>(vpool + (slot * hkv + r - hq - hkv) * KvRow<KV>::BYTES, x[e], lane);
+            continue;
+        }
+        float ss = (x[e].x * x[e].x + x[e].y * x[e].y) + (x[e].z * x[e].z + x[e].w * x[e].w);
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float f = 1.0f / sqrtf(ss / (float)D + eps);
+        const float4 n = reinterpret_cast<const float4 *>(r < hq ? q_norm : k_norm)[lane];
+        float4 y = make_float4(x[e].x * f * n.x, x[e].y * f * n.y, x[e].z * f * n.z, x[e].w * f * n.w), o;
+        o.x = __shfl_xor_sync(0xffffffffu, y.x, 16);  // (the pair's other half)
+        o.y = __shfl_xor_sync(0xffffffffu, y.y, 16);
+        o.z = __shfl_xor_sync(0xffffffffu, y.z, 16);
+        o.w = __shfl_xor_sync(0xffffffffu, y.w, 16);
+        y = make_float4(y.x * c.x + sign * o.x * s.x, y.y * c.y + sign * o.y * s.y, y.z * c.z + sign * o.z * s.z, y.w * c.w + sign * o.w * s.w);
+        if (r < hq) reinterpret_cast<float4 *>(q_out + ((size_t)t * hq + r) * D)[lane] = y;
+        else if (page >= 0) put_row4<KV>(kpool + (slot * hkv + r - hq) * KvRow<KV>::BYTES, y, lane);
     }
 }
 
@@ -536,14 +572,15 @@ int32_t brasa_k_qk_norm_rope_store_packed(brasa_cmd *cmd, brasa_arg q, brasa_arg
     BRASA_REQUIRE(ctx, arg_fits(rope_cos, table_bytes) && arg_fits(rope_sin, table_bytes), "qk_norm_rope_store_packed: RoPE tables shorter than max_pages pages");
     for (const brasa_arg *a : {&q, &k, &v, &q_norm, &k_norm, &rope_cos, &rope_sin, &q_out})
         BRASA_REQUIRE(ctx, a->offset % 16 == 0, "qk_norm_rope_store_packed: misaligned buffer");
-    const uint64_t rows = (uint64_t)run.tokens * (hq + 2 * hkv);
-    BRASA_REQUIRE(ctx, rows <= 1ull << 32, "qk_norm_rope_store_packed: more than 2^32 rows");
-    const dim3 grid((uint32_t)((rows + 3) / 4));
+    const uint32_t per_tok = (hq + 2 * hkv + STORE_ROWS - 1) / STORE_ROWS;
+    const uint64_t warps = (uint64_t)run.tokens * per_tok;
+    BRASA_REQUIRE(ctx, warps <= 1ull << 33, "qk_norm_rope_store_packed: more than 2^35 rows");
+    const dim3 grid((uint32_t)((warps + 7) / 8));
 #define STORE_PACKED(KVT)                                                                                                                                       \
-    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, qk_norm_rope_store_packed_kernel<KVT>, grid, dim3(128), 0, (const float *)arg_ptr(q), (const float *)arg_ptr(k), \
+    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, qk_norm_rope_store_packed_kernel<KVT>, grid, dim3(256), 0, (const float *)arg_ptr(q), (const float *)arg_ptr(k), \
                                            (const float *)arg_ptr(v), (const float *)arg_ptr(q_norm), (const float *)arg_ptr(k_norm),                           \
                                            (const float *)arg_ptr(rope_cos), (const float *)arg_ptr(rope_sin), arg_ptr(pg.kpool), arg_ptr(pg.vpool), p,          \
-                                           (float *)arg_ptr(q_out), hq, eps, rows))
+                                           (float *)arg_ptr(q_out), hq, eps, per_tok, warps))
     if (pg.kv == BRASA_KV_F32) STORE_PACKED(BRASA_KV_F32);
     else if (pg.kv == BRASA_KV_F16) STORE_PACKED(BRASA_KV_F16);
     else STORE_PACKED(BRASA_KV_Q8_0);

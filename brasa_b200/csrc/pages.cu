@@ -260,17 +260,30 @@ __global__ void __launch_bounds__(THREADS) pages_compact_kernel(PagePlan p, uint
     }
 }
 
-// Pages in 16-byte pieces; block x of y takes its share of one page of one layer's K or V after the other.
-__global__ void __launch_bounds__(256) pages_copy_kernel(uint8_t *kpool, uint8_t *vpool, const uint32_t *copies, uint32_t pieces, uint32_t layers, uint32_t num_pages) {
+// Pages in 16-byte pieces, COPY_PIECES to a block's turn (four a thread, asked for together); an item is one such part of one page of one layer's K or V.
+constexpr uint32_t COPY_THREADS = 256, COPY_PIECES = 4 * COPY_THREADS;
+__global__ void __launch_bounds__(COPY_THREADS) pages_copy_kernel(uint8_t *kpool, uint8_t *vpool, const uint32_t *copies, uint32_t pieces, uint32_t layers, uint32_t num_pages) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const uint64_t n = copies[0], items = n * layers * 2;
+    const uint32_t parts = (pieces + COPY_PIECES - 1) / COPY_PIECES, planes = 2 * layers, tid = threadIdx.x;
+    const uint64_t items = (uint64_t)copies[0] * planes * parts;
     for (uint64_t it = blockIdx.x; it < items; it += gridDim.x) {
-        const uint64_t c = it % n, plane = it / n;
-        uint4 *pool = reinterpret_cast<uint4 *>(plane & 1 ? vpool : kpool) + (plane >> 1) * num_pages * pieces;
+        const uint32_t part = (uint32_t)(it % parts), plane = (uint32_t)(it / parts % planes);
+        const uint64_t c = it / parts / planes;
+        uint4 *pool = reinterpret_cast<uint4 *>(plane & 1 ? vpool : kpool) + (uint64_t)(plane >> 1) * num_pages * pieces;
         const uint4 *from = pool + (uint64_t)copies[1 + 2 * c] * pieces;
         uint4 *to = pool + (uint64_t)copies[2 + 2 * c] * pieces;
-        for (uint32_t i = threadIdx.x; i < pieces; i += 256) to[i] = from[i];
+        uint4 v[4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+            const uint32_t i = part * COPY_PIECES + u * COPY_THREADS + tid;
+            if (i < pieces) v[u] = from[i];
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+            const uint32_t i = part * COPY_PIECES + u * COPY_THREADS + tid;
+            if (i < pieces) to[i] = v[u];
+        }
     }
 }
 
@@ -303,7 +316,7 @@ uint32_t flag_words(uint32_t num_pages) { return (num_pages + 1023) / 1024 * 32;
 int32_t copy_pages(brasa_cmd *cmd, const brasa_page_pool &g, const PagePlan &p) {
     brasa_ctx *ctx = cmd->ctx;
     const uint32_t pieces = (uint32_t)(brasa_kv_bytes(g.kv, (uint64_t)PAGE * g.hkv * 128) / 16);
-    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, pages_copy_kernel, dim3(ctx->sm_count * 8), dim3(256), 0, arg_ptr(g.kpool), arg_ptr(g.vpool), (const uint32_t *)p.copies, pieces,
+    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, pages_copy_kernel, dim3(ctx->sm_count * 8), dim3(COPY_THREADS), 0, arg_ptr(g.kpool), arg_ptr(g.vpool), (const uint32_t *)p.copies, pieces,
                                            g.layers, g.num_pages));
     return brasa_post_launch(cmd, "pages_copy");
 }

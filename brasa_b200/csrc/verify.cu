@@ -9,7 +9,7 @@
 
 namespace {
 
-constexpr uint32_t THREADS = 512, WARPS = THREADS / 32, CLUSTER = 8;
+constexpr uint32_t CLUSTER = 8, PIECES = 16, UNIT = 128;  // blocks of a sequence, pieces of a block's ids, ids that a warp takes at a time (four a lane)
 
 struct VerifyParams {
     const float *p, *q, *u;
@@ -38,10 +38,12 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) verify_drafts_kernel(VerifyParams a) {
+template <uint32_t THREADS>
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 1024 / THREADS) verify_drafts_kernel(VerifyParams a) {
+    constexpr uint32_t WARPS = THREADS / 32;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // (launched as a programmatic dependent: see brasa_launch_dependent)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ double block_sum[2], warp_sum[WARPS];
+    __shared__ double block_sum[2], piece_sum[PIECES], piece_start[PIECES + 1];
     __shared__ uint32_t stop_s, token_s, last_s;
     const uint32_t s = blockIdx.x / CLUSTER, me = blockIdx.x % CLUSTER, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t first = min(a.starts[s], a.rows), end = max(first, min(a.starts[s + 1], a.rows));
@@ -74,72 +76,103 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) verif
     const bool drafted = stop < n && draft0 + stop < a.ndrafts;
     const float *p = a.p + (size_t)(first + stop) * a.vocab, *q = drafted && a.q ? a.q + (draft0 + stop) * a.vocab : nullptr;
     uint32_t gone = drafted && !a.q ? a.drafts[draft0 + stop] : UINT32_MAX;  // (a given draft: its own probability was 1)
-    // ---- masses of this block's ids, warp by warp; the second time round nothing is subtracted, when nothing was left ----
-    const uint32_t per_block = (a.vocab + CLUSTER - 1) / CLUSTER, b0 = min(me * per_block, a.vocab), b1 = min(b0 + per_block, a.vocab);
-    const uint32_t per_warp = (b1 - b0 + WARPS - 1) / WARPS, w0 = min(b0 + warp * per_warp, b1), w1 = min(w0 + per_warp, b1);
-    auto mass = [&](uint32_t i) -> double {
-        if (i == gone) return 0.0;
-        const double m = q ? (double)p[i] - (double)q[i] : (double)p[i];
-        return m > 0.0 && m < INFINITY ? m : 0.0;
+    // ---- masses of this block's ids, piece by piece; the second time round nothing is subtracted, when nothing was left. Whatever the number of warps,
+    // a piece is the same ids, and a lane adds up the same of them in the same order ----
+    const uint32_t units = (a.vocab + UNIT - 1) / UNIT;
+    auto piece_at = [&](uint32_t n) { return min((uint32_t)((uint64_t)units * (me * PIECES + n) / (CLUSTER * PIECES)) * UNIT, a.vocab); };
+    const bool vec = (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (!q || (reinterpret_cast<uintptr_t>(q) & 15) == 0);
+    auto load4 = [&](const float *row, uint32_t i) {
+        if (vec && i + 4 <= a.vocab) return *reinterpret_cast<const float4 *>(row + i);
+        return make_float4(i < a.vocab ? row[i] : 0.0f, i + 1 < a.vocab ? row[i + 1] : 0.0f, i + 2 < a.vocab ? row[i + 2] : 0.0f, i + 3 < a.vocab ? row[i + 3] : 0.0f);
     };
+    auto masses = [&](uint32_t i, const float4 &x, const float4 &y, double m[4]) {
+        m[0] = (double)x.x - (double)y.x;
+        m[1] = (double)x.y - (double)y.y;
+        m[2] = (double)x.z - (double)y.z;
+        m[3] = (double)x.w - (double)y.w;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+            if (!(m[k] > 0.0 && m[k] < INFINITY) || i + k == gone) m[k] = 0.0;
+    };
+    const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     double total = 0.0, start = 0.0;
     uint32_t last = 0;  // the last of this thread's ids that has mass
     int round = 0;
     for (;; ++round) {
-        double m = 0.0;
-        for (uint32_t i = w0 + lane; i < w1; i += 32) {
-            const double x = mass(i);
-            if (x > 0.0) last = i;
-            m += x;
-        }
-        for (int x = 16; x > 0; x >>= 1) m += __shfl_xor_sync(0xffffffffu, m, x);
-        if (lane == 0) warp_sum[warp] = m;
-        __syncthreads();
-        if (tid == 0) {
+        for (uint32_t n = warp; n < PIECES; n += WARPS) {
+            const uint32_t end_id = piece_at(n + 1);
             double sum = 0.0;
-            for (uint32_t w = 0; w < WARPS; ++w) sum += warp_sum[w];
-            block_sum[round] = sum;
+#pragma unroll 4
+            for (uint32_t i = piece_at(n) + 4 * lane; i < end_id; i += UNIT) {
+                double m[4];
+                masses(i, load4(p, i), q ? load4(q, i) : none, m);
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k)
+                    if (m[k] > 0.0) last = i + k;
+                sum += (m[0] + m[1]) + (m[2] + m[3]);
+            }
+            for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            if (lane == 0) piece_sum[n] = sum;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            double v = lane < PIECES ? piece_sum[lane] : 0.0;
+            for (uint32_t x = 1; x < PIECES; x <<= 1) {
+                const double o = __shfl_up_sync(0xffffffffu, v, x);
+                if (lane >= x) v += o;
+            }
+            if (lane < PIECES) piece_start[lane + 1] = v;
+            if (lane == 0) piece_start[0] = 0.0;
+            if (lane == PIECES - 1) block_sum[round] = v;
         }
         cluster_sync();
+        double sums[CLUSTER];
+#pragma unroll
+        for (uint32_t r = 0; r < CLUSTER; ++r) sums[r] = cluster_double(&block_sum[round], r);
         total = start = 0.0;
+#pragma unroll
         for (uint32_t r = 0; r < CLUSTER; ++r) {
-            const double b = cluster_double(&block_sum[round], r);
-            if (r < me) start += b;
-            total += b;
+            if (r < me) start += sums[r];
+            total += sums[r];
         }
         if (total > 0.0 || round == 1) break;
         q = nullptr;
         gone = UINT32_MAX;
     }
-    // ---- the first id at which the running sum exceeds the point. A warp's piece of [0, total) ends where the next one's begins, in the very
-    // same sums, so one warp holds the point; two can only where rounding moved a block's end by a bit, and then the lower id counts ----
-    const double point = (double)a.u[end - 1] * total, block_end = start + block_sum[round];
-    for (uint32_t w = 0; w < warp; ++w) start += warp_sum[w];
-    const double piece_end = warp + 1 < WARPS ? start + warp_sum[warp] : block_end;
-    if (start <= point && point < piece_end) {
-        uint32_t id = UINT32_MAX;
-        for (uint32_t i0 = w0; i0 < w1 && id == UINT32_MAX; i0 += 256) {  // eight ids per lane
-            double m[8], sum = 0.0;
-            for (uint32_t k = 0; k < 8; ++k) {
-                const uint32_t i = i0 + 8 * lane + k;
-                m[k] = i < w1 ? mass(i) : 0.0;
-                sum += m[k];
-            }
+    // ---- the first id at which the running sum exceeds the point. A piece of [0, total) ends where the next one begins, in the very same sums, so one
+    // holds the point; two can only where rounding moved an end by a bit, and then the lower id counts ----
+    const double point = (double)a.u[end - 1] * total, block_start = start, block_end = start + block_sum[round];
+    for (uint32_t n = warp; n < PIECES; n += WARPS) {
+        const uint32_t end_id = piece_at(n + 1);
+        start = block_start + piece_start[n];
+        const double piece_end = n + 1 < PIECES ? block_start + piece_start[n + 1] : block_end;
+        if (!(start <= point && point < piece_end)) continue;
+        uint32_t id = UINT32_MAX, held = 0;
+        float4 x = load4(p, piece_at(n) + 4 * lane), y = q ? load4(q, piece_at(n) + 4 * lane) : none;
+        for (uint32_t i0 = piece_at(n); i0 < end_id && id == UINT32_MAX; i0 += UNIT) {
+            const uint32_t i = i0 + 4 * lane;
+            double m[4];
+            masses(i, x, y, m);
+            x = load4(p, i + UNIT);
+            y = q ? load4(q, i + UNIT) : none;
+            const double sum = (m[0] + m[1]) + (m[2] + m[3]);
             double upto = sum;
-            for (uint32_t x = 1; x < 32; x <<= 1) {
-                const double v = __shfl_up_sync(0xffffffffu, upto, x);
-                if (lane >= x) upto += v;
+            for (uint32_t z = 1; z < 32; z <<= 1) {
+                const double v = __shfl_up_sync(0xffffffffu, upto, z);
+                if (lane >= z) upto += v;
             }
             uint32_t mine = UINT32_MAX;
             double run = start + (upto - sum);
-            for (uint32_t k = 0; k < 8; ++k) {
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
                 run += m[k];
-                if (mine == UINT32_MAX && m[k] > 0.0 && run > point) mine = i0 + 8 * lane + k;
+                if (m[k] > 0.0) held = i + k;
+                if (mine == UINT32_MAX && m[k] > 0.0 && run > point) mine = i + k;
             }
             id = __reduce_min_sync(0xffffffffu, mine);
             start += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (id == UINT32_MAX) id = __reduce_max_sync(0xffffffffu, last);  // (rounding: the piece's last mass)
+        if (id == UINT32_MAX) id = __reduce_max_sync(0xffffffffu, held);  // (rounding: the piece's last mass)
         if (lane == 0) atomicMin(&token_s, id);
     }
     last = __reduce_max_sync(0xffffffffu, last);
@@ -180,6 +213,8 @@ extern "C" int32_t brasa_k_verify_drafts(brasa_cmd *cmd, brasa_arg p, brasa_arg 
     VerifyParams a{(const float *)arg_ptr(p), (const float *)arg_ptr(q), (const float *)arg_ptr(u), (const uint32_t *)arg_ptr(drafts), (const uint32_t *)arg_ptr(starts),
                    (uint32_t *)arg_ptr(tokens), (uint32_t *)arg_ptr(accepted), seqs, rows, vocab, drafts.buf ? (drafts.buf->bytes - drafts.offset) / 4 : 0};
     if (q.buf) a.ndrafts = std::min(a.ndrafts, (q.buf->bytes - q.offset) / 4 / vocab);
-    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, verify_drafts_kernel, dim3(seqs * CLUSTER), dim3(THREADS), 0, a));
+    // 16 warps a block while the blocks fit the SMs' places in one go (two to an SM), eight where there are more: 64 sequences of 151 936 ids with q 23 us (3.4 TB/s), one without 9.3.
+    const bool wide = seqs * CLUSTER <= 2 * (uint32_t)ctx->sm_count;
+    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, wide ? verify_drafts_kernel<512> : verify_drafts_kernel<256>, dim3(seqs * CLUSTER), dim3(wide ? 512 : 256), 0, a));
     return brasa_post_launch(cmd, "verify_drafts");
 }
