@@ -8,7 +8,7 @@ using namespace brasa_dev;
 namespace {
 
 constexpr uint32_t PAGE = BRASA_KV_PAGE;
-constexpr int D = 128, TS = D + 4;
+constexpr int D = 128;
 
 // y = x / sqrt(mean x^2 + eps) * w of rows of q and k, rotated by the token's own position (pairs i, i + 64), and the store of k and v. Bound by memory: q read
 // and written, k and v read, the cache's rows written. A warp takes four rows of a token (a lane four dims of each, so that a row is one
@@ -76,82 +76,6 @@ __global__ void __launch_bounds__(256) qk_norm_rope_store_packed_kernel(const fl
         y = make_float4(y.x * c.x + sign * o.x * s.x, y.y * c.y + sign * o.y * s.y, y.z * c.z + sign * o.z * s.z, y.w * c.w + sign * o.w * s.w);
         if (r < hq) reinterpret_cast<float4 *>(q_out + ((size_t)t * hq + r) * D)[lane] = y;
         else if (page >= 0) put_row4<KV>(kpool + (slot * hkv + r - hq) * KvRow<KV>::BYTES, y, lane);
-    }
-}
-
-// One block per token and key head: the group's rows against 64 keys at a time, K and V as f32 in shared memory, a running maximum, sum
-// and output per row.
-template <int KV, bool HALF_OUT>
-__global__ void __launch_bounds__(128) attn_packed_rows_kernel(const float *q, const uint8_t *kpool, const uint8_t *vpool, PackedView p, void *o, uint32_t hq,
-                                                               float scale) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    constexpr uint32_t KEYS = 64;
-    __shared__ __align__(16) float ts[KEYS * TS], qs[8 * D], ps[8 * KEYS];
-    __shared__ float ms[8], ls[8], alpha[8];
-    const uint32_t t = blockIdx.x, kh = blockIdx.y, hkv = p.hkv, G = hq / hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t seq, pos;
-    if (!packed_row(p, t, lane, seq, pos) || pos / PAGE >= p.max_pages) return;
-    const uint32_t nkeys = pos + 1;
-    for (uint32_t i = tid; i < G * D; i += 128) qs[i] = q[((size_t)t * hq + kh * G) * D + i];
-    if (tid < 8) {
-        ms[tid] = -INFINITY;
-        ls[tid] = 0.0f;
-    }
-    float acc[8];
-    for (int g = 0; g < 8; ++g) acc[g] = 0.0f;
-    auto load = [&](const uint8_t *pool, uint32_t key0) {
-        for (uint32_t i = tid; i < KEYS * (D / 8); i += 128) {
-            const uint32_t key = key0 + i / (D / 8), v8 = i % (D / 8);
-            const int32_t page = key < nkeys ? packed_page(p, seq, key) : -1;
-            float v[8] = {};
-            if (page >= 0) tile_load8<KV>(pool + (((size_t)page * PAGE + key % PAGE) * hkv + kh) * KvRow<KV>::BYTES, (int)(v8 * 8), v);
-            for (int j = 0; j < 8; ++j) ts[(i / (D / 8)) * TS + v8 * 8 + j] = v[j];
-        }
-    };
-    for (uint32_t key0 = 0; key0 < nkeys; key0 += KEYS) {
-        load(kpool, key0);
-        __syncthreads();
-        const uint32_t key = key0 + (tid & 63);
-        const bool there = key < nkeys && packed_page(p, seq, key) >= 0;
-        for (uint32_t g = tid >> 6; g < G; g += 2) {
-            float a = 0.0f;
-            for (int d = 0; d < D; ++d) a = fmaf(qs[g * D + d], ts[(tid & 63) * TS + d], a);
-            ps[g * KEYS + (tid & 63)] = there ? a * scale : -INFINITY;
-        }
-        __syncthreads();
-        load(vpool, key0);
-        for (uint32_t g = warp; g < G; g += 4) {
-            const float s0 = ps[g * KEYS + lane], s1 = ps[g * KEYS + 32 + lane];
-            float m = fmaxf(s0, s1);
-            for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-            const float before = ms[g], now = fmaxf(before, m);
-            const float p0 = s0 == -INFINITY ? 0.0f : expf(s0 - now), p1 = s1 == -INFINITY ? 0.0f : expf(s1 - now);
-            float l = p0 + p1;
-            for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-            ps[g * KEYS + lane] = p0;
-            ps[g * KEYS + 32 + lane] = p1;
-            __syncwarp();
-            if (lane == 0) {
-                const float a = before == -INFINITY ? 0.0f : expf(before - now);
-                alpha[g] = a;
-                ls[g] = ls[g] * a + l;
-                ms[g] = now;
-            }
-        }
-        __syncthreads();
-        for (uint32_t g = 0; g < G; ++g) {
-            float a = acc[g] * alpha[g];
-            for (uint32_t j = 0; j < KEYS; ++j) a = fmaf(ps[g * KEYS + j], ts[j * TS + tid], a);
-            acc[g] = a;
-        }
-        __syncthreads();
-    }
-    for (uint32_t g = 0; g < G; ++g) {
-        const float r = ls[g] == 0.0f ? 0.0f : acc[g] / ls[g];
-        const size_t at = ((size_t)t * hq + kh * G + g) * D + tid;
-        if (HALF_OUT) static_cast<__half *>(o)[at] = __float2half_rn(r);
-        else static_cast<float *>(o)[at] = r;
     }
 }
 
@@ -495,6 +419,192 @@ __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_const
     if (p.late_wait) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// ---- 32-bit arithmetic: an f32 cache, or an 8-bit one whose values keep all their bits -------------------------------------------------------------
+// A block has up to 64 rows and takes 64 keys at a time as f32 in shared memory, K's next tile on its way while V's is used. 256 threads in a square: scores four
+// rows by four keys each (keys 16 apart, so that a quarter warp's reads of K meet in no bank), outputs four rows by eight dims. Bound by the FMA units
+// with many rows, by the cache's bytes with few.
+constexpr uint32_t F32_THREADS = 256, F32_P = 68;
+constexpr size_t F32_SMEM = (3 * 64 * (size_t)FEW_TS + 64 * F32_P) * sizeof(float);
+
+template <int KV, bool HALF>
+__global__ void __launch_bounds__(F32_THREADS) attn_packed_f32_kernel(const __grid_constant__ FewParams p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    extern __shared__ __align__(16) float fs[];
+    __shared__ PackedPieces pieces;
+    float *qs = fs, *ks = qs + 64 * FEW_TS, *vs = ks + 64 * FEW_TS, *ps = vs + 64 * FEW_TS;
+    const uint32_t tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, hkv = p.l.v.hkv, G = p.l.group;
+    PackedNote note{};
+    if (!line_cut<F32_THREADS>(p.l, pieces)) {
+        if (tid == 0) p.notes[blockIdx.x] = note;
+        return;
+    }
+    PackedItem it = pieces.at[0];
+    const uint64_t end_first = pieces.at[1].first;
+    const uint32_t end_j = pieces.at[1].j;
+    if (it.j == it.tiles) line_next(p.l, it);
+    const float c = p.scale * 1.4426950408889634f;
+    while (it.first < end_first || (it.first == end_first && it.j < end_j)) {
+        const uint32_t j0 = it.j, j1 = it.first == end_first ? end_j : it.tiles, token0 = it.part * p.l.item_tokens, t0 = it.t0 + token0, rows = line_tokens(p.l, it) * G, nkeys = line_keys(p.l, it);
+        const int32_t *table = p.l.v.table + (size_t)it.seq * p.l.v.max_pages;
+        auto page_at = [&](uint32_t key) {  // of a position, -1 where there is none or nothing is seen
+            const int32_t page = key < nkeys ? table[key / PAGE] : -1;
+            return (uint32_t)page < p.l.v.num_pages ? page : -1;
+        };
+        auto fetch = [&](float *to, const uint8_t *pool, uint32_t j) {  // 64 rows, what is not there as zeros
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) {
+                const uint32_t i = tid + F32_THREADS * u, row = i >> 5, pc = i & 31, key = 64 * j + row;
+                const int32_t page = j < j1 ? page_at(key) : -1;
+                const uint8_t *src = pool + (((size_t)max(page, 0) * PAGE + (key & 15)) * hkv + it.kh) * KvRow<KV>::BYTES;
+                if (KV == BRASA_KV_F32) cp_zfill16((uint32_t)__cvta_generic_to_shared(to + row * FEW_TS + 4 * pc), src + 16 * pc, page >= 0);
+                else {
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (page >= 0) {
+                        const char4 q = reinterpret_cast<const char4 *>(src)[pc];
+                        const float d = __half2float(reinterpret_cast<const __half *>(src + 128)[pc >> 3]);
+                        v = make_float4(d * (float)q.x, d * (float)q.y, d * (float)q.z, d * (float)q.w);
+                    }
+                    *reinterpret_cast<float4 *>(to + row * FEW_TS + 4 * pc) = v;
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        fetch(ks, p.kpool, j0);
+        for (uint32_t i = tid; i < 64 * 32; i += F32_THREADS) {
+            const uint32_t r = i >> 5, token = row_token(p.l, r);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (r < rows) v = reinterpret_cast<const float4 *>(p.q + ((size_t)(t0 + token) * p.hq + it.kh * G + r - token * G) * D)[i & 31];
+            *reinterpret_cast<float4 *>(qs + r * FEW_TS + 4 * (i & 31)) = v;
+        }
+        float m[4], l[4], o[4][8];
+        uint32_t seen[4];
+#pragma unroll
+        for (uint32_t a = 0; a < 4; ++a) {
+            const uint32_t r = 4 * ty + a;
+            seen[a] = r < rows ? it.past + token0 + row_token(p.l, r) + 1 : 0;
+            m[a] = -INFINITY;
+            l[a] = 0.0f;
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) o[a][e] = 0.0f;
+        }
+        const bool live = 4 * ty < rows;
+        for (uint32_t j = j0; j < j1; ++j) {
+            fetch(vs, p.vpool, j);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncthreads();  // K and q are there
+            float s[4][4];
+#pragma unroll
+            for (uint32_t a = 0; a < 4; ++a)
+#pragma unroll
+                for (uint32_t b = 0; b < 4; ++b) s[a][b] = 0.0f;
+            if (live) {
+#pragma unroll 4
+                for (uint32_t d = 0; d < D; d += 4) {
+                    float4 x[4], y[4];
+#pragma unroll
+                    for (uint32_t a = 0; a < 4; ++a) x[a] = *reinterpret_cast<const float4 *>(qs + (4 * ty + a) * FEW_TS + d);
+#pragma unroll
+                    for (uint32_t b = 0; b < 4; ++b) y[b] = *reinterpret_cast<const float4 *>(ks + (tx + 16 * b) * FEW_TS + d);
+#pragma unroll
+                    for (uint32_t a = 0; a < 4; ++a)
+#pragma unroll
+                        for (uint32_t b = 0; b < 4; ++b)
+                            s[a][b] = fmaf(x[a].w, y[b].w, fmaf(x[a].z, y[b].z, fmaf(x[a].y, y[b].y, fmaf(x[a].x, y[b].x, s[a][b]))));
+                }
+                bool there[4];
+#pragma unroll
+                for (uint32_t b = 0; b < 4; ++b) there[b] = page_at(64 * j + 16 * b) >= 0;  // (a thread's keys lie a page apart)
+#pragma unroll
+                for (uint32_t a = 0; a < 4; ++a) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (uint32_t b = 0; b < 4; ++b) {
+                        s[a][b] = there[b] && 64 * j + tx + 16 * b < seen[a] ? s[a][b] * c : -INFINITY;
+                        top = fmaxf(top, s[a][b]);
+                    }
+                    for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffu << (tid & 16), top, x));
+                    const float now = fmaxf(m[a], top), ref = now == -INFINITY ? 0.0f : now, f = m[a] == -INFINITY ? 0.0f : exp2_approx(m[a] - ref);
+                    m[a] = now;
+                    l[a] *= f;
+#pragma unroll
+                    for (uint32_t b = 0; b < 4; ++b) {
+                        const float w = exp2_approx(s[a][b] - ref);
+                        l[a] += w;
+                        ps[(4 * ty + a) * F32_P + tx + 16 * b] = w;
+                    }
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) o[a][e] *= f;
+                }
+            }
+            __syncthreads();  // K is done with
+            fetch(ks, p.kpool, j + 1);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncthreads();  // V is there
+            if (live) {
+#pragma unroll 2
+                for (uint32_t k = 0; k < 64; k += 4) {
+                    float4 w[4];
+#pragma unroll
+                    for (uint32_t a = 0; a < 4; ++a) w[a] = *reinterpret_cast<const float4 *>(ps + (4 * ty + a) * F32_P + k);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        const float4 y0 = *reinterpret_cast<const float4 *>(vs + (k + e) * FEW_TS + 4 * tx), y1 = *reinterpret_cast<const float4 *>(vs + (k + e) * FEW_TS + 64 + 4 * tx);
+#pragma unroll
+                        for (uint32_t a = 0; a < 4; ++a) {
+                            const float f = e == 0 ? w[a].x : (e == 1 ? w[a].y : (e == 2 ? w[a].z : w[a].w));
+                            o[a][0] = fmaf(f, y0.x, o[a][0]);
+                            o[a][1] = fmaf(f, y0.y, o[a][1]);
+                            o[a][2] = fmaf(f, y0.z, o[a][2]);
+                            o[a][3] = fmaf(f, y0.w, o[a][3]);
+                            o[a][4] = fmaf(f, y1.x, o[a][4]);
+                            o[a][5] = fmaf(f, y1.y, o[a][5]);
+                            o[a][6] = fmaf(f, y1.z, o[a][6]);
+                            o[a][7] = fmaf(f, y1.w, o[a][7]);
+                        }
+                    }
+                }
+            }
+            __syncthreads();  // V and the weights are done with
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        const bool whole = j0 == 0 && j1 == it.tiles;
+        float *part = p.part + (size_t)(2 * blockIdx.x + (j0 == 0)) * packed_part_floats(FEW_ROWS);
+        if (live) {
+#pragma unroll
+            for (uint32_t a = 0; a < 4; ++a) {
+                const uint32_t r = 4 * ty + a;
+                for (int x = 8; x > 0; x >>= 1) l[a] += __shfl_xor_sync(0xffffu << (tid & 16), l[a], x);
+                if (r >= rows) continue;
+                if (whole) {
+                    const uint32_t token = row_token(p.l, r);
+                    const size_t at = ((size_t)(t0 + token) * p.hq + it.kh * G + r - token * G) * D + 4 * tx;
+                    const float inv = l[a] == 0.0f ? 0.0f : 1.0f / l[a];
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        const float4 v = make_float4(o[a][4 * e] * inv, o[a][4 * e + 1] * inv, o[a][4 * e + 2] * inv, o[a][4 * e + 3] * inv);
+                        if (HALF) *reinterpret_cast<uint2 *>(static_cast<__half *>(p.o) + at + 64 * e) = make_uint2(pack_h2(v.x, v.y), pack_h2(v.z, v.w));
+                        else *reinterpret_cast<float4 *>(static_cast<float *>(p.o) + at + 64 * e) = v;
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e)
+                        *reinterpret_cast<float4 *>(part + r * D + 64 * e + 4 * tx) = make_float4(o[a][4 * e], o[a][4 * e + 1], o[a][4 * e + 2], o[a][4 * e + 3]);
+                    if (tx == 0) {
+                        part[FEW_ROWS * D + r] = m[a];
+                        part[FEW_ROWS * D + FEW_ROWS + r] = l[a];
+                    }
+                }
+            }
+        }
+        if (!whole && j0 == 0) note = PackedNote{1, note.closes, t0, rows, it.kh};
+        if (j0 > 0 && j1 == it.tiles) note.closes = 1;
+        __syncthreads();  // (q's place is free)
+        if (j1 < it.tiles || !line_next(p.l, it)) break;
+    }
+    if (tid == 0) p.notes[blockIdx.x] = note;
+}
+
 // What either kernel left of the items that several blocks worked on.
 struct PackedParts {
     const float *part;
@@ -598,40 +708,40 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
     const uint64_t n = (uint64_t)run.tokens * hq * D;
     BRASA_REQUIRE(ctx, arg_fits(q, n * 4) && arg_fits(o, n * (half ? 2 : 4)), "attention_packed: q or o too small");
     BRASA_REQUIRE(ctx, q.offset % 16 == 0 && o.offset % 16 == 0, "attention_packed: misaligned buffer");
-    BRASA_REQUIRE(ctx, run.tokens < 1u << 31 && hkv <= 65535, "attention_packed: more than 2^31 tokens or 65 535 key heads");
     BRASA_REQUIRE(ctx, (uint64_t)run.tokens * (hq / hkv) < 1ull << 31, "attention_packed: more than 2^31 rows of a key head's group");
     const float scale = 1.0f / sqrtf((float)D);
-    if (pg.kv == BRASA_KV_F16 || (pg.kv == BRASA_KV_Q8_0 && half)) {
-        // Sequences of many rows go to the tensor-core kernel where there is one (16-bit products) and the call can have any.
-        const uint32_t G = hq / hkv, sms = ctx->sm_count, blocks = sms * 2;
-        const bool tc = half && (uint64_t)run.longest * G >= PACKED_TC_MIN_ROWS && (uint64_t)pg.num_pages * PAGE < 1ull << 31;
-        // the workspace: parts of either kernel's items, then what they belong to
-        const size_t few_floats = 2 * (size_t)blocks * packed_part_floats(FEW_ROWS), tc_floats = 2 * (size_t)sms * packed_part_floats(PACKED_TC_ROWS);
-        BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, (few_floats + tc_floats) * sizeof(float) + (blocks + sms) * sizeof(PackedNote)));
-        float *few_part = (float *)ctx->packed_work, *tc_part = few_part + few_floats;
-        PackedNote *few_notes = (PackedNote *)(tc_part + tc_floats), *tc_notes = few_notes + blocks;
-        if (tc) BRASA_TRY(brasa_packed_tc_launch(cmd, p, pg.kv, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), tc_part, tc_notes, hq, scale));
-        FewParams f{packed_line(p, G, FEW_ROWS, 6, 1, 1, 3, 1, tc ? PACKED_TC_MIN_ROWS - 1 : UINT32_MAX), (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), few_part,
-                    few_notes, hq, scale, tc ? 1u : 0u};
-        void (*const kernel)(FewParams) = pg.kv == BRASA_KV_Q8_0 ? attn_packed_few_kernel<BRASA_KV_Q8_0, true>
-                                          : half ? attn_packed_few_kernel<BRASA_KV_F16, true> : attn_packed_few_kernel<BRASA_KV_F16, false>;
-        const size_t smem = pg.kv == BRASA_KV_Q8_0 ? FewStage<BRASA_KV_Q8_0>::STAGES * few_stage_bytes<BRASA_KV_Q8_0>() : FewStage<BRASA_KV_F16>::STAGES * few_stage_bytes<BRASA_KV_F16>();
-        BRASA_TRY(brasa_smem_optin(ctx, (const void *)kernel, smem));
-        BRASA_CUDA(ctx, brasa_launch_dependent(ctx, kernel, dim3(blocks), dim3(128), smem, f));
-        BRASA_TRY(brasa_post_launch(cmd, "attn_packed_few"));
-        const PackedParts tc_parts{tc_part, tc_notes, tc ? sms : 0u, PACKED_TC_ROWS, 4}, few_parts{few_part, few_notes, blocks, FEW_ROWS, 1};
-        BRASA_CUDA(ctx, brasa_launch_dependent(ctx, half ? attn_packed_merge_kernel<true> : attn_packed_merge_kernel<false>, dim3((tc ? 4 * sms : 0) + blocks), dim3(256), 0, tc_parts,
-                                               few_parts, (void *)arg_ptr(o), hq, packed_line(p, G, FEW_ROWS, 0, 0, 0, 0, 0, 0)));
-        return brasa_post_launch(cmd, "attn_packed_merge");
+    // Sequences of many rows go to the tensor-core kernel where there is one (16-bit products) and the call can have any. What is neither an f16 cache nor 16-bit
+    // products of an 8-bit one is computed in 32 bits.
+    const uint32_t G = hq / hkv, sms = ctx->sm_count;
+    const bool f32 = pg.kv == BRASA_KV_F32 || (pg.kv == BRASA_KV_Q8_0 && !half);
+    const bool tc = half && !f32 && (uint64_t)run.longest * G >= PACKED_TC_MIN_ROWS && (uint64_t)pg.num_pages * PAGE < 1ull << 31;
+    const uint32_t blocks = f32 ? sms : 2 * sms;
+    // the workspace: parts of either kernel's items, then what they belong to
+    const size_t few_floats = 2 * (size_t)(2 * sms) * packed_part_floats(FEW_ROWS), tc_floats = 2 * (size_t)sms * packed_part_floats(PACKED_TC_ROWS);
+    BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, (few_floats + tc_floats) * sizeof(float) + 3 * sms * sizeof(PackedNote)));
+    float *few_part = (float *)ctx->packed_work, *tc_part = few_part + few_floats;
+    PackedNote *few_notes = (PackedNote *)(tc_part + tc_floats), *tc_notes = few_notes + 2 * sms;
+    if (tc) BRASA_TRY(brasa_packed_tc_launch(cmd, p, pg.kv, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), tc_part, tc_notes, hq, scale));
+    const FewParams f{packed_line(p, G, FEW_ROWS, 6, 1, 1, 3, 1, tc ? PACKED_TC_MIN_ROWS - 1 : UINT32_MAX), (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), few_part,
+                      few_notes, hq, scale, tc ? 1u : 0u};
+    void (*kernel)(FewParams);
+    size_t smem = F32_SMEM;
+    if (f32) {
+        kernel = pg.kv == BRASA_KV_Q8_0 ? attn_packed_f32_kernel<BRASA_KV_Q8_0, false> : half ? attn_packed_f32_kernel<BRASA_KV_F32, true> : attn_packed_f32_kernel<BRASA_KV_F32, false>;
+    } else if (pg.kv == BRASA_KV_Q8_0) {
+        kernel = attn_packed_few_kernel<BRASA_KV_Q8_0, true>;
+        smem = FewStage<BRASA_KV_Q8_0>::STAGES * few_stage_bytes<BRASA_KV_Q8_0>();
+    } else {
+        kernel = half ? attn_packed_few_kernel<BRASA_KV_F16, true> : attn_packed_few_kernel<BRASA_KV_F16, false>;
+        smem = FewStage<BRASA_KV_F16>::STAGES * few_stage_bytes<BRASA_KV_F16>();
     }
-#define ATTN_PACKED(KVT)                                                                                                                                  \
-    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, half ? attn_packed_rows_kernel<KVT, true> : attn_packed_rows_kernel<KVT, false>, dim3(run.tokens, hkv), dim3(128), 0, \
-                                           (const float *)arg_ptr(q), (const uint8_t *)arg_ptr(pg.kpool), (const uint8_t *)arg_ptr(pg.vpool), p, (void *)arg_ptr(o), hq, scale))
-    if (pg.kv == BRASA_KV_F32) ATTN_PACKED(BRASA_KV_F32);
-    else if (pg.kv == BRASA_KV_F16) ATTN_PACKED(BRASA_KV_F16);
-    else ATTN_PACKED(BRASA_KV_Q8_0);
-#undef ATTN_PACKED
-    return brasa_post_launch(cmd, "attn_packed_rows");
+    BRASA_TRY(brasa_smem_optin(ctx, (const void *)kernel, smem));
+    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, kernel, dim3(blocks), dim3(f32 ? F32_THREADS : 128), smem, f));
+    BRASA_TRY(brasa_post_launch(cmd, f32 ? "attn_packed_f32" : "attn_packed_few"));
+    const PackedParts tc_parts{tc_part, tc_notes, tc ? sms : 0u, PACKED_TC_ROWS, 4}, few_parts{few_part, few_notes, blocks, FEW_ROWS, 1};
+    BRASA_CUDA(ctx, brasa_launch_dependent(ctx, half ? attn_packed_merge_kernel<true> : attn_packed_merge_kernel<false>, dim3((tc ? 4 * sms : 0) + blocks), dim3(256), 0, tc_parts,
+                                           few_parts, (void *)arg_ptr(o), hq, packed_line(p, G, FEW_ROWS, 0, 0, 0, 0, 0, 0)));
+    return brasa_post_launch(cmd, "attn_packed_merge");
 }
 
 }  // extern "C"
