@@ -99,9 +99,9 @@ struct FewParams {
 };
 constexpr uint32_t FEW_ROWS = 64, FEW_KEYS = 64;
 template <int KV> struct FewStage;
-template <> struct FewStage<BRASA_KV_F16> { static constexpr uint32_t K_PITCH = 256, V_PITCH = 256, STAGES = 3; };
+template <> struct FewStage<BRASA_KV_F16> { static constexpr uint32_t K_PITCH = 256, V_PITCH = 256, STAGES = 3, BLOCKS = 2; };
 // (pitches at which neither the 8-byte reads of K nor the transposed reads of V meet in a bank)
-template <> struct FewStage<BRASA_KV_Q8_0> { static constexpr uint32_t K_PITCH = 160, V_PITCH = 144, STAGES = 4; };
+template <> struct FewStage<BRASA_KV_Q8_0> { static constexpr uint32_t K_PITCH = 160, V_PITCH = 144, STAGES = 4, BLOCKS = 2; };
 template <int KV> constexpr uint32_t few_stage_bytes() { return FEW_KEYS * (FewStage<KV>::K_PITCH + FewStage<KV>::V_PITCH); }
 constexpr uint32_t FEW_TS = D + 4;
 
@@ -142,7 +142,7 @@ __device__ __forceinline__ void terms_h2(float x, float y, uint32_t &hi, uint32_
     }
 }
 template <int KV, bool HALF>
-__global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_constant__ FewParams p) {
+__global__ void __launch_bounds__(128, FewStage<KV>::BLOCKS) attn_packed_few_kernel(const __grid_constant__ FewParams p) {
     // Launched as a programmatic dependent. late_wait: the kernel before this one is the same call's tensor-core form, which has itself waited for what both read
     // and whose output this one does not touch: the two run side by side, and this one waits for the other at its end, so that whoever waits for it has
     // waited for both.
@@ -173,9 +173,12 @@ __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_const
         const uint32_t token0 = it.part * p.l.item_tokens, t0 = it.t0 + token0, rows = line_tokens(p.l, it) * G, nkeys = line_keys(p.l, it);
         const uint32_t share = rows <= 16 ? 4 : (rows <= 32 ? 2 : 1), kp = warp % share, rt = warp / share;
         const bool active = rt * 16 < rows;
-        // ---- copies of 64 keys: pages one chunk ahead, what the item's last row does not see as zeros ----
+        // ---- copies of 64 keys, a page to a warp and two rows at a time: pages looked up one chunk ahead, what the item's last row does not see as zeros ----
         const int32_t *table = p.l.v.table + (size_t)it.seq * p.l.v.max_pages;
         const size_t page_bytes = (size_t)PAGE * hkv * ROW;
+        const uint32_t r2 = lane >> 4, pc = lane & 15, step = 2 * hkv * ROW;
+        const uint32_t own = (r2 * hkv + it.kh) * ROW + (Q8 ? 8 : 16) * pc;                                    // this lane's piece of the page's first rows
+        const uint32_t tail = ((tid & 15) * hkv + it.kh) * ROW + 128, tail_at = (tid & 63) * (tid < 64 ? S::K_PITCH : S::V_PITCH) + 128 + (tid < 64 ? 0 : V_AT);  // (8 bit: scales)
         int32_t pg[4];
         uint32_t there = 0;  // which pages of the last chunks are, four bits each, the newest lowest
         auto look = [&](uint32_t j) {
@@ -191,28 +194,29 @@ __global__ void __launch_bounds__(128) attn_packed_few_kernel(const __grid_const
                 const uint32_t stage = ring + (j % S::STAGES) * STAGE;
 #pragma unroll
                 for (uint32_t x = 0; x < 4; ++x) bits |= (pg[x] >= 0 ? 1u : 0u) << x;
-                if (!Q8) {
-                    const uint32_t r = tid >> 4, c = tid & 15;
+                const int32_t page = warp & 2 ? (warp & 1 ? pg[3] : pg[2]) : (warp & 1 ? pg[1] : pg[0]);
+                const uint32_t first = 64 * j + 16 * warp, left = page >= 0 && first < nkeys ? nkeys - first : 0u;  // rows of the page that are seen (16 or more: all)
+                const size_t at = (size_t)max(page, 0) * page_bytes + own;
+                const uint8_t *ks = p.kpool + at, *vs = p.vpool + at;
 #pragma unroll
-                    for (uint32_t k = 0; k < 8; ++k) {
-                        const uint32_t row = 8 * k + r;
-                        const bool ok = pg[k >> 1] >= 0 && 64 * j + row < nkeys;
-                        const size_t at = (ok ? (size_t)pg[k >> 1] : 0) * page_bytes + ((row & 15) * hkv + it.kh) * ROW + 16 * c;
-                        const uint32_t to = stage + row * 256 + ((c ^ (row & 7)) << 4);
-                        cp_zfill16(to, p.kpool + at, ok);
-                        cp_zfill16(to + V_AT, p.vpool + at, ok);
+                for (uint32_t u = 0; u < 8; ++u) {
+                    const uint32_t row = 16 * warp + 2 * u + r2;
+                    const bool ok = 2 * u + r2 < left;
+                    if (Q8) {
+                        cp_zfill8(stage + row * S::K_PITCH + 8 * pc, ks, ok);
+                        cp_zfill8(stage + V_AT + row * S::V_PITCH + 8 * pc, vs, ok);
+                    } else {
+                        const uint32_t to = stage + row * 256 + ((pc ^ (row & 7)) << 4);
+                        cp_zfill16(to, ks, ok);
+                        cp_zfill16(to + V_AT, vs, ok);
                     }
-                } else {
-#pragma unroll
-                    for (uint32_t k = 0; k < 9; ++k) {
-                        const uint32_t i = tid + 128 * k, row = i / 17, c = i % 17;
-                        if (i >= FEW_KEYS * 17) break;
-                        const int32_t page = row < 32 ? (row < 16 ? pg[0] : pg[1]) : (row < 48 ? pg[2] : pg[3]);
-                        const bool ok = page >= 0 && 64 * j + row < nkeys;
-                        const size_t at = (ok ? (size_t)page : 0) * page_bytes + ((row & 15) * hkv + it.kh) * ROW + 8 * c;
-                        cp_zfill8(stage + row * S::K_PITCH + 8 * c, p.kpool + at, ok);
-                        cp_zfill8(stage + V_AT + row * S::V_PITCH + 8 * c, p.vpool + at, ok);
-                    }
+                    ks += ok ? step : 0;  // (a pointer stays inside the page)
+                    vs += ok ? step : 0;
+                }
+                if (Q8) {
+                    const uint32_t x = (tid & 63) >> 4;
+                    const int32_t mine = x & 2 ? (x & 1 ? pg[3] : pg[2]) : (x & 1 ? pg[1] : pg[0]);
+                    cp_zfill8(stage + tail_at, (tid < 64 ? p.kpool : p.vpool) + (size_t)max(mine, 0) * page_bytes + tail, mine >= 0 && 64 * j + (tid & 63) < nkeys);
                 }
                 look(j + 1);
             }
@@ -715,12 +719,12 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
     const uint32_t G = hq / hkv, sms = ctx->sm_count;
     const bool f32 = pg.kv == BRASA_KV_F32 || (pg.kv == BRASA_KV_Q8_0 && !half);
     const bool tc = half && !f32 && (uint64_t)run.longest * G >= PACKED_TC_MIN_ROWS && (uint64_t)pg.num_pages * PAGE < 1ull << 31;
-    const uint32_t blocks = f32 ? sms : 2 * sms;
+    const uint32_t blocks = sms * (f32 ? 1 : (pg.kv == BRASA_KV_Q8_0 ? FewStage<BRASA_KV_Q8_0>::BLOCKS : FewStage<BRASA_KV_F16>::BLOCKS));
     // the workspace: parts of either kernel's items, then what they belong to
-    const size_t few_floats = 2 * (size_t)(2 * sms) * packed_part_floats(FEW_ROWS), tc_floats = 2 * (size_t)sms * packed_part_floats(PACKED_TC_ROWS);
-    BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, (few_floats + tc_floats) * sizeof(float) + 3 * sms * sizeof(PackedNote)));
+    const size_t few_floats = 2 * (size_t)(4 * sms) * packed_part_floats(FEW_ROWS), tc_floats = 2 * (size_t)sms * packed_part_floats(PACKED_TC_ROWS);
+    BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, (few_floats + tc_floats) * sizeof(float) + 5 * sms * sizeof(PackedNote)));
     float *few_part = (float *)ctx->packed_work, *tc_part = few_part + few_floats;
-    PackedNote *few_notes = (PackedNote *)(tc_part + tc_floats), *tc_notes = few_notes + 2 * sms;
+    PackedNote *few_notes = (PackedNote *)(tc_part + tc_floats), *tc_notes = few_notes + 4 * sms;
     if (tc) BRASA_TRY(brasa_packed_tc_launch(cmd, p, pg.kv, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), tc_part, tc_notes, hq, scale));
     const FewParams f{packed_line(p, G, FEW_ROWS, 6, 1, 1, 3, 1, tc ? PACKED_TC_MIN_ROWS - 1 : UINT32_MAX), (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), few_part,
                       few_notes, hq, scale, tc ? 1u : 0u};
