@@ -187,23 +187,28 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                 // Rows are turned into f16(d * code) on the way: this warp has pages 4 w .. 4 w + 3 of a tile, two rows at a time, eight codes a lane; a tile's codes are
                 // fetched while the tile before is turned.
                 const uint32_t w = (warp - K_WARP) >> 1, c = lane & 15, r2 = lane >> 4;
-                const uint8_t *pool = is_v ? p.vpool : p.kpool;
+                const size_t page_bytes = (size_t)PAGE * hkv * 136;
+                const uint32_t step = 2 * hkv * 136;  // two rows on
+                const uint8_t *codes0 = (is_v ? p.vpool : p.kpool) + (r2 * hkv + kh) * 136 + 8 * c;
+                const uint8_t *scales0 = (is_v ? p.vpool : p.kpool) + ((lane >> 1) * hkv + kh) * 136 + 128 + 4 * (lane & 1);  // two scales of a row a lane, for a page
                 uint2 code[32];
-                __half scale[32];
-                uint32_t there = 0;
+                uint32_t scale[4];
+                uint32_t there = 0, to[4];
+#pragma unroll
+                for (uint32_t u = 0; u < 4; ++u) to[u] = tile_piece(64 * w + 2 * u + r2, 8 * c);
                 auto fetch = [&](uint32_t j) {  // of tile j0 + j
                     const int32_t mine = j < len ? page_at(8 * (j0 + j) + (lane & 7)) : -1;
                     there = __ballot_sync(0xffffffffu, (uint32_t)mine < p.l.v.num_pages) & 255u;
 #pragma unroll
-                    for (uint32_t e = 0; e < 32; ++e) {
-                        const uint32_t i = 4 * w + (e >> 3), r = 2 * (e & 7) + r2;
-                        const int32_t page = __shfl_sync(0xffffffffu, mine, i);
-                        code[e] = make_uint2(0, 0);
-                        scale[e] = __ushort_as_half(0);
-                        if ((there >> i & 1) && 128 * (j0 + j) + 16 * i + r < nkeys) {
-                            const uint8_t *row = pool + (((size_t)page * PAGE + r) * hkv + kh) * 136;
-                            code[e] = reinterpret_cast<const uint2 *>(row)[c];
-                            scale[e] = reinterpret_cast<const __half *>(row + 128)[c >> 2];
+                    for (uint32_t g = 0; g < 4; ++g) {
+                        const uint32_t i = 4 * w + g, first = 128 * (j0 + j) + 16 * i;
+                        const size_t at = (size_t)(uint32_t)__shfl_sync(0xffffffffu, mine, i) * page_bytes;
+                        const uint32_t seen = there >> i & 1 ? min(16u, nkeys - first) : 0;  // rows of the page (a page that is one has some that are seen)
+                        scale[g] = lane >> 1 < seen ? *reinterpret_cast<const uint32_t *>(scales0 + at) : 0u;
+#pragma unroll
+                        for (uint32_t u = 0; u < 8; ++u) {
+                            code[8 * g + u] = make_uint2(0, 0);
+                            if (2 * u + r2 < seen) code[8 * g + u] = *reinterpret_cast<const uint2 *>(codes0 + at + u * step);
                         }
                     }
                 };
@@ -215,9 +220,10 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                     if (walks && lane == 0) there_s[loads & 7] = there;  // (read by whoever sees this tile's scores, four tiles behind at most)
 #pragma unroll
                     for (uint32_t e = 0; e < 32; ++e) {
-                        const __half2 d = __half2half2(scale[e]);
+                        const uint32_t dd = __byte_perm(__shfl_sync(0xffffffffu, scale[e >> 3], 2 * (2 * (e & 7) + r2) + (c >> 3)), 0, c & 4 ? 0x3232 : 0x1010);
+                        const __half2 d = *reinterpret_cast<const __half2 *>(&dd);
                         const uint32_t lo = code[e].x ^ 0x80808080u, hi = code[e].y ^ 0x80808080u;
-                        *reinterpret_cast<uint4 *>(slot + tile_piece(64 * w + 16 * (e >> 3) + 2 * (e & 7) + r2, 8 * c)) =
+                        *reinterpret_cast<uint4 *>(slot + to[e & 3] + 1024 * (e >> 2)) =
                             make_uint4(bytes_h2(lo, 0x4140, d), bytes_h2(lo, 0x4342, d), bytes_h2(hi, 0x4140, d), bytes_h2(hi, 0x4342, d));
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
