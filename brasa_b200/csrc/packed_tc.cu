@@ -22,7 +22,7 @@ namespace {
 
 constexpr uint32_t PAGE = BRASA_KV_PAGE, D = 128, WAIT_LIMIT = 1u << 20, TILE_BYTES = 128 * 128 * 2, ROWS = PACKED_TC_ROWS;
 constexpr uint32_t SOFTMAX_WARPS = 8, MMA_WARP = 8, K_WARP = 10, V_WARP = 11;  // (one MMA warp for each row tile)
-constexpr uint32_t THREADS = 384, THREADS_Q8 = 448;  // an 8-bit pool's K and V have two warps each
+constexpr uint32_t THREADS = 384, WARPS_Q8 = 3, THREADS_Q8 = 512;  // an 8-bit pool's K and V have three warps each
 
 struct PackedMaps {
     CUtensorMap k, v;
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
 
     if (tid == 0) {
         for (uint32_t i = 0; i < 4; ++i) {  // [K or V][slot]
-            mbar_init(&full[i >> 1][i & 1], Q8 ? 2 : 1);
+            mbar_init(&full[i >> 1][i & 1], Q8 ? WARPS_Q8 : 1);
             mbar_init(&freed[i >> 1][i & 1], 2);  // by either row tile's products
         }
         for (int i = 0; i < 2; ++i) {
@@ -184,26 +184,26 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                 for (uint32_t t = lane; t * G < share.rows; t += 32)
                     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.q + ((size_t)(share.t0 + t) * p.hq + kh * G) * D), "r"(G * D * 4) : "memory");
             if constexpr (Q8) {
-                // Rows are turned into f16(d * code) on the way: this warp has pages 4 w .. 4 w + 3 of a tile, two rows at a time, eight codes a lane; a tile's codes are
+                // Rows are turned into f16(d * code) on the way: this warp has pages w, w + 3 and w + 6 of a tile, two rows at a time, eight codes a lane; a tile's codes are
                 // fetched while the tile before is turned.
                 const uint32_t w = (warp - K_WARP) >> 1, c = lane & 15, r2 = lane >> 4;
                 const size_t page_bytes = (size_t)PAGE * hkv * 136;
                 const uint32_t step = 2 * hkv * 136;  // two rows on
                 const uint8_t *codes0 = (is_v ? p.vpool : p.kpool) + (r2 * hkv + kh) * 136 + 8 * c;
                 const uint8_t *scales0 = (is_v ? p.vpool : p.kpool) + ((lane >> 1) * hkv + kh) * 136 + 128 + 4 * (lane & 1);  // two scales of a row a lane, for a page
-                uint2 code[32];
-                uint32_t scale[4];
-                uint32_t there = 0, to[4];
+                uint2 code[24];
+                uint32_t scale[3];
+                uint32_t there = 0, to[4];  // (rows four pairs apart are swizzled alike)
 #pragma unroll
-                for (uint32_t u = 0; u < 4; ++u) to[u] = tile_piece(64 * w + 2 * u + r2, 8 * c);
+                for (uint32_t u = 0; u < 4; ++u) to[u] = tile_piece(16 * w + 2 * u + r2, 8 * c);
                 auto fetch = [&](uint32_t j) {  // of tile j0 + j
                     const int32_t mine = j < len ? page_at(8 * (j0 + j) + (lane & 7)) : -1;
                     there = __ballot_sync(0xffffffffu, (uint32_t)mine < p.l.v.num_pages) & 255u;
 #pragma unroll
-                    for (uint32_t g = 0; g < 4; ++g) {
-                        const uint32_t i = 4 * w + g, first = 128 * (j0 + j) + 16 * i;
-                        const size_t at = (size_t)(uint32_t)__shfl_sync(0xffffffffu, mine, i) * page_bytes;
-                        const uint32_t seen = there >> i & 1 ? min(16u, nkeys - first) : 0;  // rows of the page (a page that is one has some that are seen)
+                    for (uint32_t g = 0; g < 3; ++g) {
+                        const uint32_t i = w + WARPS_Q8 * g, first = 128 * (j0 + j) + 16 * i;
+                        const size_t at = (size_t)(uint32_t)__shfl_sync(0xffffffffu, mine, i & 7) * page_bytes;
+                        const uint32_t seen = i < 8 && there >> i & 1 ? min(16u, nkeys - first) : 0;  // rows of the page (a page that is one has some that are seen)
                         scale[g] = lane >> 1 < seen ? *reinterpret_cast<const uint32_t *>(scales0 + at) : 0u;
 #pragma unroll
                         for (uint32_t u = 0; u < 8; ++u) {
@@ -219,11 +219,12 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                     uint8_t *slot = ring + (size_t)(2 * is_v + s) * TILE_BYTES;
                     if (walks && lane == 0) there_s[loads & 7] = there;  // (read by whoever sees this tile's scores, four tiles behind at most)
 #pragma unroll
-                    for (uint32_t e = 0; e < 32; ++e) {
+                    for (uint32_t e = 0; e < 24; ++e) {
+                        if (e >= 16 && w == 2) break;  // (a tile has eight pages)
                         const uint32_t dd = __byte_perm(__shfl_sync(0xffffffffu, scale[e >> 3], 2 * (2 * (e & 7) + r2) + (c >> 3)), 0, c & 4 ? 0x3232 : 0x1010);
                         const __half2 d = *reinterpret_cast<const __half2 *>(&dd);
                         const uint32_t lo = code[e].x ^ 0x80808080u, hi = code[e].y ^ 0x80808080u;
-                        *reinterpret_cast<uint4 *>(slot + to[e & 3] + 1024 * (e >> 2)) =
+                        *reinterpret_cast<uint4 *>(slot + to[e & 3] + 1024 * (e >> 2 & 1) + 2048 * WARPS_Q8 * (e >> 3)) =
                             make_uint4(bytes_h2(lo, 0x4140, d), bytes_h2(lo, 0x4342, d), bytes_h2(hi, 0x4140, d), bytes_h2(hi, 0x4342, d));
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
