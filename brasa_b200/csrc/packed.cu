@@ -122,14 +122,32 @@ __device__ __forceinline__ void mma_f16(float c[4], const uint32_t a[4], uint32_
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ uint32_t pack_h2(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t *>(&h);
+}
+// A block's rows that are to be taken again (bits of `rows`): the warps share them, and write over what the block wrote before the barrier ahead of this.
+template <int KV, bool HALF, uint32_t THREADS>
+__device__ __noinline__ void few_again(const FewParams &p, const PackedItem &it, uint64_t rows, uint32_t from, uint32_t to, bool whole, float *part) {
+    const uint32_t lane = threadIdx.x & 31, G = p.l.group, token0 = it.part * p.l.item_tokens;
+    for (uint32_t n = 0; rows; rows &= rows - 1, ++n) {
+        if (n % (THREADS / 32) != threadIdx.x >> 5) continue;
+        const uint32_t r = __ffsll(rows) - 1, token = row_token(p.l, r);
+        const size_t at = ((size_t)(it.t0 + token0 + token) * p.hq + it.kh * G + r - token * G) * D + 4 * lane;
+        const PackedRowSums x = packed_row_again<KV>(p.l.v, p.kpool, p.vpool, p.q + at - 4 * lane, p.scale, it.seq, it.kh, from, min(to, it.past + token0 + token + 1));
+        if (whole) {
+            const float inv = x.l == 0.0f ? 0.0f : 1.0f / x.l;
+            const float4 v = make_float4(x.o.x * inv, x.o.y * inv, x.o.z * inv, x.o.w * inv);
+            if (HALF) *reinterpret_cast<uint2 *>(static_cast<__half *>(p.o) + at) = make_uint2(pack_h2(v.x, v.y), pack_h2(v.z, v.w));
+            else *reinterpret_cast<float4 *>(static_cast<float *>(p.o) + at) = v;
+        } else {
+            reinterpret_cast<float4 *>(part + r * D)[lane] = x.o;
+            if (lane == 0) {
+                part[FEW_ROWS * D + r] = x.m;
+                part[FEW_ROWS * D + FEW_ROWS + r] = x.l;
+            }
+        }
+    }
 }
 // x, y -> f16 pair and, with two terms, the pair of what its rounding dropped
 template <bool HALF>
@@ -156,6 +174,7 @@ __global__ void __launch_bounds__(128, FewStage<KV>::BLOCKS) attn_packed_few_ker
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PackedPieces pieces;
     __shared__ float sums[4][2][16];
+    __shared__ uint32_t again[2];  // rows whose output is not finite
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem), hkv = p.l.v.hkv, G = p.l.group;
     PackedNote note{};
@@ -388,8 +407,10 @@ __global__ void __launch_bounds__(128, FewStage<KV>::BLOCKS) attn_packed_few_ker
                 }
             }
         }
+        if (tid < 2) again[tid] = 0;
         __syncthreads();
         const bool whole = j0 == 0 && j1 == it.tiles;
+        const uint32_t upto = min(nkeys, 64 * j1);
         float *part = p.part + (size_t)(2 * blockIdx.x + (j0 == 0)) * packed_part_floats(FEW_ROWS);
         for (uint32_t r = 0; r < rows; ++r) {
             const uint32_t w0 = r / 16 * share, x = r % 16;
@@ -400,6 +421,7 @@ __global__ void __launch_bounds__(128, FewStage<KV>::BLOCKS) attn_packed_few_ker
                 L = fmaf(sums[w][1][x], f, L);
                 acc = fmaf(reinterpret_cast<float *>(smem)[(w * 16 + x) * FEW_TS + tid], f, acc);
             }
+            if (not_finite(acc) && it.past + token0 + row_token(p.l, r) + 1 < upto) atomicOr(&again[r >> 5], 1u << (r & 31));
             if (whole) {
                 const uint32_t token = row_token(p.l, r);
                 const size_t at = ((size_t)(t0 + token) * p.hq + it.kh * G + r - token * G) * D + tid;
@@ -417,6 +439,7 @@ __global__ void __launch_bounds__(128, FewStage<KV>::BLOCKS) attn_packed_few_ker
         if (!whole && j0 == 0) note = PackedNote{1, note.closes, t0, rows, it.kh};
         if (j0 > 0 && j1 == it.tiles) note.closes = 1;
         __syncthreads();  // the ring and the sums are free again
+        if (again[0] | again[1]) few_again<KV, HALF, 128>(p, it, again[0] | (uint64_t)again[1] << 32, 64 * j0, upto, whole, part);
         if (j1 < it.tiles || !line_next(p.l, it)) break;
     }
     if (tid == 0) p.notes[blockIdx.x] = note;
@@ -431,11 +454,12 @@ constexpr uint32_t F32_THREADS = 256, F32_P = 68;
 constexpr size_t F32_SMEM = (3 * 64 * (size_t)FEW_TS + 64 * F32_P) * sizeof(float);
 
 template <int KV, bool HALF>
-__global__ void __launch_bounds__(F32_THREADS) attn_packed_f32_kernel(const __grid_constant__ FewParams p) {
+__global__ void __launch_bounds__(F32_THREADS, 1) attn_packed_f32_kernel(const __grid_constant__ FewParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(16) float fs[];
     __shared__ PackedPieces pieces;
+    __shared__ uint32_t again[2];  // rows whose output is not finite
     float *qs = fs, *ks = qs + 64 * FEW_TS, *vs = ks + 64 * FEW_TS, *ps = vs + 64 * FEW_TS;
     const uint32_t tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, hkv = p.l.v.hkv, G = p.l.group;
     PackedNote note{};
@@ -572,7 +596,10 @@ __global__ void __launch_bounds__(F32_THREADS) attn_packed_f32_kernel(const __gr
             __syncthreads();  // V and the weights are done with
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (tid < 2) again[tid] = 0;
+        __syncthreads();
         const bool whole = j0 == 0 && j1 == it.tiles;
+        const uint32_t upto = min(nkeys, 64 * j1);
         float *part = p.part + (size_t)(2 * blockIdx.x + (j0 == 0)) * packed_part_floats(FEW_ROWS);
         if (live) {
 #pragma unroll
@@ -580,6 +607,10 @@ __global__ void __launch_bounds__(F32_THREADS) attn_packed_f32_kernel(const __gr
                 const uint32_t r = 4 * ty + a;
                 for (int x = 8; x > 0; x >>= 1) l[a] += __shfl_xor_sync(0xffffu << (tid & 16), l[a], x);
                 if (r >= rows) continue;
+                bool bad = false;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) bad = bad || not_finite(o[a][e]);
+                if (bad && seen[a] < upto) atomicOr(&again[r >> 5], 1u << (r & 31));
                 if (whole) {
                     const uint32_t token = row_token(p.l, r);
                     const size_t at = ((size_t)(t0 + token) * p.hq + it.kh * G + r - token * G) * D + 4 * tx;
@@ -604,6 +635,7 @@ __global__ void __launch_bounds__(F32_THREADS) attn_packed_f32_kernel(const __gr
         if (!whole && j0 == 0) note = PackedNote{1, note.closes, t0, rows, it.kh};
         if (j0 > 0 && j1 == it.tiles) note.closes = 1;
         __syncthreads();  // (q's place is free)
+        if (again[0] | again[1]) few_again<KV, HALF, F32_THREADS>(p, it, again[0] | (uint64_t)again[1] << 32, 64 * j0, upto, whole, part);
         if (j1 < it.tiles || !line_next(p.l, it)) break;
     }
     if (tid == 0) p.notes[blockIdx.x] = note;
@@ -721,10 +753,10 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
     const bool tc = half && !f32 && (uint64_t)run.longest * G >= PACKED_TC_MIN_ROWS && (uint64_t)pg.num_pages * PAGE < 1ull << 31;
     const uint32_t blocks = sms * (f32 ? 1 : (pg.kv == BRASA_KV_Q8_0 ? FewStage<BRASA_KV_Q8_0>::BLOCKS : FewStage<BRASA_KV_F16>::BLOCKS));
     // the workspace: parts of either kernel's items, then what they belong to
-    const size_t few_floats = 2 * (size_t)(4 * sms) * packed_part_floats(FEW_ROWS), tc_floats = 2 * (size_t)sms * packed_part_floats(PACKED_TC_ROWS);
-    BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, (few_floats + tc_floats) * sizeof(float) + 5 * sms * sizeof(PackedNote)));
+    const size_t few_floats = 2 * (size_t)(2 * sms) * packed_part_floats(FEW_ROWS), tc_floats = 2 * (size_t)sms * packed_part_floats(PACKED_TC_ROWS);
+    BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, (few_floats + tc_floats) * sizeof(float) + 3 * sms * sizeof(PackedNote)));
     float *few_part = (float *)ctx->packed_work, *tc_part = few_part + few_floats;
-    PackedNote *few_notes = (PackedNote *)(tc_part + tc_floats), *tc_notes = few_notes + 4 * sms;
+    PackedNote *few_notes = (PackedNote *)(tc_part + tc_floats), *tc_notes = few_notes + 2 * sms;
     if (tc) BRASA_TRY(brasa_packed_tc_launch(cmd, p, pg.kv, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), tc_part, tc_notes, hq, scale));
     const FewParams f{packed_line(p, G, FEW_ROWS, 6, 1, 1, 3, 1, tc ? PACKED_TC_MIN_ROWS - 1 : UINT32_MAX), (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), few_part,
                       few_notes, hq, scale, tc ? 1u : 0u};

@@ -52,6 +52,67 @@ __device__ __forceinline__ uint32_t bytes_h2(uint32_t w, uint32_t sel, __half2 s
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
+
+// The sums of one row over the keys [from, to) of its sequence, a warp, four dims a lane: m, the sum of 2^(s - m) and that times V. This is for what the matrix
+// products cannot do: a weight of zero times an infinity or NaN of V is NaN, so that a key behind a row's own position, new in the same run, would
+// reach it. A kernel whose output is not finite although keys of the tile lie behind the row (`to` of it and more) takes the row again this way, without them.
+struct PackedRowSums {
+    float m, l;
+    float4 o;
+};
+template <int KV>
+__device__ __forceinline__ float4 packed_row4(const uint8_t *row, uint32_t lane) {
+    const float2 a = tile_at2<KV>(row, 4 * lane), b = tile_at2<KV>(row, 4 * lane + 2);
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+template <int KV>
+__device__ __noinline__ PackedRowSums packed_row_again(const PackedView &v, const uint8_t *kpool, const uint8_t *vpool, const float *q, float scale, uint32_t seq, uint32_t kh, uint32_t from, uint32_t to) {
+    constexpr uint32_t AT_ONCE = 4;
+    const uint32_t lane = threadIdx.x & 31;
+    const float4 x = reinterpret_cast<const float4 *>(q)[lane];
+    const float c = scale * 1.4426950408889634f;
+    PackedRowSums r{-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    for (uint32_t k0 = from; k0 < to; k0 += AT_ONCE) {
+        const int32_t page = packed_page(v, seq, k0);
+        if (page < 0) continue;
+        float s[AT_ONCE];
+        float4 y[AT_ONCE];
+#pragma unroll
+        for (uint32_t e = 0; e < AT_ONCE; ++e) {
+            const size_t at = (((size_t)page * BRASA_KV_PAGE + (k0 + e) % BRASA_KV_PAGE) * v.hkv + kh) * KvRow<KV>::BYTES;
+            y[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            s[e] = -INFINITY;
+            if (k0 + e < to) {
+                const float4 k = packed_row4<KV>(kpool + at, lane);
+                y[e] = packed_row4<KV>(vpool + at, lane);
+                s[e] = fmaf(x.w, k.w, fmaf(x.z, k.z, fmaf(x.y, k.y, x.x * k.x)));
+                for (int i = 16; i > 0; i >>= 1) s[e] += __shfl_xor_sync(0xffffffffu, s[e], i);
+                s[e] *= c;
+            }
+        }
+        float now = r.m;
+#pragma unroll
+        for (uint32_t e = 0; e < AT_ONCE; ++e) now = fmaxf(now, s[e]);
+        const float ref = now == -INFINITY ? 0.0f : now, f = r.m == -INFINITY ? 0.0f : exp2_approx(r.m - ref);
+        r.m = now;
+        r.l *= f;
+        r.o = make_float4(r.o.x * f, r.o.y * f, r.o.z * f, r.o.w * f);
+#pragma unroll
+        for (uint32_t e = 0; e < AT_ONCE; ++e) {
+            const float w = exp2_approx(s[e] - ref);
+            r.l += w;
+            r.o = make_float4(fmaf(w, y[e].x, r.o.x), fmaf(w, y[e].y, r.o.y), fmaf(w, y[e].z, r.o.z), fmaf(w, y[e].w, r.o.w));
+        }
+    }
+    return r;
+}
+
 // ---- the work of a run in a line, cut evenly ----
 // An item is up to item_tokens tokens of one sequence, each with the heads of a key head's group, against that key head. In the line an item takes `start`
 // units for its beginning and end and one per 2^tile_log2 keys that its last token sees. Equal pieces of the line go to the blocks; a block works

@@ -74,11 +74,6 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t v[8]) {
                  : "r"(taddr)
                  : "memory");
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -432,7 +427,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                     bool move = false;
                     if (tmax > m + SLACK || (m == -INFINITY && tmax != -INFINITY)) {
                         move = m != -INFINITY;
-                        rescale = move ? ex2((m - tmax) * LOG2E) : 1.0f;
+                        rescale = move ? exp2_approx((m - tmax) * LOG2E) : 1.0f;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) l[e] *= rescale;
                         m = tmax;
@@ -461,7 +456,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                         if (c == 3 && rows > 128 && lane == 0) tc_mbar_arrive(&turn[x ^ 1]);
                         float y[16];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) y[e] = ex2(fmaf(__uint_as_float(v[c >> 1][(c & 1) * 16 + e]), LOG2E, mneg));
+                        for (int e = 0; e < 16; ++e) y[e] = exp2_approx(fmaf(__uint_as_float(v[c >> 1][(c & 1) * 16 + e]), LOG2E, mneg));
                         uint32_t w[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
@@ -488,8 +483,9 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                 const float sum = (l[0] + l[1]) + (l[2] + l[3]);
                 const uint32_t r = 128 * x + row;
                 const bool live = r < rows;
+                bool bad = false;  // an output that is not finite
+                float *const dst = p.part + (size_t)(2 * blockIdx.x + (j0 == 0)) * packed_part_floats(ROWS);
                 if (!share.whole) {
-                    float *dst = p.part + (size_t)(2 * blockIdx.x + (j0 == 0)) * packed_part_floats(ROWS);
                     if (live) {
                         dst[ROWS * D + r] = m * LOG2E;
                         dst[ROWS * D + ROWS + r] = sum;
@@ -499,6 +495,8 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                         uint32_t o[32];
                         tmem_ld32(to + 32 * c, o);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) bad = bad || not_finite(__uint_as_float(o[e]));
 #pragma unroll
                         for (int g = 0; g < 8; ++g)
                             if (live) reinterpret_cast<uint4 *>(dst + (size_t)r * D)[8 * c + g] = make_uint4(o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]);
@@ -511,6 +509,8 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                         uint32_t o[32], packed[16];
                         tmem_ld32(to + 32 * c, o);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) bad = bad || not_finite(__uint_as_float(o[e]));
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
                             const __half2 hh = __floats2half2_rn(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
@@ -527,6 +527,25 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                             if (re < rows) reinterpret_cast<uint4 *>(p.o + ((size_t)(share.t0 + tk) * p.hq + share.kh * G + re - tk * G) * D + 32 * c)[lane & 3] = w;
                         }
                         __syncwarp();
+                    }
+                }
+                const uint32_t upto = min(share.nkeys, 128 * (j0 + share.len));
+                uint32_t again = __ballot_sync(0xffffffffu, live && bad && seen_all < upto);
+#pragma unroll 1
+                for (__syncwarp(); again; again &= again - 1) {  // (see packed_row_again)
+                    const uint32_t re = 128 * x + wrow + __ffs(again) - 1, tk = row_token(p.l, re);
+                    const size_t at = ((size_t)(share.t0 + tk) * p.hq + share.kh * G + re - tk * G) * D;
+                    const PackedRowSums y = packed_row_again<Q8 ? BRASA_KV_Q8_0 : BRASA_KV_F16>(p.l.v, p.kpool, p.vpool, p.q + at, p.scale, share.seq, share.kh, 128 * j0, min(upto, share.past + tk + 1));
+                    if (share.whole) {
+                        const float f = y.l == 0.0f ? 0.0f : 1.0f / y.l;
+                        const __half2 a = __floats2half2_rn(y.o.x * f, y.o.y * f), b = __floats2half2_rn(y.o.z * f, y.o.w * f);
+                        reinterpret_cast<uint2 *>(p.o + at)[lane] = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+                    } else {
+                        reinterpret_cast<float4 *>(dst + (size_t)re * D)[lane] = y.o;
+                        if (lane == 0) {
+                            dst[ROWS * D + re] = y.m;
+                            dst[ROWS * D + ROWS + re] = y.l;
+                        }
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -124,6 +124,32 @@ def test_attention_positions_without_pages(ctx, K, kv, half):
     assert (got[a:b] == 0).all() and (got[b:b + 128] == 0).all()
 
 
+@pytest.mark.parametrize("bad", ["nan", "inf in v", "inf in k"])
+@pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("q8_0", False), ("f32", False), ("f32", True)])
+def test_attention_rows_before_a_bad_one(ctx, K, kv, half, bad):
+    """A token whose key or value is not finite counts for its own row and those behind it, never for a row before it: one piece of the work or several,
+    few rows and many."""
+    run = R.Run([(5, 130), (3, 0), (4, 3000), (200, 33), (129, 250), (150, 2200)], 4, 2, kv, seed=21)
+    want, tol = run.attention(half)
+    first = [3, 1, 2, 150, 128, 60]  # of each sequence's new tokens, the bad one
+    for s, j in enumerate(first):
+        at = int(run.lens[s]) + j
+        row = np.full((run.hkv, R.D), np.nan if bad == "nan" else np.inf, np.float32)
+        if kv == "q8_0":  # (codes of 1 under a scale that is not finite)
+            raw = np.concatenate([np.ones((run.hkv, 128), np.uint8), row[:, :4].astype(np.float16).view(np.uint8)], -1)
+        else:
+            raw = R.to_bytes(row, kv)
+        for pool in (run.k, run.v):
+            if bad == "nan" or (bad == "inf in v") == (pool is run.v):
+                pool[run.table[s, at // R.PAGE], at % R.PAGE] = raw
+    got, _ = attend(ctx, K, run, half)
+    for s, j in enumerate(first):
+        a, b, e = int(run.starts[s]), int(run.starts[s]) + j, int(run.starts[s + 1])
+        check(got[a:b], want[a:b], tol[a:b])
+        if bad != "inf in k":
+            assert not np.isfinite(got[b:e]).any()
+
+
 def test_attention_keeps_to_what_the_call_says(ctx, K):
     """`longest` and `tokens` below what starts say, starts that fall, positions behind the table: such rows are left alone."""
     run = R.Run([(3, 40), (150, 20), (2, 30)], 4, 2, "f16", seed=5)
