@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
     __shared__ PackedShare shares[SHARES];
     __shared__ uint32_t tmem_base_s, abort_s, there_s[8];  // (there: of the last key tiles, which of their eight pages are pages)
     __shared__ PackedPieces pieces;
+    __shared__ PackedNote note;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.l.group, hkv = p.l.v.hkv;
 
     if (tid == 0) {
@@ -147,12 +148,14 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
     if (warp >= K_WARP) {  // ---- copies, as far ahead of the products as there are slots; K's warp walks the line and hands the shares on ----
         const uint32_t is_v = (warp - K_WARP) & 1;
         const bool walks = warp == K_WARP;
-        PackedItem item = pieces.at[0];
-        const uint64_t end_first = pieces.at[1].first;
-        const uint32_t end_j = pieces.at[1].j;
-        if (work && item.j == item.tiles) line_next(p.l, item);
-        bool more = work && (item.first < end_first || (item.first == end_first && item.j < end_j)), ok = true;
-        PackedNote note{};
+        PackedItem &item = pieces.at[0];  // (where the walk is: one lane's, in shared memory, since the converting warps have no registers to spare)
+        const PackedItem &end = pieces.at[1];
+        bool more = false, ok = true;
+        if (walks && lane == 0) {
+            if (work && item.j == item.tiles) line_next(p.l, item);
+            more = work && (item.first < end.first || (item.first == end.first && item.j < end.j));
+            note = PackedNote{};
+        }
         uint32_t loads = 0;  // tiles copied so far
 #pragma unroll 1
         for (uint32_t n = 0; ok; ++n) {
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                 if (lane == 0) {
                     share.rows = 0;
                     if (more) {
-                        const uint32_t j1 = item.first == end_first ? end_j : item.tiles, token0 = item.part * p.l.item_tokens, rows = line_tokens(p.l, item) * G;
+                        const uint32_t j1 = item.first == end.first ? end.j : item.tiles, token0 = item.part * p.l.item_tokens, rows = line_tokens(p.l, item) * G;
                         share = PackedShare{item.t0 + token0, rows, item.kh, item.past + token0, item.seq, line_keys(p.l, item), item.j, j1 - item.j, min(2 * (j1 - item.j), (line_keys(p.l, item) - 128 * item.j + 63) / 64),
                                             item.j == 0 && j1 == item.tiles};
                         if (j1 < item.tiles && item.j == 0) note = PackedNote{1, note.closes, item.t0 + token0, rows, item.kh};
@@ -268,9 +271,9 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                     if (whole && lane < 16) tma_load_3d(slot + half * 16384 + i * 2048, is_v ? &maps.v : &maps.k, (int)(half * 64), (int)kh, page * (int)PAGE, &full[is_v][s]);
                 }
             }
-            if (walks && ok) {
-                const uint32_t j1 = item.first == end_first ? end_j : item.tiles;
-                more = j1 == item.tiles && line_next(p.l, item) && (item.first < end_first || (item.first == end_first && end_j > 0));
+            if (walks && ok && lane == 0) {
+                const uint32_t j1 = item.first == end.first ? end.j : item.tiles;
+                more = j1 == item.tiles && line_next(p.l, item) && (item.first < end.first || (item.first == end.first && end.j > 0));
             }
         }
         if (!Q8 && *abort_flag && lane == 0) {  // leaving early: let the copies in flight land before the block's shared memory is handed on
@@ -483,9 +486,9 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                 const float sum = (l[0] + l[1]) + (l[2] + l[3]);
                 const uint32_t r = 128 * x + row;
                 const bool live = r < rows;
-                bool bad = false;  // an output that is not finite
-                float *const dst = p.part + (size_t)(2 * blockIdx.x + (j0 == 0)) * packed_part_floats(ROWS);
+                float zeros = 0.0f;  // 0 times every output: NaN when one is not finite
                 if (!share.whole) {
+                    float *dst = p.part + (size_t)(2 * blockIdx.x + (j0 == 0)) * packed_part_floats(ROWS);
                     if (live) {
                         dst[ROWS * D + r] = m * LOG2E;
                         dst[ROWS * D + ROWS + r] = sum;
@@ -496,7 +499,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                         tmem_ld32(to + 32 * c, o);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) bad = bad || not_finite(__uint_as_float(o[e]));
+                        for (int e = 0; e < 32; ++e) zeros = fmaf(__uint_as_float(o[e]), 0.0f, zeros);
 #pragma unroll
                         for (int g = 0; g < 8; ++g)
                             if (live) reinterpret_cast<uint4 *>(dst + (size_t)r * D)[8 * c + g] = make_uint4(o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]);
@@ -510,7 +513,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                         tmem_ld32(to + 32 * c, o);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) bad = bad || not_finite(__uint_as_float(o[e]));
+                        for (int e = 0; e < 32; ++e) zeros = fmaf(__uint_as_float(o[e]), 0.0f, zeros);
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
                             const __half2 hh = __floats2half2_rn(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
@@ -530,7 +533,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                     }
                 }
                 const uint32_t upto = min(share.nkeys, 128 * (j0 + share.len));
-                uint32_t again = __ballot_sync(0xffffffffu, live && bad && seen_all < upto);
+                uint32_t again = __ballot_sync(0xffffffffu, live && zeros != 0.0f && seen_all < upto);
 #pragma unroll 1
                 for (__syncwarp(); again; again &= again - 1) {  // (see packed_row_again)
                     const uint32_t re = 128 * x + wrow + __ffs(again) - 1, tk = row_token(p.l, re);
@@ -541,6 +544,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                         const __half2 a = __floats2half2_rn(y.o.x * f, y.o.y * f), b = __floats2half2_rn(y.o.z * f, y.o.w * f);
                         reinterpret_cast<uint2 *>(p.o + at)[lane] = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
                     } else {
+                        float *dst = p.part + (size_t)(2 * blockIdx.x + (j0 == 0)) * packed_part_floats(ROWS);
                         reinterpret_cast<float4 *>(dst + (size_t)re * D)[lane] = y.o;
                         if (lane == 0) {
                             dst[ROWS * D + re] = y.m;
