@@ -692,6 +692,7 @@ __global__ void __launch_bounds__(256) attn_packed_merge_kernel(PackedParts a, P
 
 // What both operators ask of a run beside its pool; the run's view for the kernels.
 int32_t packed_view(brasa_ctx *ctx, const char *who, const brasa_paged_kv &pg, const brasa_packed_run &run, uint32_t hq, uint32_t hkv, PackedView *out) {
+    BRASA_REQUIRE(ctx, (uint64_t)pg.max_pages * PAGE < 1ull << 31, "%s: max_pages for 2^31 positions or more", who);
     BRASA_TRY(brasa_check_paged(ctx, pg, hq, hkv));
     BRASA_REQUIRE(ctx, hq > 0, "%s: no heads", who);
     BRASA_REQUIRE(ctx, run.tokens >= 1 && run.longest >= 1, "%s: empty run", who);

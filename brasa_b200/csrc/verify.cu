@@ -213,8 +213,9 @@ extern "C" int32_t brasa_k_verify_drafts(brasa_cmd *cmd, brasa_arg p, brasa_arg 
     VerifyParams a{(const float *)arg_ptr(p), (const float *)arg_ptr(q), (const float *)arg_ptr(u), (const uint32_t *)arg_ptr(drafts), (const uint32_t *)arg_ptr(starts),
                    (uint32_t *)arg_ptr(tokens), (uint32_t *)arg_ptr(accepted), seqs, rows, vocab, drafts.buf ? (drafts.buf->bytes - drafts.offset) / 4 : 0};
     if (q.buf) a.ndrafts = std::min(a.ndrafts, (q.buf->bytes - q.offset) / 4 / vocab);
-    // 16 warps a block while the blocks fit the SMs' places in one go (two to an SM), eight where there are more: 64 sequences of 151 936 ids with q 23 us (3.4 TB/s), one without 9.3.
-    const bool wide = seqs * CLUSTER <= 2 * (uint32_t)ctx->sm_count;
+    // 16 warps a block while all blocks are resident at once (clusters of eight fill 128 of the SMs, two blocks to each), eight warps where there are more sequences. 151 936 ids
+    // with q, 16 | 8 warps: 1 sequence 23.4 | 28.9 us, 32 sequences 27.7 | 34.4, 34 sequences 37.6 | 34.1, 64 sequences 42 | 35 (each behind a flush of the L2).
+    const bool wide = seqs <= 32;
     BRASA_CUDA(ctx, brasa_launch_dependent(ctx, wide ? verify_drafts_kernel<512> : verify_drafts_kernel<256>, dim3(seqs * CLUSTER), dim3(wide ? 512 : 256), 0, a));
     return brasa_post_launch(cmd, "verify_drafts");
 }

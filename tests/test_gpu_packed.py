@@ -450,6 +450,108 @@ def test_compact(ctx, K, rows, max_pages, num_pages, layers, hkv, kv, in_place):
             b.free()
 
 
+def test_recorded_steps_of_two_sizes(B, ctx, K):
+    """Verification and pages out of recorded graphs: two graphs of one context share its workspaces, the second made them grow, and each replay follows what
+    the buffers hold by then."""
+    g = np.random.default_rng(31)
+
+    class Step:
+        def __init__(self, rows, max_pages, num_pages):
+            self.P = P = Pages(g, rows, max_pages, num_pages, 2, 1, "f16", 0.5)
+            self.p, self.q, self.d, self.u, self.starts = random_verify(g, rows, 3, 500, True)
+            self.pool = P.device(ctx, K)
+            self.ver = [ctx.buffer_from(x) for x in (self.p, self.q, self.d, self.u, self.starts)] + [ctx.buffer(4 * len(self.p)), ctx.buffer(4 * rows)]
+            self.src, self.room = np.arange(rows, dtype=np.int32), np.full(rows, 4, np.uint32)
+            self.ins = [ctx.buffer_from(self.src), ctx.buffer_from(self.room)]
+            self.table, self.lens, self.moved = ctx.buffer(P.table.nbytes), ctx.buffer(4 * rows), ctx.buffer(4 * num_pages)
+            self.results = ctx.buffer(16), ctx.buffer(16)
+            self.after = K.page_pool(*P.bufs[:2], self.table, self.lens, P.bufs[4], rows, max_pages, num_pages, 2, 1, 1)
+
+        def __call__(self, c):
+            K.verify_drafts(c, *self.ver[:5], len(self.src), len(self.p), 500, *self.ver[5:])
+            K.pages_reassign(c, self.pool, self.ins[0], None, self.ins[1], self.table, self.lens, self.results[0], accepted=self.ver[6])
+            K.pages_compact(c, self.after, self.table, self.moved, self.results[1])
+
+        def reset(self):
+            self.u = g.random(len(self.u)).astype(np.float32)
+            self.src = g.integers(-1, len(self.src), len(self.src)).astype(np.int32)
+            for b, x in zip(self.P.bufs[:2] + [self.ver[3], self.ins[0]], (self.P.k, self.P.v, self.u, self.src)):
+                b.upload(x)
+
+        def check(self):
+            P = self.P
+            tokens, acc = np.zeros(len(self.p), np.uint32), np.zeros(len(self.src), np.uint32)
+            R.verify(self.p, self.q, self.d, self.u, self.starts, tokens, acc)
+            assert (self.ver[5].download(np.uint32) == tokens).all() and (self.ver[6].download(np.uint32) == acc).all()
+            table, lens, result, copies = R.reassign(P.table, P.lens, P.pinned, P.num_pages, self.src, None, self.room, acc)
+            last, moved, after, moves = R.compact(table, P.pinned, P.num_pages)
+            assert (self.lens.download(np.uint32) == lens).all() and list(self.results[0].download(np.uint32)) == result
+            assert (self.table.download(np.int32).reshape(last.shape) == last).all() and list(self.results[1].download(np.uint32)) == after
+            for b, was in zip(P.bufs[:2], (P.k, P.v)):
+                want = was.copy()
+                for x, to in copies:
+                    want[:, to] = was[:, x]
+                then = want.copy()
+                for x, to in moves:
+                    then[:, to] = want[:, x]
+                assert (b.download(np.uint8).reshape(was.shape) == then).all()
+
+    small = Step(3, 5, 40)
+    go(ctx, small)
+    small.check()
+    graphs = [ctx.capture(small)]
+    large = Step(50, 9, 900)
+    go(ctx, large)
+    large.check()
+    graphs.append(ctx.capture(large))
+    for _ in range(3):
+        for x in (small, large):
+            x.reset()
+        cmd = ctx.command()
+        for graph in graphs:
+            graph.launch(cmd)
+        cmd.wait()
+        for x in (small, large):
+            x.check()
+    for graph in graphs:
+        graph.free()
+
+
+def test_two_contexts_at_once(B, ctx, K):
+    """Calls of two contexts, in flight together: each has its own stream and workspaces."""
+    run = R.Run([(130, 600), (5, 2000), (1, 40)], 8, 2, "f16", seed=41)
+    want, tol = run.attention(True)
+    other = B.Context(0)
+    sides = []
+    for c in (ctx, other):
+        k = B.Kernels(c)
+        sides.append((c, k, OnDevice(c, k, run), c.buffer(run.tokens * 8 * 256)))
+    for c, k, dev, o in sides:  # (the first call makes the workspaces)
+        go(c, lambda cmd: k.attention_packed(cmd, dev.q, dev.paged, dev.packed, o, 8, 2, 0))
+        o.fill(0)
+    cmds = [c.command() for c, *_ in sides]
+    for _ in range(8):
+        for cmd, (c, k, dev, o) in zip(cmds, sides):
+            k.attention_packed(cmd, dev.q, dev.paged, dev.packed, o, 8, 2, 0)
+    for cmd in cmds:
+        cmd.wait()
+    for c, k, dev, o in sides:
+        check(o.download(np.float16).astype(np.float64).reshape(run.tokens, 8, 128), want, tol)
+        o.free()
+        dev.free()
+    other.close()
+
+
+def test_refusals_of_positions_past_31_bits(B, ctx, K):
+    run = R.Run([(2, 20)], 4, 2, "f16")
+    dev = OnDevice(ctx, K, run)
+    far = K.paged_kv(dev.kpool, dev.vpool, dev.bufs[2], dev.bufs[3], 1, 2 ** 27, run.num_pages, 1)
+    o = ctx.buffer(run.tokens * 4 * 256)
+    with pytest.raises(B.BrasaError, match="2\\^31 positions") as e:
+        go(ctx, lambda c: K.attention_packed(c, dev.q, far, dev.packed, o, 4, 2, 0))
+    assert e.value.code == B.EINVAL
+
+
 def test_refusals(B, ctx, K):
     """Every precondition comes back as EINVAL, with nothing launched."""
     run = R.Run([(2, 20), (1, 3)], 4, 2, "f16")
