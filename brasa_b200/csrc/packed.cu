@@ -12,7 +12,8 @@ constexpr int D = 128;
 
 // y = x / sqrt(mean x^2 + eps) * w of rows of q and k, rotated by the token's own position (pairs i, i + 64), and the store of k and v. Bound by memory: q read
 // and written, k and v read, the cache's rows written. A warp takes four rows of a token (a lane four dims of each, so that a row is one
-// request and a pair's other half lies sixteen lanes on), asks for all of them first and finds the token's sequence, position and page meanwhile.
+// request and a pair's other half lies sixteen lanes on), asks for all of them first and finds the token's sequence, position and page meanwhile. 9 prompts of
+// 7257 tokens (32 heads on 8, f16) 70 us, 4.7 TB/s (one row a warp: 92 us).
 constexpr uint32_t STORE_ROWS = 4;
 
 // four dims a lane of one row, rounded to the cache type
@@ -85,7 +86,10 @@ __global__ void __launch_bounds__(256) qk_norm_rope_store_packed_kernel(const fl
 // running maximum, sum and output (the maximum moves only when a score passes it by 2^8), the warps meet at the item's end. The 16 keys of a
 // warp's step are one page: a page that is none is skipped, and rows of the cache that the sequence has not reached are never loaded.
 // HALF: one f16 term of q * scale and of P, 8-bit rows as f16(d * code): what the F16 precision says. Otherwise q and P enter as two terms, hi + lo
-// (2^-22 of the value), and an f16 cache's rows as they are.
+// (2^-22 of the value), and an f16 cache's rows as they are. l sums the weights as the product reads them, by a column of ones beside V.
+// Bound by the cache's bytes while an item has one row tile or two, by mma.sync and its waits beyond that, where the tcgen05 kernel takes over (PACKED_TC_MIN_ROWS). 64
+// sequences of two to five tokens behind 2600 (32 heads on 8, f16) 153 us, 4.6 TB/s; 16 of three behind 3000 with an 8-bit cache 67 us against 68 with an f16
+// one: there the conversions bound it (5 instructions for two codes), 1.6 TB/s.
 struct FewParams {
     PackedLine l;
     const float *q;
@@ -97,11 +101,13 @@ struct FewParams {
     float scale;
     uint32_t late_wait;
 };
-constexpr uint32_t FEW_ROWS = 64, FEW_KEYS = 64;
+// FEW_BLOCKS: of an SM. 8 bit, the 16 sequences above and 28 of 2000 to 6000 positions (64 heads on 8): two blocks of four stages 77 and 158 us, three
+// of three 81 and 163, four of two 100 and 199 (before the copies had a page to a warp).
+constexpr uint32_t FEW_ROWS = 64, FEW_KEYS = 64, FEW_BLOCKS = 2;
 template <int KV> struct FewStage;
-template <> struct FewStage<BRASA_KV_F16> { static constexpr uint32_t K_PITCH = 256, V_PITCH = 256, STAGES = 3, BLOCKS = 2; };
+template <> struct FewStage<BRASA_KV_F16> { static constexpr uint32_t K_PITCH = 256, V_PITCH = 256, STAGES = 3; };
 // (pitches at which neither the 8-byte reads of K nor the transposed reads of V meet in a bank)
-template <> struct FewStage<BRASA_KV_Q8_0> { static constexpr uint32_t K_PITCH = 160, V_PITCH = 144, STAGES = 4, BLOCKS = 2; };
+template <> struct FewStage<BRASA_KV_Q8_0> { static constexpr uint32_t K_PITCH = 160, V_PITCH = 144, STAGES = 4; };
 template <int KV> constexpr uint32_t few_stage_bytes() { return FEW_KEYS * (FewStage<KV>::K_PITCH + FewStage<KV>::V_PITCH); }
 constexpr uint32_t FEW_TS = D + 4;
 
@@ -160,7 +166,7 @@ __device__ __forceinline__ void terms_h2(float x, float y, uint32_t &hi, uint32_
     }
 }
 template <int KV, bool HALF>
-__global__ void __launch_bounds__(128, FewStage<KV>::BLOCKS) attn_packed_few_kernel(const __grid_constant__ FewParams p) {
+__global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const __grid_constant__ FewParams p) {
     // Launched as a programmatic dependent. late_wait: the kernel before this one is the same call's tensor-core form, which has itself waited for what both read
     // and whose output this one does not touch: the two run side by side, and this one waits for the other at its end, so that whoever waits for it has
     // waited for both.
@@ -449,7 +455,7 @@ __global__ void __launch_bounds__(128, FewStage<KV>::BLOCKS) attn_packed_few_ker
 // ---- 32-bit arithmetic: an f32 cache, or an 8-bit one whose values keep all their bits -------------------------------------------------------------
 // A block has up to 64 rows and takes 64 keys at a time as f32 in shared memory, K's next tile on its way while V's is used. 256 threads in a square: scores four
 // rows by four keys each (keys 16 apart, so that a quarter warp's reads of K meet in no bank), outputs four rows by eight dims. Bound by the FMA units
-// with many rows, by the cache's bytes with few.
+// with many rows, by the cache's bytes with few: 2100 prompt tokens (8 heads on 2) 30 TFLOP/s, two to five tokens a sequence 1.5 TB/s.
 constexpr uint32_t F32_THREADS = 256, F32_P = 68;
 constexpr size_t F32_SMEM = (3 * 64 * (size_t)FEW_TS + 64 * F32_P) * sizeof(float);
 
@@ -648,7 +654,7 @@ struct PackedParts {
     uint32_t pieces, rows_item, spread;  // blocks, rows of an item, merging blocks to a piece
 };
 // Such an item is the work of the piece that began and left it open, each of that piece's `spread` blocks with every spread * 8-th row: the sum of 2^(m - M) O over
-// that of 2^(m - M) l, in the order of the keys.
+// that of 2^(m - M) l, in the order of the keys. Latency: it is part of the 12 us of a call for one token behind 700.
 template <bool HALF>
 __global__ void __launch_bounds__(256) attn_packed_merge_kernel(PackedParts a, PackedParts b, void *o, uint32_t hq, PackedLine l) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -752,12 +758,12 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
     const uint32_t G = hq / hkv, sms = ctx->sm_count;
     const bool f32 = pg.kv == BRASA_KV_F32 || (pg.kv == BRASA_KV_Q8_0 && !half);
     const bool tc = half && !f32 && (uint64_t)run.longest * G >= PACKED_TC_MIN_ROWS && (uint64_t)pg.num_pages * PAGE < 1ull << 31;
-    const uint32_t blocks = sms * (f32 ? 1 : (pg.kv == BRASA_KV_Q8_0 ? FewStage<BRASA_KV_Q8_0>::BLOCKS : FewStage<BRASA_KV_F16>::BLOCKS));
+    const uint32_t blocks = sms * (f32 ? 1 : FEW_BLOCKS);
     // the workspace: parts of either kernel's items, then what they belong to
-    const size_t few_floats = 2 * (size_t)(2 * sms) * packed_part_floats(FEW_ROWS), tc_floats = 2 * (size_t)sms * packed_part_floats(PACKED_TC_ROWS);
-    BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, (few_floats + tc_floats) * sizeof(float) + 3 * sms * sizeof(PackedNote)));
+    const size_t few_floats = 2 * (size_t)(FEW_BLOCKS * sms) * packed_part_floats(FEW_ROWS), tc_floats = 2 * (size_t)sms * packed_part_floats(PACKED_TC_ROWS);
+    BRASA_TRY(brasa_workspace(ctx, (void **)&ctx->packed_work, &ctx->packed_work_bytes, (few_floats + tc_floats) * sizeof(float) + (FEW_BLOCKS + 1) * sms * sizeof(PackedNote)));
     float *few_part = (float *)ctx->packed_work, *tc_part = few_part + few_floats;
-    PackedNote *few_notes = (PackedNote *)(tc_part + tc_floats), *tc_notes = few_notes + 2 * sms;
+    PackedNote *few_notes = (PackedNote *)(tc_part + tc_floats), *tc_notes = few_notes + FEW_BLOCKS * sms;
     if (tc) BRASA_TRY(brasa_packed_tc_launch(cmd, p, pg.kv, (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), tc_part, tc_notes, hq, scale));
     const FewParams f{packed_line(p, G, FEW_ROWS, 6, 1, 1, 3, 1, tc ? PACKED_TC_MIN_ROWS - 1 : UINT32_MAX), (const float *)arg_ptr(q), arg_ptr(pg.kpool), arg_ptr(pg.vpool), arg_ptr(o), few_part,
                       few_notes, hq, scale, tc ? 1u : 0u};

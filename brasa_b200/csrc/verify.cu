@@ -5,6 +5,7 @@
 // One row of p (and of q) per sequence is all that has to be read: 2 x 0.6 MB for a vocabulary of 151 936, so a cluster of eight blocks
 // takes a sequence, each with an eighth of the ids. Masses and their sums are 64-bit: p - q of two f32 numbers is exact up to the last
 // bits, and where the running sum passes the drawn point is decided far below the smallest mass. The sums' order depends on the vocabulary alone.
+// 64 sequences of 151 936 ids with q 23 us (3.4 TB/s), bound by two passes of a cluster whose second waits for the first; one sequence without q 9.3 us, latency.
 #include "brasa_internal.h"
 
 namespace {

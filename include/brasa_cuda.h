@@ -452,7 +452,9 @@ int32_t brasa_k_qk_norm_rope_store_packed(brasa_cmd *cmd, brasa_arg q, brasa_arg
 /* Causal attention of the run's tokens: a token attends to the positions of its sequence up to its own, which the call before it has
  * stored. q f32 [tokens][hq][128]; precision F16: o f16 [tokens][hq][128], q * scale, the weights and an 8-bit cache's
  * values rounded to f16, sums in 32 bits; F32: o f32, 32-bit arithmetic. Cache rows that a sequence has not reached may hold anything, infinities and NaN included. A token
- * that sees no position gives zeros. */
+ * that sees no position gives zeros. A token whose key or value is not finite counts for its own row and those behind it, never for one
+ * before it. o and q must not overlap. max_pages up to 2^27 - 1. The first call of a context makes its workspace, so that it must not be one that is
+ * recorded; lengths, tables and starts are read on the device, a recorded call follows what they hold by then. */
 int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv paged, brasa_packed_run run, brasa_arg o, uint32_t hq, uint32_t hkv, int32_t precision);
 /* Verification of drafted tokens. Sequence s has rows starts[s] .. starts[s + 1] - 1 (u32 [seqs + 1], not falling, at most `rows`) of p
  * f32 [rows][vocab], the target model's probabilities behind its last token and behind each of its drafted ones, so one row more
@@ -485,7 +487,7 @@ typedef struct brasa_page_pool {
  * on, to the rows in order (a copy's page ahead of those for new positions). Table entries that name no page are kept as -1.
  * table_out i32 [rows][max_pages] and lens_out u32 [rows] must not overlap table and lens. result u32[4]: pages in use (pinned ones among them), pages
  * copied, pages free, pages missing; when pages are missing nothing is copied and table_out and lens_out are table and lens (entries
- * that name no page are -1). */
+ * that name no page are -1). The first call with so many rows and pages makes the workspace of this and the next call: that one must not be recorded. */
 int32_t brasa_k_pages_reassign(brasa_cmd *cmd, brasa_page_pool pool, brasa_arg source, brasa_arg keep, brasa_arg accepted, brasa_arg room, brasa_arg table_out,
                                brasa_arg lens_out, brasa_arg result);
 /* Moves pages to the front of the pool: the highest page in use that is not pinned to the lowest free one, until none lies behind a free
