@@ -654,7 +654,7 @@ struct PackedParts {
     uint32_t pieces, rows_item, spread;  // blocks, rows of an item, merging blocks to a piece
 };
 // Such an item is the work of the piece that began and left it open, each of that piece's `spread` blocks with every spread * 8-th row: the sum of 2^(m - M) O over
-// that of 2^(m - M) l, in the order of the keys. Latency: it is part of the 12 us of a call for one token behind 700.
+// that of 2^(m - M) l, O in the order of the keys, l in that of a tree: the same every time. Latency bounds it, so that notes, weights and parts are asked for many at a time.
 template <bool HALF>
 __global__ void __launch_bounds__(256) attn_packed_merge_kernel(PackedParts a, PackedParts b, void *o, uint32_t hq, PackedLine l) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -667,8 +667,13 @@ __global__ void __launch_bounds__(256) attn_packed_merge_kernel(PackedParts a, P
     if (!n.opens || piece + 1 == p.pieces) return;  // (the line ends with a whole item)
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t step = packed_part_floats(rows_item);
-    uint32_t last = piece + 1;  // the piece that ends the item
-    while (last + 1 < p.pieces && !notes[last].closes) ++last;
+    uint32_t last = piece + 1;  // the piece that ends the item: mostly the next, otherwise 32 of them looked at together
+    if (last + 1 < p.pieces && !notes[last].closes)
+        for (uint32_t bits = 0; !bits;) {
+            const uint32_t k = last + 1 + lane;
+            bits = __ballot_sync(0xffffffffu, k + 1 >= p.pieces || notes[k].closes);
+            last += bits ? __ffs(bits) : 32;
+        }
     for (uint32_t r = share * 8 + warp; r < n.rows; r += p.spread * 8) {
         const float *ms = part + rows_item * D + r, *ls = ms + rows_item, *os = part + (size_t)r * D + 4 * lane;
         // (slot 2 b + 1 is what piece b left open, slot 2 k piece k's share of an item that began before it)
@@ -678,15 +683,35 @@ __global__ void __launch_bounds__(256) attn_packed_merge_kernel(PackedParts a, P
         for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
         float L = 0.0f;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        // Few parts: everything of a part asked for at once. Many (one row over many pieces): a part's weight to a lane, then only the parts themselves (one token behind
+        // 16 000: 64 -> 46 us; with it for all, the prompts of 16 138 tokens 577 -> 587).
+        if (last - piece < 8) {
 #pragma unroll 4
-        for (uint32_t k = piece; k <= last; ++k) {
-            const float m = ms[slot(k)], f = m == -INFINITY ? 0.0f : exp2_approx(m - M);
-            const float4 v = *reinterpret_cast<const float4 *>(os + slot(k));
-            L = fmaf(ls[slot(k)], f, L);
-            acc.x = fmaf(v.x, f, acc.x);
-            acc.y = fmaf(v.y, f, acc.y);
-            acc.z = fmaf(v.z, f, acc.z);
-            acc.w = fmaf(v.w, f, acc.w);
+            for (uint32_t k = piece; k <= last; ++k) {
+                const float m = ms[slot(k)], f = m == -INFINITY ? 0.0f : exp2_approx(m - M);
+                const float4 v = *reinterpret_cast<const float4 *>(os + slot(k));
+                L = fmaf(ls[slot(k)], f, L);
+                acc.x = fmaf(v.x, f, acc.x);
+                acc.y = fmaf(v.y, f, acc.y);
+                acc.z = fmaf(v.z, f, acc.z);
+                acc.w = fmaf(v.w, f, acc.w);
+            }
+        } else {
+            for (uint32_t k0 = piece; k0 <= last; k0 += 32) {
+                const uint32_t k = min(k0 + lane, last), many = min(32u, last - k0 + 1);
+                const float m = ms[slot(k)], mine = m == -INFINITY ? 0.0f : exp2_approx(m - M);  // (a part to a lane)
+                if (lane < many) L = fmaf(ls[slot(k)], mine, L);
+#pragma unroll 8
+                for (uint32_t e = 0; e < many; ++e) {
+                    const float4 v = *reinterpret_cast<const float4 *>(os + slot(k0 + e));
+                    const float f = __shfl_sync(0xffffffffu, mine, e);
+                    acc.x = fmaf(v.x, f, acc.x);
+                    acc.y = fmaf(v.y, f, acc.y);
+                    acc.z = fmaf(v.z, f, acc.z);
+                    acc.w = fmaf(v.w, f, acc.w);
+                }
+            }
+            for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
         }
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
         const uint32_t token = row_token(l, r);

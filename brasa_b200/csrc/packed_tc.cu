@@ -21,7 +21,7 @@
 // Bound by the round of a step, not by one unit: a row tile's scores, exponentials (16 a clock and SM, 1024 cycles for both row tiles' 64 keys), the weights' way
 // into tensor memory and their product follow one another, with two row tiles and two steps in flight; on the prompts below the tensor core works 40 % of the
 // time and the exponential unit 41 %. Measured: 1000 new tokens behind 9000 (64 heads on 8 key heads) 360 us, 865 TFLOP/s, with an 8-bit cache 459 us, 679 TFLOP/s (the
-// conversions take issue slots and registers from the softmax); 14 prompts of 16 138 tokens (32 on 8) 575 us, 645 TFLOP/s.
+// conversions take issue slots and registers from the softmax); 14 prompts of 16 138 tokens (32 on 8) 577 us, 642 TFLOP/s.
 #include <math.h>
 #include <string.h>
 
