@@ -776,6 +776,7 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
     const uint64_t n = (uint64_t)run.tokens * hq * D;
     BRASA_REQUIRE(ctx, arg_fits(q, n * 4) && arg_fits(o, n * (half ? 2 : 4)), "attention_packed: q or o too small");
     BRASA_REQUIRE(ctx, q.offset % 16 == 0 && o.offset % 16 == 0, "attention_packed: misaligned buffer");
+    BRASA_REQUIRE(ctx, q.buf != o.buf || q.offset + n * 4 <= o.offset || o.offset + n * (half ? 2 : 4) <= q.offset, "attention_packed: o must not overlap q");
     BRASA_REQUIRE(ctx, (uint64_t)run.tokens * (hq / hkv) < 1ull << 31, "attention_packed: more than 2^31 rows of a key head's group");
     const float scale = 1.0f / sqrtf((float)D);
     // Sequences of many rows go to the tensor-core kernel where there is one (16-bit products) and the call can have any. What is neither an f16 cache nor 16-bit

@@ -552,6 +552,21 @@ def test_refusals_of_positions_past_31_bits(B, ctx, K):
     assert e.value.code == B.EINVAL
 
 
+def test_refusals_of_an_output_over_the_queries(B, ctx, K):
+    run = R.Run([(2, 20)], 4, 2, "f16")
+    dev = OnDevice(ctx, K, run)
+    n = run.tokens * 4 * 128
+    both = ctx.buffer(n * 8)
+    for half, at in ((True, 0), (True, 2 * n), (False, 0), (False, 4 * n - 16)):
+        with pytest.raises(B.BrasaError, match="overlap") as e:
+            go(ctx, lambda c: K.attention_packed(c, both, dev.paged, dev.packed, both.at(at), 4, 2, 0 if half else 1))
+        assert e.value.code == B.EINVAL
+    both.upload(run.q, 0)
+    go(ctx, lambda c: K.attention_packed(c, both, dev.paged, dev.packed, both.at(4 * n), 4, 2, 1))
+    want, tol = run.attention(False)
+    check(both.download(np.float32)[n:].astype(np.float64).reshape(run.tokens, 4, 128), want, tol)
+
+
 def test_refusals(B, ctx, K):
     """Every precondition comes back as EINVAL, with nothing launched."""
     run = R.Run([(2, 20), (1, 3)], 4, 2, "f16")
