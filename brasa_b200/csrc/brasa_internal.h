@@ -187,6 +187,9 @@ static inline uint8_t *arg_ptr(const brasa_arg &a) {
 static inline bool arg_fits(const brasa_arg &a, uint64_t n) {
     return a.buf && a.offset <= a.buf->bytes && n <= a.buf->bytes - a.offset;
 }
+static inline bool arg_overlap(const brasa_arg &a, uint64_t an, const brasa_arg &b, uint64_t bn) {
+    return a.buf == b.buf && an && bn && a.offset < b.offset + bn && b.offset < a.offset + an;
+}
 static inline bool qm_fits(const brasa_qmatrix &m) {
     return arg_fits(m.data, brasa_qtype_nbytes(m.qtype, (uint64_t)m.rows * m.cols));
 }

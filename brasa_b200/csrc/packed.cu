@@ -750,6 +750,9 @@ int32_t brasa_k_qk_norm_rope_store_packed(brasa_cmd *cmd, brasa_arg q, brasa_arg
     BRASA_REQUIRE(ctx, arg_fits(rope_cos, table_bytes) && arg_fits(rope_sin, table_bytes), "qk_norm_rope_store_packed: RoPE tables shorter than max_pages pages");
     for (const brasa_arg *a : {&q, &k, &v, &q_norm, &k_norm, &rope_cos, &rope_sin, &q_out})
         BRASA_REQUIRE(ctx, a->offset % 16 == 0, "qk_norm_rope_store_packed: misaligned buffer");
+    // (in place every warp writes the rows that it has read)
+    BRASA_REQUIRE(ctx, ((q.buf == q_out.buf && q.offset == q_out.offset) || !arg_overlap(q, nq, q_out, nq)) && !arg_overlap(k, nkv, q_out, nq) && !arg_overlap(v, nkv, q_out, nq),
+                  "qk_norm_rope_store_packed: q_out must be q or overlap none of q, k and v");
     const uint32_t per_tok = (hq + 2 * hkv + STORE_ROWS - 1) / STORE_ROWS;
     const uint64_t warps = (uint64_t)run.tokens * per_tok;
     BRASA_REQUIRE(ctx, warps <= 1ull << 33, "qk_norm_rope_store_packed: more than 2^35 rows");
@@ -776,7 +779,7 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
     const uint64_t n = (uint64_t)run.tokens * hq * D;
     BRASA_REQUIRE(ctx, arg_fits(q, n * 4) && arg_fits(o, n * (half ? 2 : 4)), "attention_packed: q or o too small");
     BRASA_REQUIRE(ctx, q.offset % 16 == 0 && o.offset % 16 == 0, "attention_packed: misaligned buffer");
-    BRASA_REQUIRE(ctx, q.buf != o.buf || q.offset + n * 4 <= o.offset || o.offset + n * (half ? 2 : 4) <= q.offset, "attention_packed: o must not overlap q");
+    BRASA_REQUIRE(ctx, !arg_overlap(q, n * 4, o, n * (half ? 2 : 4)), "attention_packed: o must not overlap q");
     BRASA_REQUIRE(ctx, (uint64_t)run.tokens * (hq / hkv) < 1ull << 31, "attention_packed: more than 2^31 rows of a key head's group");
     const float scale = 1.0f / sqrtf((float)D);
     // Sequences of many rows go to the tensor-core kernel where there is one (16-bit products) and the call can have any. What is neither an f16 cache nor 16-bit

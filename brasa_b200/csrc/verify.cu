@@ -211,6 +211,12 @@ extern "C" int32_t brasa_k_verify_drafts(brasa_cmd *cmd, brasa_arg p, brasa_arg 
     BRASA_REQUIRE(ctx, arg_fits(drafts, nd * 4) && (!q.buf || arg_fits(q, nd * vocab * 4)), "verify_drafts: drafts or q too small");
     BRASA_REQUIRE(ctx, arg_fits(tokens, (uint64_t)rows * 4) && arg_fits(accepted, (uint64_t)seqs * 4), "verify_drafts: tokens or accepted too small");
     for (const brasa_arg *a : {&p, &q, &drafts, &u, &starts, &tokens, &accepted}) BRASA_REQUIRE(ctx, a->offset % 4 == 0, "verify_drafts: misaligned buffer");
+    // sequences run side by side, and a sequence's tokens begin behind its drafts' places: nothing can be written in place
+    const std::pair<const brasa_arg *, uint64_t> ins[] = {{&p, (uint64_t)rows * vocab * 4}, {&q, nd * vocab * 4}, {&drafts, nd * 4}, {&u, (uint64_t)rows * 4}, {&starts, ((uint64_t)seqs + 1) * 4}};
+    for (const auto &i : ins)
+        BRASA_REQUIRE(ctx, !arg_overlap(*i.first, i.second, tokens, (uint64_t)rows * 4) && !arg_overlap(*i.first, i.second, accepted, (uint64_t)seqs * 4),
+                      "verify_drafts: tokens and accepted must not overlap what is read");
+    BRASA_REQUIRE(ctx, !arg_overlap(tokens, (uint64_t)rows * 4, accepted, (uint64_t)seqs * 4), "verify_drafts: tokens and accepted must not overlap");
     VerifyParams a{(const float *)arg_ptr(p), (const float *)arg_ptr(q), (const float *)arg_ptr(u), (const uint32_t *)arg_ptr(drafts), (const uint32_t *)arg_ptr(starts),
                    (uint32_t *)arg_ptr(tokens), (uint32_t *)arg_ptr(accepted), seqs, rows, vocab, drafts.buf ? (drafts.buf->bytes - drafts.offset) / 4 : 0};
     if (q.buf) a.ndrafts = std::min(a.ndrafts, (q.buf->bytes - q.offset) / 4 / vocab);

@@ -444,7 +444,7 @@ typedef struct brasa_packed_run {
     uint32_t tokens;  /* rows of the buffers, at least starts[seqs] */
     uint32_t longest; /* the most tokens one sequence has in this run */
 } brasa_packed_run;
-/* brasa_k_qk_norm_rope_store_paged for such a run: q f32 [tokens][hq][128] is normalised and rotated into q_out (which may be q), k and
+/* brasa_k_qk_norm_rope_store_paged for such a run: q f32 [tokens][hq][128] is normalised and rotated into q_out (q itself or apart from q, k and v), k and
  * v f32 [tokens][hkv][128] are read: normalised and rotated k, and v, are rounded to the cache type and stored into the pages. No two
  * tokens may share a place of the pool. Tables as for the paged call: every position that max_pages pages reach. */
 int32_t brasa_k_qk_norm_rope_store_packed(brasa_cmd *cmd, brasa_arg q, brasa_arg k, brasa_arg v, brasa_arg q_norm, brasa_arg k_norm, brasa_arg rope_cos,
@@ -465,7 +465,8 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pag
  * from p of the last row when none was refused: the first id at which the running sum, from id 0 on and in 64 bits, exceeds u times the
  * whole. q.buf NULL: the drafts were not drawn but given, q is 1 at the draft and 0 elsewhere. Entries that are no positive finite
  * numbers count as 0, a draft that is not below vocab is refused; where max(p - q, 0) holds nothing p takes its place, and
- * where p does not either the token is 0. Rows of no sequence are left alone, one without rows gets accepted 0. */
+ * where p does not either the token is 0. Rows of no sequence are left alone, one without rows gets accepted 0.
+ * tokens and accepted must overlap neither one another nor what is read. */
 int32_t brasa_k_verify_drafts(brasa_cmd *cmd, brasa_arg p, brasa_arg q, brasa_arg drafts, brasa_arg u, brasa_arg starts, uint32_t seqs, uint32_t rows,
                               uint32_t vocab, brasa_arg tokens, brasa_arg accepted);
 /* Pages of all layers and who holds them, for a caller that keeps its own page tables: kpool, vpool [layers][num_pages]
@@ -485,7 +486,7 @@ typedef struct brasa_page_pool {
  * full, becomes its own to write into: the first row that ends in it keeps it, unless it is pinned or held as a whole page too, the
  * others get copies of it in all layers. Pages that no new row holds are free at once; free ones are handed out from the lowest
  * on, to the rows in order (a copy's page ahead of those for new positions). Table entries that name no page are kept as -1.
- * table_out i32 [rows][max_pages] and lens_out u32 [rows] must not overlap table and lens. result u32[4]: pages in use (pinned ones among them), pages
+ * table_out i32 [rows][max_pages] and lens_out u32 [rows] must not overlap one another or what is read. result u32[4]: pages in use (pinned ones among them), pages
  * copied, pages free, pages missing; when pages are missing nothing is copied and table_out and lens_out are table and lens (entries
  * that name no page are -1). The first call with so many rows and pages makes the workspace of this and the next call: that one must not be recorded. */
 int32_t brasa_k_pages_reassign(brasa_cmd *cmd, brasa_page_pool pool, brasa_arg source, brasa_arg keep, brasa_arg accepted, brasa_arg room, brasa_arg table_out,

@@ -567,6 +567,45 @@ def test_refusals_of_an_output_over_the_queries(B, ctx, K):
     check(both.download(np.float32)[n:].astype(np.float64).reshape(run.tokens, 4, 128), want, tol)
 
 
+def test_refusals_of_outputs_over_inputs(B, ctx, K):
+    """Two sequences' rows, pages and tokens are written side by side: outputs over what is read, or over one another, are refused; the queries in place are not."""
+    run = R.Run([(2, 20)], 4, 2, "f16")
+    dev, T = OnDevice(ctx, K, run), run.tokens
+    rope, norm, b = B.RopeTable(ctx, THETA, 128, run.max_pages * 16), ctx.buffer_from(np.ones(128, np.float32)), ctx.buffer(T * 512 * 16)
+    kv, far = b.at(T * 512 * 4), b.at(T * 512 * 8)
+
+    def store(q, out):
+        go(ctx, lambda c: K.qk_norm_rope_store_packed(c, q, kv, kv, norm, norm, EPS, rope, dev.paged, dev.packed, out, 4, 2))
+
+    x = ctx.buffer(4 * 300)
+    f = {n: ctx.buffer(4096) for n in ("p", "q", "d", "u", "s", "t", "a")}
+
+    def ver(out, acc):
+        go(ctx, lambda c: K.verify_drafts(c, f["p"], f["q"], f["d"], f["u"], f["s"], 2, 4, 100, out, acc))
+
+    pool = ctx.buffer(2 * 8 * 16 * 256)
+    page = K.page_pool(pool, pool, ctx.buffer(48), ctx.buffer(16), None, 4, 3, 8, 2, 1, 1)
+    a, room = ctx.buffer(16), ctx.buffer(64)
+
+    def rea(out, lens, res):
+        go(ctx, lambda c: K.pages_reassign(c, page, a, None, room, out, lens, res))
+
+    def com(out, moved, res):
+        go(ctx, lambda c: K.pages_compact(c, page, out, moved, res))
+    store(b, b), store(b, far), ver(x, x.at(16)), rea(x, x.at(48), x.at(64)), com(x, x.at(48), x.at(80))
+    before = ctx.launch_count()
+    bad = [(store, b, b.at(512)), (store, b.at(512), b), (store, far, kv), (store, far, b.at(T * 512 * 3)), (store, far, b.at(T * 512 * 6 - 512)),
+           (ver, f["d"], f["a"]), (ver, f["u"].at(12), f["a"]), (ver, f["p"].at(1596), f["a"]), (ver, f["q"].at(400), f["a"]), (ver, f["s"].at(8), f["a"]), (ver, f["t"], f["d"].at(4)),
+           (ver, f["t"], f["u"]), (ver, f["t"], f["t"].at(12)), (ver, f["t"].at(4), f["t"]),
+           (rea, x, x.at(44), x.at(64)), (rea, x, x.at(48), x.at(32)), (rea, x, x.at(48), x.at(60)), (rea, room, x.at(48), x.at(64)),
+           (com, x, x.at(44), x.at(80)), (com, x, x.at(48), x.at(76)), (com, x, x.at(48), x.at(40))]
+    for call, *args in bad:
+        with pytest.raises(B.BrasaError, match="overlap") as e:
+            call(*args)
+        assert e.value.code == B.EINVAL
+    assert ctx.launch_count() == before
+
+
 def test_refusals(B, ctx, K):
     """Every precondition comes back as EINVAL, with nothing launched."""
     run = R.Run([(2, 20), (1, 3)], 4, 2, "f16")
@@ -586,9 +625,9 @@ def test_refusals(B, ctx, K):
     def att(c, paged=dev.paged, packed=run2, q=q, o=o, hq=4, hkv=2, precision=0):
         K.attention_packed(c, q, paged, packed, o, hq, hkv, precision)
     short = B.RopeTable(ctx, THETA, 128, 16)
-    f = {x: ctx.buffer(4096) for x in "pquds"}
+    f = {x: ctx.buffer(4096) for x in "pqudsta"}
 
-    def ver(c, p=f["p"], q=f["q"], d=f["d"], u=f["u"], st=f["s"], seqs=2, rows=4, vocab=100, out=f["d"], acc=f["u"]):
+    def ver(c, p=f["p"], q=f["q"], d=f["d"], u=f["u"], st=f["s"], seqs=2, rows=4, vocab=100, out=f["t"], acc=f["a"]):
         K.verify_drafts(c, p, q, d, u, st, seqs, rows, vocab, out, acc)
     kp = ctx.buffer(2 * 8 * 16 * 256)
     tb, tb2, ln, ln2, pins = ctx.buffer(4 * 3 * 4), ctx.buffer(4 * 3 * 4), ctx.buffer(16), ctx.buffer(16), ctx.buffer(32)
