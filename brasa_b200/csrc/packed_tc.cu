@@ -32,7 +32,7 @@ using namespace brasa_dev;
 
 namespace {
 
-constexpr uint32_t PAGE = BRASA_KV_PAGE, D = 128, WAIT_LIMIT = 1u << 20, TILE_BYTES = 128 * 128 * 2, ROWS = PACKED_TC_ROWS;
+constexpr uint32_t PAGE = BRASA_KV_PAGE, D = 128, WAIT_LIMIT = 1u << 22, TILE_BYTES = 128 * 128 * 2, ROWS = PACKED_TC_ROWS;
 constexpr uint32_t SOFTMAX_WARPS = 8, MMA_WARP = 8, K_WARP = 10, V_WARP = 11;  // (one MMA warp for each row tile)
 constexpr uint32_t THREADS = 384, WARPS_Q8 = 3, THREADS_Q8 = 512;  // an 8-bit pool's K and V have three warps each
 
@@ -58,7 +58,9 @@ struct PackedShare {
     uint32_t j0, len, steps;      // first key tile, key tiles, steps of 64 keys as far as any are seen
     uint32_t whole;               // all of the item's keys
 };
-constexpr uint32_t SHARES = 8;  // (the copies are at most four items ahead of the outputs)
+// A place of the ring is written again when every warp is done with the share that it held: the second row tile's softmax has no part in an item of up to
+// 128 rows, and nothing else keeps the copies from going round while it is at an output.
+constexpr uint32_t SHARES = 8;
 
 // byte offset of the 16-byte piece of columns [c, c + 8) of row r in a swizzled 128 x 128 tile of 16-bit values
 __device__ __forceinline__ uint32_t tile_piece(uint32_t r, uint32_t c) {
@@ -100,7 +102,7 @@ template <bool Q8>
 __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_kernel(const __grid_constant__ PackedMaps maps, const __grid_constant__ PackedTcParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *ring = smem + 2 * TILE_BYTES;
-    __shared__ uint64_t full[2][2], freed[2][2], q_full[2], s_ready[2][2], p_ready[2][2], pv_done[2], o_done[2], turn[2], share_full[SHARES];
+    __shared__ uint64_t full[2][2], freed[2][2], q_full[2], s_ready[2][2], p_ready[2][2], pv_done[2], o_done[2], turn[2], share_full[SHARES], share_free[SHARES];
     __shared__ PackedShare shares[SHARES];
     __shared__ uint32_t tmem_base_s, abort_s, there_s[8];  // (there: of the last key tiles, which of their eight pages are pages)
     __shared__ PackedPieces pieces;
@@ -122,7 +124,10 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
             mbar_init(&turn[i], 4);  // of the other row tile's warps
             mbar_init(&o_done[i], 1);
         }
-        for (uint32_t i = 0; i < SHARES; ++i) mbar_init(&share_full[i], 1);
+        for (uint32_t i = 0; i < SHARES; ++i) {
+            mbar_init(&share_full[i], 1);
+            mbar_init(&share_free[i], 2 * (Q8 ? WARPS_Q8 : 1) - 1 + 2 + SOFTMAX_WARPS);  // by all warps but the one that walks
+        }
         abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -156,6 +161,10 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
     }
     const bool work = line_cut<256>(p.l, pieces) && !abort_s;
     auto share_at = [&](uint32_t i) -> bool { return all_wait(&share_full[i % SHARES], (i / SHARES) & 1); };  // the block's i-th share is handed on
+    auto share_done = [&](uint32_t i) {  // and this warp has read what it needs of it
+        __syncwarp();
+        if (lane == 0) tc_mbar_arrive(&share_free[i % SHARES]);
+    };
 
     if (warp >= K_WARP) {  // ---- copies, as far ahead of the products as there are slots; K's warp walks the line and hands the shares on ----
         const uint32_t is_v = (warp - K_WARP) & 1;
@@ -173,6 +182,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
         for (uint32_t n = 0; ok; ++n) {
             PackedShare &share = shares[n % SHARES];
             if (walks) {
+                if (n >= SHARES && !(ok = all_wait(&share_free[n % SHARES], (n / SHARES - 1) & 1))) break;
                 if (lane == 0) {
                     share.rows = 0;
                     if (more) {
@@ -283,6 +293,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                     if (whole && lane < 16) tma_load_3d(slot + half * 16384 + i * 2048, is_v ? &maps.v : &maps.k, (int)(half * 64), (int)kh, page * (int)PAGE, &full[is_v][s]);
                 }
             }
+            if (!walks) share_done(n);
             if (walks && ok && lane == 0) {
                 const uint32_t j1 = item.first == end.first ? end.j : item.tiles;
                 more = j1 == item.tiles && line_next(p.l, item) && (item.first < end.first || (item.first == end.first && end.j > 0));
@@ -353,6 +364,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                 ++segs;
             }
             loads += len;
+            share_done(i);
         }
         if (*abort_flag) {  // leaving early: the products in flight end before the block's memory is handed on (one commit more to the output's barrier)
             if (tc_elect_one()) tc_commit(&o_done[x]);
@@ -567,6 +579,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             }
             tiles0 += share.len;
+            share_done(i);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

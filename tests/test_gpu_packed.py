@@ -150,6 +150,29 @@ def test_attention_rows_before_a_bad_one(ctx, K, kv, half, bad):
             assert not np.isfinite(got[b:e]).any()
 
 
+@pytest.mark.parametrize("bad", ["k", "v"])
+@pytest.mark.parametrize("kv", ["f16", "q8_0"])
+def test_attention_many_short_items_behind_a_bad_one(ctx, K, kv, bad):
+    """An item of two row tiles whose second holds a value that is not finite, and more short items behind it in the same block's share of the work than the
+    block hands on at a time: every other sequence has the bits of the run without that value."""
+    seqs = [(60, 2000)] + [(9, 0)] * 2400  # 240 rows, then 36 each
+    run = R.Run(seqs, 8, 2, kv, seed=51)
+    clean, _ = attend(ctx, K, run, True)
+    tall, last = 60, [1, 9, 700, 2400]
+    run.seqs = [x if s == 0 or s in last else (0, x[1]) for s, x in enumerate(seqs)]
+    want, tol = run.attention(True)
+    for s in [0] + last:
+        a, b = int(run.starts[s]), int(run.starts[s + 1])
+        check(clean[a:b], want[a:b], tol[a:b])
+    j = 33 if bad == "k" else 59  # (rows 132 and on; all rows before the last token)
+    row = np.full((2, R.D), np.inf, np.float32)
+    raw = R.to_bytes(row, kv) if kv == "f16" else np.concatenate([np.ones((2, 128), np.uint8), row[:, :4].astype(np.float16).view(np.uint8)], -1)
+    (run.k if bad == "k" else run.v)[run.table[0, (2000 + j) // R.PAGE], (2000 + j) % R.PAGE] = raw
+    got, _ = attend(ctx, K, run, True)
+    check(got[:j], want[:j], tol[:j])
+    assert (got[tall:] == clean[tall:]).all()
+
+
 def test_attention_keeps_to_what_the_call_says(ctx, K):
     """`longest` and `tokens` below what starts say, starts that fall, positions behind the table: such rows are left alone."""
     run = R.Run([(3, 40), (150, 20), (2, 30)], 4, 2, "f16", seed=5)
