@@ -132,29 +132,6 @@ __device__ __forceinline__ uint32_t pack_h2(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// A block's rows that are to be taken again (bits of `rows`): the warps share them, and write over what the block wrote before the barrier ahead of this.
-template <int KV, bool HALF, uint32_t THREADS>
-__device__ __noinline__ void few_again(const FewParams &p, const PackedItem &it, uint64_t rows, uint32_t from, uint32_t to, bool whole, float *part) {
-    const uint32_t lane = threadIdx.x & 31, G = p.l.group, token0 = it.part * p.l.item_tokens;
-    for (uint32_t n = 0; rows; rows &= rows - 1, ++n) {
-        if (n % (THREADS / 32) != threadIdx.x >> 5) continue;
-        const uint32_t r = __ffsll(rows) - 1, token = row_token(p.l, r);
-        const size_t at = ((size_t)(it.t0 + token0 + token) * p.hq + it.kh * G + r - token * G) * D + 4 * lane;
-        const PackedRowSums x = packed_row_again<KV>(p.l.v, p.kpool, p.vpool, p.q + at - 4 * lane, p.scale, it.seq, it.kh, from, min(to, it.past + token0 + token + 1));
-        if (whole) {
-            const float inv = x.l == 0.0f ? 0.0f : 1.0f / x.l;
-            const float4 v = make_float4(x.o.x * inv, x.o.y * inv, x.o.z * inv, x.o.w * inv);
-            if (HALF) *reinterpret_cast<uint2 *>(static_cast<__half *>(p.o) + at) = make_uint2(pack_h2(v.x, v.y), pack_h2(v.z, v.w));
-            else *reinterpret_cast<float4 *>(static_cast<float *>(p.o) + at) = v;
-        } else {
-            reinterpret_cast<float4 *>(part + r * D)[lane] = x.o;
-            if (lane == 0) {
-                part[FEW_ROWS * D + r] = x.m;
-                part[FEW_ROWS * D + FEW_ROWS + r] = x.l;
-            }
-        }
-    }
-}
 // x, y -> f16 pair and, with two terms, the pair of what its rounding dropped
 template <bool HALF>
 __device__ __forceinline__ void terms_h2(float x, float y, uint32_t &hi, uint32_t &lo) {
@@ -180,7 +157,7 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PackedPieces pieces;
     __shared__ float sums[4][2][16];
-    __shared__ uint32_t again[2];  // rows whose output is not finite
+    __shared__ uint32_t again;  // a row is not finite although keys lie behind it
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem), hkv = p.l.v.hkv, G = p.l.group;
     PackedNote note{};
@@ -413,7 +390,7 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
                 }
             }
         }
-        if (tid < 2) again[tid] = 0;
+        if (tid == 0) again = 0;
         __syncthreads();
         const bool whole = j0 == 0 && j1 == it.tiles;
         const uint32_t upto = min(nkeys, 64 * j1);
@@ -427,7 +404,7 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
                 L = fmaf(sums[w][1][x], f, L);
                 acc = fmaf(reinterpret_cast<float *>(smem)[(w * 16 + x) * FEW_TS + tid], f, acc);
             }
-            if (not_finite(acc) && it.past + token0 + row_token(p.l, r) + 1 < upto) atomicOr(&again[r >> 5], 1u << (r & 31));
+            if (not_finite(acc) && it.past + token0 + row_token(p.l, r) + 1 < upto) again = 1;
             if (whole) {
                 const uint32_t token = row_token(p.l, r);
                 const size_t at = ((size_t)(t0 + token) * p.hq + it.kh * G + r - token * G) * D + tid;
@@ -445,7 +422,7 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
         if (!whole && j0 == 0) note = PackedNote{1, note.closes, t0, rows, it.kh};
         if (j0 > 0 && j1 == it.tiles) note.closes = 1;
         __syncthreads();  // the ring and the sums are free again
-        if (again[0] | again[1]) few_again<KV, HALF, 128>(p, it, again[0] | (uint64_t)again[1] << 32, 64 * j0, upto, whole, part);
+        if (again) packed_rows_again<KV, HALF>(p.l, PackedAgain{p.q, p.kpool, p.vpool, p.o, part, p.hq, p.scale, it.seq, it.kh, t0, rows, it.past + token0, 64 * j0, upto, FEW_ROWS, whole});
         if (j1 < it.tiles || !line_next(p.l, it)) break;
     }
     if (tid == 0) p.notes[blockIdx.x] = note;
@@ -465,7 +442,7 @@ __global__ void __launch_bounds__(F32_THREADS, 1) attn_packed_f32_kernel(const _
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(16) float fs[];
     __shared__ PackedPieces pieces;
-    __shared__ uint32_t again[2];  // rows whose output is not finite
+    __shared__ uint32_t again;  // a row is not finite although keys lie behind it
     float *qs = fs, *ks = qs + 64 * FEW_TS, *vs = ks + 64 * FEW_TS, *ps = vs + 64 * FEW_TS;
     const uint32_t tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, hkv = p.l.v.hkv, G = p.l.group;
     PackedNote note{};
@@ -602,7 +579,7 @@ __global__ void __launch_bounds__(F32_THREADS, 1) attn_packed_f32_kernel(const _
             __syncthreads();  // V and the weights are done with
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        if (tid < 2) again[tid] = 0;
+        if (tid == 0) again = 0;
         __syncthreads();
         const bool whole = j0 == 0 && j1 == it.tiles;
         const uint32_t upto = min(nkeys, 64 * j1);
@@ -616,7 +593,7 @@ __global__ void __launch_bounds__(F32_THREADS, 1) attn_packed_f32_kernel(const _
                 bool bad = false;
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) bad = bad || not_finite(o[a][e]);
-                if (bad && seen[a] < upto) atomicOr(&again[r >> 5], 1u << (r & 31));
+                if (bad && seen[a] < upto) again = 1;
                 if (whole) {
                     const uint32_t token = row_token(p.l, r);
                     const size_t at = ((size_t)(t0 + token) * p.hq + it.kh * G + r - token * G) * D + 4 * tx;
@@ -641,7 +618,7 @@ __global__ void __launch_bounds__(F32_THREADS, 1) attn_packed_f32_kernel(const _
         if (!whole && j0 == 0) note = PackedNote{1, note.closes, t0, rows, it.kh};
         if (j0 > 0 && j1 == it.tiles) note.closes = 1;
         __syncthreads();  // (q's place is free)
-        if (again[0] | again[1]) few_again<KV, HALF, F32_THREADS>(p, it, again[0] | (uint64_t)again[1] << 32, 64 * j0, upto, whole, part);
+        if (again) packed_rows_again<KV, HALF>(p.l, PackedAgain{p.q, p.kpool, p.vpool, p.o, part, p.hq, p.scale, it.seq, it.kh, t0, rows, it.past + token0, 64 * j0, upto, FEW_ROWS, whole});
         if (j1 < it.tiles || !line_next(p.l, it)) break;
     }
     if (tid == 0) p.notes[blockIdx.x] = note;

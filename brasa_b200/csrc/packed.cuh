@@ -59,60 +59,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
 
-// The sums of one row over the keys [from, to) of its sequence, a warp, four dims a lane: m, the sum of 2^(s - m) and that times V. This is for what the matrix
-// products cannot do: a weight of zero times an infinity or NaN of V is NaN, so that a key behind a row's own position, new in the same run, would
-// reach it. A kernel whose output is not finite although keys of the tile lie behind the row (`to` of it and more) takes the row again this way, without them.
-struct PackedRowSums {
-    float m, l;
-    float4 o;
-};
-template <int KV>
-__device__ __forceinline__ float4 packed_row4(const uint8_t *row, uint32_t lane) {
-    const float2 a = tile_at2<KV>(row, 4 * lane), b = tile_at2<KV>(row, 4 * lane + 2);
-    return make_float4(a.x, a.y, b.x, b.y);
-}
-template <int KV>
-__device__ __noinline__ PackedRowSums packed_row_again(const PackedView &v, const uint8_t *kpool, const uint8_t *vpool, const float *q, float scale, uint32_t seq, uint32_t kh, uint32_t from, uint32_t to) {
-    constexpr uint32_t AT_ONCE = 4;
-    const uint32_t lane = threadIdx.x & 31;
-    const float4 x = reinterpret_cast<const float4 *>(q)[lane];
-    const float c = scale * 1.4426950408889634f;
-    PackedRowSums r{-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-    for (uint32_t k0 = from; k0 < to; k0 += AT_ONCE) {
-        const int32_t page = packed_page(v, seq, k0);
-        if (page < 0) continue;
-        float s[AT_ONCE];
-        float4 y[AT_ONCE];
-#pragma unroll
-        for (uint32_t e = 0; e < AT_ONCE; ++e) {
-            const size_t at = (((size_t)page * BRASA_KV_PAGE + (k0 + e) % BRASA_KV_PAGE) * v.hkv + kh) * KvRow<KV>::BYTES;
-            y[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            s[e] = -INFINITY;
-            if (k0 + e < to) {
-                const float4 k = packed_row4<KV>(kpool + at, lane);
-                y[e] = packed_row4<KV>(vpool + at, lane);
-                s[e] = fmaf(x.w, k.w, fmaf(x.z, k.z, fmaf(x.y, k.y, x.x * k.x)));
-                for (int i = 16; i > 0; i >>= 1) s[e] += __shfl_xor_sync(0xffffffffu, s[e], i);
-                s[e] *= c;
-            }
-        }
-        float now = r.m;
-#pragma unroll
-        for (uint32_t e = 0; e < AT_ONCE; ++e) now = fmaxf(now, s[e]);
-        const float ref = now == -INFINITY ? 0.0f : now, f = r.m == -INFINITY ? 0.0f : exp2_approx(r.m - ref);
-        r.m = now;
-        r.l *= f;
-        r.o = make_float4(r.o.x * f, r.o.y * f, r.o.z * f, r.o.w * f);
-#pragma unroll
-        for (uint32_t e = 0; e < AT_ONCE; ++e) {
-            const float w = exp2_approx(s[e] - ref);
-            r.l += w;
-            r.o = make_float4(fmaf(w, y[e].x, r.o.x), fmaf(w, y[e].y, r.o.y), fmaf(w, y[e].z, r.o.z), fmaf(w, y[e].w, r.o.w));
-        }
-    }
-    return r;
-}
-
 // ---- the work of a run in a line, cut evenly ----
 // An item is up to item_tokens tokens of one sequence, each with the heads of a key head's group, against that key head. In the line an item takes `start`
 // units for its beginning and end and one per 2^tile_log2 keys that its last token sees. Equal pieces of the line go to the blocks; a block works
@@ -258,6 +204,131 @@ __device__ __forceinline__ bool line_next(const PackedLine &l, PackedItem &it) {
     }
     it.tiles = line_tiles(l, it);
     return true;
+}
+
+// ---- rows before a value that is not finite ----
+// A weight of zero times an infinity or NaN of V is NaN, so that in a matrix product a key behind a row's own position, new in the same run, reaches the row. A kernel
+// that finds a row not finite although keys of its share lie behind it comes here with all its threads, at a place where no other warp waits for them.
+// Dim by dim, V of the share's new positions says where the last value is that is not finite and where the first NaN: a row is taken again when it has a dim
+// that a value behind it spoiled and that no NaN at or before it makes NaN anyway. What the row's older positions hold is not looked at: a value there costs
+// this one look at up to 256 positions. An 8-bit value that the products round to an f16 infinity spoils like one.
+struct PackedAgain {
+    const float *q;
+    const uint8_t *kpool, *vpool;
+    void *o;
+    float *part;  // the share's slot, when it is not the whole of its item's keys
+    uint32_t hq;
+    float scale;
+    uint32_t seq, kh, t0, rows, past;  // of the item: its first row of the run, its rows, positions before its first token
+    uint32_t from, upto, rows_item;    // keys of the share; rows of a slot
+    bool whole;
+};
+struct PackedRowSums {
+    float m, l;
+    float4 o;
+};
+template <int KV>
+__device__ __forceinline__ float4 packed_row4(const uint8_t *row, uint32_t lane) {
+    const float2 a = tile_at2<KV>(row, 4 * lane), b = tile_at2<KV>(row, 4 * lane + 2);
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+// The sums of one row over the keys [from, to), a warp, four dims a lane: m, the sum of 2^(s - m) and that times V. Backwards, until nothing is left that is not NaN.
+template <int KV>
+__device__ __forceinline__ PackedRowSums packed_row_again(const PackedView &v, const uint8_t *kpool, const uint8_t *vpool, const float *q, float scale, uint32_t seq, uint32_t kh, uint32_t from, uint32_t to) {
+    constexpr uint32_t AT_ONCE = 8;  // (half a page)
+    const uint32_t lane = threadIdx.x & 31;
+    const float4 x = reinterpret_cast<const float4 *>(q)[lane];
+    const float c = scale * 1.4426950408889634f;
+    PackedRowSums r{-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    for (uint32_t n = to > from ? (to - from + AT_ONCE - 1) / AT_ONCE : 0; n > 0; --n) {  // (from is a multiple of 64)
+        const uint32_t k0 = from + (n - 1) * AT_ONCE;
+        const int32_t page = packed_page(v, seq, k0);
+        if (page < 0) continue;
+        float s[AT_ONCE];
+        float4 y[AT_ONCE];
+#pragma unroll
+        for (uint32_t e = 0; e < AT_ONCE; ++e) {
+            const size_t at = (((size_t)page * BRASA_KV_PAGE + (k0 + e) % BRASA_KV_PAGE) * v.hkv + kh) * KvRow<KV>::BYTES;
+            y[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            s[e] = -INFINITY;
+            if (k0 + e < to) {
+                const float4 k = packed_row4<KV>(kpool + at, lane);
+                y[e] = packed_row4<KV>(vpool + at, lane);
+                s[e] = fmaf(x.w, k.w, fmaf(x.z, k.z, fmaf(x.y, k.y, x.x * k.x)));
+                for (int i = 16; i > 0; i >>= 1) s[e] += __shfl_xor_sync(0xffffffffu, s[e], i);
+                s[e] *= c;
+            }
+        }
+        float now = r.m;
+#pragma unroll
+        for (uint32_t e = 0; e < AT_ONCE; ++e) now = fmaxf(now, s[e]);
+        const float ref = now == -INFINITY ? 0.0f : now, f = r.m == -INFINITY ? 0.0f : exp2_approx(r.m - ref);
+        r.m = now;
+        r.l *= f;
+        r.o = make_float4(r.o.x * f, r.o.y * f, r.o.z * f, r.o.w * f);
+#pragma unroll
+        for (uint32_t e = 0; e < AT_ONCE; ++e) {
+            const float w = exp2_approx(s[e] - ref);
+            r.l += w;
+            r.o = make_float4(fmaf(w, y[e].x, r.o.x), fmaf(w, y[e].y, r.o.y), fmaf(w, y[e].z, r.o.z), fmaf(w, y[e].w, r.o.w));
+        }
+        if (__all_sync(0xffffffffu, r.o.x != r.o.x && r.o.y != r.o.y && r.o.z != r.o.z && r.o.w != r.o.w)) break;
+    }
+    return r;
+}
+template <int KV, bool HALF>
+__device__ __noinline__ void packed_rows_again(const PackedLine &l, const PackedAgain &a) {
+    __shared__ uint32_t first_nan[128], past_bad[128];  // by dim: positions, the second one further on
+    constexpr float LIMIT = KV == BRASA_KV_Q8_0 && HALF ? 65520.0f : INFINITY;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    for (uint32_t i = threadIdx.x; i < 128; i += blockDim.x) {
+        first_nan[i] = UINT32_MAX;
+        past_bad[i] = 0;
+    }
+    __syncthreads();
+    for (uint32_t p = max(a.past, a.from) + warp; p < a.upto; p += warps) {
+        const int32_t page = packed_page(l.v, a.seq, p);
+        if (page < 0) continue;
+        const float4 y = packed_row4<KV>(a.vpool + (((size_t)page * BRASA_KV_PAGE + p % BRASA_KV_PAGE) * l.v.hkv + a.kh) * KvRow<KV>::BYTES, lane);
+        const float ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+            if (!(fabsf(ys[e]) < LIMIT)) {
+                atomicMax(&past_bad[4 * lane + e], p + 1);
+                if (ys[e] != ys[e]) atomicMin(&first_nan[4 * lane + e], p);
+            }
+    }
+    __syncthreads();
+    const uint4 nan = reinterpret_cast<const uint4 *>(first_nan)[lane], bad = reinterpret_cast<const uint4 *>(past_bad)[lane];
+    for (uint32_t r = warp; r < a.rows; r += warps) {
+        const uint32_t token = row_token(l, r), own = a.past + token;
+        const size_t at = ((size_t)(a.t0 + token) * a.hq + a.kh * l.group + r - token * l.group) * 128 + 4 * lane;
+        float4 y;
+        if (!a.whole) y = reinterpret_cast<const float4 *>(a.part + (size_t)r * 128)[lane];
+        else if (HALF) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(a.o) + at);
+            const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+            y = make_float4(lo.x, lo.y, hi.x, hi.y);
+        } else y = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.o) + at);
+        auto spoiled = [&](float v, uint32_t upto, uint32_t first) { return not_finite(v) && upto > own + 1 && first > own; };
+        if (!__any_sync(0xffffffffu, spoiled(y.x, bad.x, nan.x) || spoiled(y.y, bad.y, nan.y) || spoiled(y.z, bad.z, nan.z) || spoiled(y.w, bad.w, nan.w))) continue;
+        const PackedRowSums x = packed_row_again<KV>(l.v, a.kpool, a.vpool, a.q + at - 4 * lane, a.scale, a.seq, a.kh, a.from, min(a.upto, own + 1));
+        if (a.whole) {
+            const float inv = x.l == 0.0f ? 0.0f : 1.0f / x.l;
+            const float4 v = make_float4(x.o.x * inv, x.o.y * inv, x.o.z * inv, x.o.w * inv);
+            if (HALF) {
+                const __half2 lo = __floats2half2_rn(v.x, v.y), hi = __floats2half2_rn(v.z, v.w);
+                *reinterpret_cast<uint2 *>(static_cast<__half *>(a.o) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+            } else *reinterpret_cast<float4 *>(static_cast<float *>(a.o) + at) = v;
+        } else {
+            reinterpret_cast<float4 *>(a.part + (size_t)r * 128)[lane] = x.o;
+            if (lane == 0) {
+                a.part[(size_t)a.rows_item * 128 + r] = x.m;
+                a.part[(size_t)a.rows_item * 129 + r] = x.l;
+            }
+        }
+    }
+    __syncthreads();
 }
 
 }  // namespace brasa_dev

@@ -14,7 +14,7 @@
 // share before has its last step. The row tiles take turns with the exponentials: side by side, both would hold the unit up and then leave it idle.
 //
 // Cache rows behind the item's last position may hold anything: their scores are replaced before they count, and V's are written as zeros. A
-// row whose output is not finite although new tokens lie behind it is taken again without them (packed_row_again).
+// row whose output is not finite although new tokens lie behind it may be taken again without them, when the block's shares are done (packed_rows_again).
 // Rounded to fewer than 32 bits: q * scale and the weights to f16, as the product takes them (2^-11 each, what the F16 precision says), an 8-bit cache's values
 // likewise, the output to f16. l sums the rounded weights, so that their error largely cancels in O / l.
 //
@@ -98,15 +98,28 @@ __device__ __forceinline__ void add_halves(uint32_t pair, float &a, float &b) {
     asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tadd.rn.f32.f16 %0, x, %0;\n\tadd.rn.f32.f16 %1, y, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(pair));
 }
 
+// Rows before a value that is not finite: all warps walk the block's piece once more, now that none waits for another.
+template <bool Q8>
+__device__ __noinline__ void packed_tc_again(const PackedTcParams &p, PackedItem it, const PackedItem &end) {
+    for (bool more = true; more && (it.first < end.first || (it.first == end.first && it.j < end.j));) {
+        const uint32_t j1 = it.first == end.first ? end.j : it.tiles, token0 = it.part * p.l.item_tokens;
+        packed_rows_again<Q8 ? BRASA_KV_Q8_0 : BRASA_KV_F16, true>(
+            p.l, PackedAgain{p.q, p.kpool, p.vpool, p.o, p.part + (size_t)(2 * blockIdx.x + (it.j == 0)) * packed_part_floats(ROWS), p.hq, p.scale, it.seq, it.kh, it.t0 + token0,
+                             line_tokens(p.l, it) * p.l.group, it.past + token0, 128 * it.j, min(line_keys(p.l, it), 128 * j1), ROWS, it.j == 0 && j1 == it.tiles});
+        more = j1 == it.tiles && line_next(p.l, it);
+    }
+}
+
 template <bool Q8>
 __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_kernel(const __grid_constant__ PackedMaps maps, const __grid_constant__ PackedTcParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *ring = smem + 2 * TILE_BYTES;
     __shared__ uint64_t full[2][2], freed[2][2], q_full[2], s_ready[2][2], p_ready[2][2], pv_done[2], o_done[2], turn[2], share_full[SHARES], share_free[SHARES];
     __shared__ PackedShare shares[SHARES];
-    __shared__ uint32_t tmem_base_s, abort_s, there_s[8];  // (there: of the last key tiles, which of their eight pages are pages)
+    __shared__ uint32_t tmem_base_s, abort_s, again_s, there_s[8];  // (there: of the last key tiles, which of their eight pages are pages)
     __shared__ PackedPieces pieces;
     __shared__ PackedNote note;
+    __shared__ PackedItem begin;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.l.group, hkv = p.l.v.hkv;
 
     if (tid == 0) {
@@ -128,7 +141,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
             mbar_init(&share_full[i], 1);
             mbar_init(&share_free[i], 2 * (Q8 ? WARPS_Q8 : 1) - 1 + 2 + SOFTMAX_WARPS);  // by all warps but the one that walks
         }
-        abort_s = 0;
+        abort_s = again_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == MMA_WARP) {  // tensor memory: S of A, two steps, then P over them, in [0, 128), of B in [128, 256); O of A in [256, 384), of B in [384, 512)
@@ -174,6 +187,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
         bool more = false, ok = true;
         if (walks && lane == 0) {
             if (work && item.j == item.tiles) line_next(p.l, item);
+            begin = item;
             more = work && (item.first < end.first || (item.first == end.first && item.j < end.j));
             note = PackedNote{};
         }
@@ -309,7 +323,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
         const uint64_t q = tc_desc_kmajor(smem_u32(smem + x * TILE_BYTES));
         auto landed = [&](uint32_t is_v, uint32_t t) { return all_wait(&full[is_v][t & 1], (t >> 1) & 1); };
         auto slot = [&](uint32_t is_v, uint32_t t) { return smem_u32(ring + (size_t)(2 * is_v + (t & 1)) * TILE_BYTES); };
-        uint32_t loads = 0, segs = 0, used[2] = {0, 0};  // of the shares before: key tiles, shares with this row tile, uses of either step's columns
+        uint32_t loads = 0, segs = 0, used = 0;  // of the shares before: key tiles, shares with this row tile, uses of either step's columns
         bool ok = true;
 #pragma unroll 1
         for (uint32_t i = 0; ok; ++i) {
@@ -345,7 +359,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                 for (uint32_t k = 0; k < steps && ok; ++k) {
                     const uint32_t t = loads + (k >> 1), b = k & 1;
                     if (b == 0) ok = landed(1, t) && (k + 2 >= steps || landed(0, t + 1));
-                    ok = ok && all_wait(&p_ready[x][b], (used[b] + (k >> 1)) & 1);
+                    ok = ok && all_wait(&p_ready[x][b], ((used >> b & 1) + (k >> 1)) & 1);
                     if (!ok) break;
                     if (tc_elect_one()) {  // O += P V
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -359,8 +373,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                     __syncwarp();
                     if (k + 2 < steps) scores(k + 2);
                 }
-                used[0] += (steps + 1) / 2;
-                used[1] += steps / 2;
+                used ^= ((steps + 1) / 2 & 1) | (steps / 2 & 1) << 1;
                 ++segs;
             }
             loads += len;
@@ -375,7 +388,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
         constexpr float LOG2E = 1.4426950408889634f, SLACK = 5.545177444f;  // 8 ln 2
         const uint32_t x = warp >> 2, wrow = (warp & 3) * 32, row = wrow + lane;
         const uint32_t ts = tmem + 128 * x + (wrow << 16), to = tmem + 256 + 128 * x + (wrow << 16);
-        uint32_t used[2] = {0, 0}, all_steps = 0, segs = 0, tiles0 = 0;  // of the shares before: uses of either step's columns, steps and shares of this row tile; all key tiles
+        uint32_t used = 0, all_steps = 0, segs = 0, tiles0 = 0;  // of the shares before: uses of either step's columns, steps and shares of this row tile; all key tiles
         uint32_t turns = 0;                                              // steps so far with the other row tile beside
         // The warp's 32 rows of a share's q: fetched, and when `before` has waited for the last scores of the share before, scaled, rounded to f16 and stored
         // swizzled K-major over that one's (rows past the last are zeros).
@@ -416,7 +429,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
             if (rows == 0) break;
             const uint32_t seen_all = 128 * x + row < rows ? share.past + row_token(p.l, 128 * x + row) + 1 : 0;
             const uint32_t nfree = (share.past + row_token(p.l, 128 * x) + 1) / 64;  // steps [0, nfree) of all keys lie wholly at or below every row's own position
-            float m = -INFINITY, mneg = 0.0f, l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float m = -INFINITY, mneg = 0.0f, l[2] = {0.0f, 0.0f};
             if (rows <= 128 * x) {
                 ok = share_at(i + 1);
                 if (ok && next.rows > 128 * x) ok = bring_q(next, nothing);
@@ -424,7 +437,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
 #pragma unroll 1
                 for (uint32_t k = 0; k < steps; ++k) {
                     const uint32_t b = k & 1, at = 2 * j0 + k;
-                    auto scores = [&] { return all_wait(&s_ready[x][b], (used[b] + (k >> 1)) & 1); };  // S of this step, and with it every product issued before
+                    auto scores = [&] { return all_wait(&s_ready[x][b], ((used >> b & 1) + (k >> 1)) & 1); };  // S of this step, and with it every product issued before
                     if (k + 1 < steps) ok = scores();
                     else {  // (the next share's queries on the way)
                         ok = share_at(i + 1);
@@ -456,7 +469,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                         move = m != -INFINITY;
                         rescale = move ? exp2_approx((m - tmax) * LOG2E) : 1.0f;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) l[e] *= rescale;
+                        for (int e = 0; e < 2; ++e) l[e] *= rescale;
                         m = tmax;
                         mneg = -m * LOG2E;
                     }
@@ -491,7 +504,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                             w[e] = *reinterpret_cast<const uint32_t *>(&pp);
                         }
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) add_halves(w[e], l[2 * e & 3], l[(2 * e & 3) + 1]);
+                        for (int e = 0; e < 8; ++e) add_halves(w[e], l[0], l[1]);
                         tmem_st8(ts + 64 * b + 8 * c, w);
                     }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -499,15 +512,14 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                     __syncwarp();
                     if (lane == 0) tc_mbar_arrive(&p_ready[x][b]);
                 }
-                used[0] += (steps + 1) / 2;
-                used[1] += steps / 2;
+                used ^= ((steps + 1) / 2 & 1) | (steps / 2 & 1) << 1;
                 all_steps += steps;
                 // ---- output: O / l, rounded to f16, whole rows by way of shared memory; a part of the item's keys: O, m and l as they are ----
                 ok = ok && all_wait(&o_done[x], segs & 1);
                 ++segs;
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const float sum = (l[0] + l[1]) + (l[2] + l[3]);
+                const float sum = l[0] + l[1];
                 const uint32_t r = 128 * x + row;
                 const bool live = r < rows;
                 float zeros = 0.0f;  // 0 times every output: NaN when one is not finite
@@ -557,25 +569,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                     }
                 }
                 const uint32_t upto = min(share.nkeys, 128 * (j0 + share.len));
-                uint32_t again = __ballot_sync(0xffffffffu, live && zeros != 0.0f && seen_all < upto);
-#pragma unroll 1
-                for (__syncwarp(); again; again &= again - 1) {  // (see packed_row_again)
-                    const uint32_t re = 128 * x + wrow + __ffs(again) - 1, tk = row_token(p.l, re);
-                    const size_t at = ((size_t)(share.t0 + tk) * p.hq + share.kh * G + re - tk * G) * D;
-                    const PackedRowSums y = packed_row_again<Q8 ? BRASA_KV_Q8_0 : BRASA_KV_F16>(p.l.v, p.kpool, p.vpool, p.q + at, p.scale, share.seq, share.kh, 128 * j0, min(upto, share.past + tk + 1));
-                    if (share.whole) {
-                        const float f = y.l == 0.0f ? 0.0f : 1.0f / y.l;
-                        const __half2 a = __floats2half2_rn(y.o.x * f, y.o.y * f), b = __floats2half2_rn(y.o.z * f, y.o.w * f);
-                        reinterpret_cast<uint2 *>(p.o + at)[lane] = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
-                    } else {
-                        float *dst = p.part + (size_t)(2 * blockIdx.x + (j0 == 0)) * packed_part_floats(ROWS);
-                        reinterpret_cast<float4 *>(dst + (size_t)re * D)[lane] = y.o;
-                        if (lane == 0) {
-                            dst[ROWS * D + re] = y.m;
-                            dst[ROWS * D + ROWS + re] = y.l;
-                        }
-                    }
-                }
+                if (live && zeros != 0.0f && seen_all < upto) again_s = 1;  // (looked after when all shares are done)
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             }
             tiles0 += share.len;
@@ -589,6 +583,8 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
         const uint32_t ncols = 512;
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(ncols) : "memory");
     }
+    if (!again_s || abort_s) return;
+    packed_tc_again<Q8>(p, begin, pieces.at[1]);
 }
 
 }  // namespace

@@ -173,6 +173,88 @@ def test_attention_many_short_items_behind_a_bad_one(ctx, K, kv, bad):
     assert (got[tall:] == clean[tall:]).all()
 
 
+def put_row(run, pool, s, at, row):
+    """One position's row of all key heads, f32 [hkv, 128]; in 8 bits values that are not finite are codes of 1 under such a scale, others codes of 100."""
+    if run.kv == "q8_0":
+        block = row.reshape(run.hkv, 4, 32)[:, :, 0]
+        odd = ~np.isfinite(block)
+        raw = np.concatenate([np.repeat(np.where(odd, 1, 100), 32, -1).astype(np.uint8), np.where(odd, block, block / 100).astype(np.float16).view(np.uint8).reshape(run.hkv, 8)], -1)
+    else:
+        raw = R.to_bytes(row, run.kv)
+    pool[run.table[s, at // R.PAGE], at % R.PAGE] = raw
+
+
+@pytest.mark.parametrize("where", ["first", "every"])
+@pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("q8_0", False), ("f32", False)])
+def test_attention_a_bad_value_that_all_rows_see(ctx, K, kv, half, where):
+    """A NaN at the first position, or at every new one, makes the rows NaN that see it, and the call takes no longer for it than a call takes."""
+    run = R.Run([(500, 6000), (2, 50)], 8, 2, kv, seed=52)
+    seqs = run.seqs
+    run.seqs = [(0, 0), seqs[1]]
+    want, tol = run.attention(half)
+    run.seqs = seqs
+    row = np.full((2, R.D), np.nan, np.float32)
+    times = []
+    for bad in (False, True):
+        if bad:
+            for j in [0] if where == "first" else range(6000, 6500):
+                put_row(run, run.k, 0, j, row)
+                put_row(run, run.v, 0, j, row)
+        dev = OnDevice(ctx, K, run)
+        o = ctx.buffer(run.tokens * 8 * 128 * 4)
+        took = []
+        for _ in range(4):
+            cmd = ctx.command()
+            K.attention_packed(cmd, dev.q, dev.paged, dev.packed, o, 8, 2, 0 if half else 1)
+            took.append(cmd.wait())
+        times.append(min(took))
+        got = o.download(np.float16 if half else np.float32)[:run.tokens * 8 * 128].astype(np.float64).reshape(run.tokens, 8, 128)
+        o.free()
+        dev.free()
+    assert np.isnan(got[:500]).all()
+    check(got[500:], want[500:], tol[500:])
+    assert times[1] < 2 * times[0] + 2e-4, times
+
+
+@pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("q8_0", False), ("f32", False), ("f32", True)])
+def test_attention_bad_values_dim_by_dim(ctx, K, kv, half):
+    """NaN in 32 dims of one token, infinities in 32 other dims of a later one: of the rows between them only the first dims are NaN; a row before both has neither."""
+    run = R.Run([(150, 700), (6, 1500)], 4, 2, kv, seed=53)
+    want, tol = run.attention(half)
+    for s, (first, then) in enumerate(((40, 120), (2, 4))):
+        for j, dims, value in ((first, slice(0, 32), np.nan), (then, slice(64, 96), np.inf)):
+            at = int(run.lens[s]) + j
+            row = np.array(R.from_bytes(run.v[run.table[s, at // R.PAGE], at % R.PAGE], kv), np.float32)
+            row[:, dims] = value
+            if kv == "q8_0":  # (the other dims as they are)
+                raw = run.v[run.table[s, at // R.PAGE], at % R.PAGE]
+                raw[:, dims] = 1
+                raw[:, 128:].view(np.float16)[:, dims.start // 32] = value
+            else:
+                put_row(run, run.v, s, at, row)
+    got, _ = attend(ctx, K, run, half)
+    for s, (first, then) in enumerate(((40, 120), (2, 4))):
+        a, n = int(run.starts[s]), run.seqs[s][0]
+        check(got[a:a + first], want[a:a + first], tol[a:a + first])
+        assert np.isnan(got[a + first:a + n, :, :32]).all()
+        check(got[a + first:a + then, :, 32:], want[a + first:a + then, :, 32:], tol[a + first:a + then, :, 32:])
+        for d in (slice(32, 64), slice(96, 128)):
+            check(got[a + then:a + n, :, d], want[a + then:a + n, :, d], tol[a + then:a + n, :, d])
+        assert not np.isfinite(got[a + then:a + n, :, 64:96]).any()
+
+
+@pytest.mark.parametrize("shape", [[(6, 40)], [(60, 900)]])
+def test_attention_8_bit_values_past_f16(ctx, K, shape):
+    """A new token's value that is finite in 8 bits and infinite in f16, as the products of F16 precision round it, does not reach the rows before it."""
+    run = R.Run(shape, 8, 2, "q8_0", seed=54)
+    want, tol = run.attention(True)
+    n, past = shape[0]
+    at = past + n - 2
+    put_row(run, run.v, 0, at, np.full((2, R.D), 1e5, np.float32))
+    got, _ = attend(ctx, K, run, True)
+    check(got[:n - 2], want[:n - 2], tol[:n - 2])
+
+
 def test_attention_keeps_to_what_the_call_says(ctx, K):
     """`longest` and `tokens` below what starts say, starts that fall, positions behind the table: such rows are left alone."""
     run = R.Run([(3, 40), (150, 20), (2, 30)], 4, 2, "f16", seed=5)
