@@ -85,8 +85,10 @@ __global__ void __launch_bounds__(256) qk_norm_rope_store_packed_kernel(const fl
 // with one tile the warps share the keys (a page each), with two they go in pairs, with more every warp has a tile of its own. Each warp keeps a
 // running maximum, sum and output (the maximum moves only when a score passes it by 2^8), the warps meet at the item's end. The 16 keys of a
 // warp's step are one page: a page that is none is skipped, and rows of the cache that the sequence has not reached are never loaded.
-// HALF: one f16 term of q * scale and of P, 8-bit rows as f16(d * code): what the F16 precision says. Otherwise q and P enter as two terms, hi + lo
-// (2^-22 of the value), and an f16 cache's rows as they are. l sums the weights as the product reads them, by a column of ones beside V.
+// HALF: one f16 term of q * scale and of P, 8-bit rows as f16(d * code): what the F16 precision says. Otherwise q and P enter as two terms, hi + lo, and an f16
+// cache's rows as they are. f16 ends at 2^-25, so that both are brought up first, by powers of two: q to a row's largest of 2^14 to 2^15, the weights of a row's 16
+// keys to at most 2^15. Hi + lo is then off by 2^-22 of the value, or 2^-40 of the largest, whatever the other keys weigh; a step's product is added to O in 32 bits.
+// l sums the weights as the product reads them, by a column of ones beside V.
 // Bound by the cache's bytes while an item has one row tile or two, by mma.sync and its waits beyond that, where the tcgen05 kernel takes over (PACKED_TC_MIN_ROWS). 64
 // sequences of two to five tokens behind 2600 (32 heads on 8, f16) 153 us, 4.6 TB/s; 16 of three behind 3000 with an 8-bit cache 67 us against 68 with an f16
 // one: there the conversions bound it (5 instructions for two codes), 1.6 TB/s.
@@ -231,6 +233,7 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
         // ---- q fragments: k-step ks holds dims 16 ks + 2 tq, +1 and + 8 (8-bit rows: 32 (ks / 2) + 8 tq + 4 (ks % 2) .. + 3, so that a lane's codes lie together) ----
         uint32_t qh[8][4], ql[8][4];
         uint32_t seen[2];
+        float c[2] = {HALF ? LOG2E : p.scale * LOG2E, HALF ? LOG2E : p.scale * LOG2E};
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
             const uint32_t r = rt * 16 + g + 8 * h;
@@ -238,22 +241,34 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
             const uint32_t token = live ? row_token(p.l, r) : 0, head = live ? r - token * G : 0;
             seen[h] = live ? it.past + token0 + token + 1 : 0;
             const float *src = p.q + ((size_t)(t0 + token) * p.hq + it.kh * G + head) * D;
+            float2 a[8][2];
+            float top = 0.0f;
 #pragma unroll
             for (uint32_t ks = 0; ks < 8; ++ks) {
-                float2 a = make_float2(0.0f, 0.0f), b = a;
+                a[ks][0] = a[ks][1] = make_float2(0.0f, 0.0f);
                 const uint32_t d0 = Q8 ? 32 * (ks >> 1) + 8 * tq + 4 * (ks & 1) : 16 * ks + 2 * tq, d1 = Q8 ? d0 + 2 : d0 + 8;
                 if (live) {
-                    a = *reinterpret_cast<const float2 *>(src + d0);
-                    b = *reinterpret_cast<const float2 *>(src + d1);
+                    a[ks][0] = *reinterpret_cast<const float2 *>(src + d0);
+                    a[ks][1] = *reinterpret_cast<const float2 *>(src + d1);
                 }
-                const float f = HALF ? p.scale : 1.0f;
-                terms_h2<HALF>(a.x * f, a.y * f, qh[ks][h], ql[ks][h]);
-                terms_h2<HALF>(b.x * f, b.y * f, qh[ks][h + 2], ql[ks][h + 2]);
+                if (!HALF) top = fmaxf(fmaxf(top, fmaxf(fabsf(a[ks][0].x), fabsf(a[ks][0].y))), fmaxf(fabsf(a[ks][1].x), fabsf(a[ks][1].y)));
+            }
+            float f = p.scale;
+            if (!HALF) {  // the row's largest to [2^14, 2^15), as far as powers of two reach; an infinity stays one
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int at = (int)(__float_as_uint(top) >> 23), up = at == 255 ? 0 : min(14 - (at - 127), 100);
+                f = __uint_as_float((uint32_t)(127 + up) << 23);
+                c[h] *= __uint_as_float((uint32_t)(127 - up) << 23);
+            }
+#pragma unroll
+            for (uint32_t ks = 0; ks < 8; ++ks) {
+                terms_h2<HALF>(a[ks][0].x * f, a[ks][0].y * f, qh[ks][h], ql[ks][h]);
+                terms_h2<HALF>(a[ks][1].x * f, a[ks][1].y * f, qh[ks][h + 2], ql[ks][h + 2]);
             }
         }
         const uint32_t most = __reduce_max_sync(0xffffffffu, max(seen[0], seen[1]));  // keys that any row of the tile sees
-        const float c = HALF ? LOG2E : p.scale * LOG2E;
-        float m[2] = {-INFINITY, -INFINITY}, l[4] = {0.0f, 0.0f, 0.0f, 0.0f}, o[16][4];  // (l: a column of ones beside V, so that it sums the very P)
+        float m[2] = {-INFINITY, -INFINITY}, l[4] = {0.0f, 0.0f, 0.0f, 0.0f}, o[16][4];  // (l: a column of ones beside V, so that it sums the very P; two of the four are the same sums again)
 #pragma unroll
         for (int n = 0; n < 16; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
         for (uint32_t j = j0; j < j1; ++j) {
@@ -295,17 +310,17 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
                         }
                     }
                 }
-                // ---- P = 2^(s - m) ----
+                // ---- P = 2^(s - m), in two terms 2^(s - the step's largest + 15): O takes the step's product times what the two differ by ----
                 uint32_t ph[4], pl[4];
                 bool moved = false;
-                float back[2] = {1.0f, 1.0f};
+                float back[2] = {1.0f, 1.0f}, share_of[2] = {1.0f, 1.0f};
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {
                     float x[4], top = -INFINITY;
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) {
                         const uint32_t key = key0 + 8 * (e >> 1) + 2 * tq + (e & 1);
-                        x[e] = key < seen[h] ? s[e >> 1][2 * h + (e & 1)] * c : -INFINITY;
+                        x[e] = key < seen[h] ? s[e >> 1][2 * h + (e & 1)] * c[h] : -INFINITY;
                         top = fmaxf(top, x[e]);
                     }
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -315,7 +330,11 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
                         back[h] = m[h] == -INFINITY ? 0.0f : exp2_approx(m[h] - top);
                         m[h] = top;
                     }
-                    const float ref = m[h] == -INFINITY ? 0.0f : m[h];
+                    float ref = m[h] == -INFINITY ? 0.0f : m[h];
+                    if (!HALF) {
+                        share_of[h] = exp2_approx(top - ref - 15.0f);
+                        ref = top == -INFINITY ? 0.0f : top - 15.0f;
+                    }
                     float e[4];
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k) e[k] = exp2_approx(x[k] - ref);
@@ -335,17 +354,22 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
                 }
                 // ---- O += P V ----
                 const uint32_t vrow = 16 * u + (lane & 15), ones = 0x3C003C00u;
-                mma_f16(l, ph, ones, ones);
-                if (!HALF) mma_f16(l, pl, ones, ones);
+                auto add = [&](float to[4], uint32_t b0, uint32_t b1) {
+                    if (HALF) return mma_f16(to, ph, b0, b1);
+                    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma_f16(x, pl, b0, b1);
+                    mma_f16(x, ph, b0, b1);
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) to[k] = fmaf(x[k], share_of[k >> 1], to[k]);
+                };
+                add(l, ones, ones);
                 if (!Q8) {
 #pragma unroll
                     for (uint32_t n = 0; n < 16; n += 2) {
                         uint32_t b[4];
                         ldsm_x4_t(b, vt + vrow * 256 + (((n + (lane >> 4)) ^ (vrow & 7)) << 4));
-                        mma_f16(o[n], ph, b[0], b[1]);
-                        if (!HALF) mma_f16(o[n], pl, b[0], b[1]);
-                        mma_f16(o[n + 1], ph, b[2], b[3]);
-                        if (!HALF) mma_f16(o[n + 1], pl, b[2], b[3]);
+                        add(o[n], b[0], b[1]);
+                        add(o[n + 1], b[2], b[3]);
                     }
                 } else {  // (a transposed 16-bit read brings two dims of two keys: n-tile 2 x holds dims 16 x + 2 col, 2 x + 1 those + 1)
                     uint2 sc[4];  // scales of keys 2 tq, 2 tq + 1, and + 8

@@ -451,7 +451,8 @@ int32_t brasa_k_qk_norm_rope_store_packed(brasa_cmd *cmd, brasa_arg q, brasa_arg
                                           brasa_arg rope_sin, float eps, brasa_paged_kv paged, brasa_packed_run run, brasa_arg q_out, uint32_t hq, uint32_t hkv);
 /* Causal attention of the run's tokens: a token attends to the positions of its sequence up to its own, which the call before it has
  * stored. q f32 [tokens][hq][128]; precision F16: o f16 [tokens][hq][128], q * scale, the weights and an 8-bit cache's
- * values rounded to f16, sums in 32 bits; F32: o f32, 32-bit arithmetic. Cache rows that a sequence has not reached may hold anything, infinities and NaN included. A token
+ * values rounded to f16, sums in 32 bits; F32: o f32, 32-bit arithmetic, over an f16 cache with q and the
+ * weights as two f16 terms, scaled so that neither range nor size of either matters (2^-22 of the value, or 2^-40 of the largest of the row or of sixteen keys). Cache rows that a sequence has not reached may hold anything, infinities and NaN included. A token
  * that sees no position gives zeros. A token whose key or value is not finite counts for its own row and those behind it, never for one
  * before it. o and q must not overlap. max_pages up to 2^27 - 1. The first call of a context makes its workspace, so that it must not be one that is
  * recorded; lengths, tables and starts are read on the device, a recorded call follows what they hold by then. */

@@ -110,6 +110,52 @@ def test_attention_large_scores(ctx, K, kv, half):
     check(attend(ctx, K, run, half)[0], want, tol)
 
 
+@pytest.mark.parametrize("n", [6000, 32000])
+@pytest.mark.parametrize("kv", ["f16"])
+def test_attention_small_weights_count(ctx, K, kv, n):
+    """F32 precision: one key 18 nats above all others, whose weights are near 2^-26 each and a hundredth of a percent and more together. 300 sequences over the same
+    pages, so that a block has whole rows.
+    A weight is off by 2^-19 of itself at most (its exponential and the step's, terms of 2^-22, sums of sixteen); the sums in 32 bits round once for every 16 keys
+    and part, 2^-24 of what they hold: 2^-24 (n / 16 + 40) of sum p |v|."""
+    S, hq = 300, 4
+    run = R.Run([(1, n - 1)], hq, 1, kv, seed=61)
+    g = np.random.default_rng(62)
+    u = g.standard_normal(128)
+    u /= np.linalg.norm(u)
+    k, v = 0.05 * g.standard_normal((n, 1, 128)), 1.0 + 0.1 * g.standard_normal((n, 1, 128))
+    k[5, 0], v[5, 0] = 12.8 * u, -1.0
+    for pool, x in ((run.k, k), (run.v, v)):
+        rows = R.to_bytes(x.astype(np.float32), kv)
+        for i in range(n):
+            pool[run.table[0, i // R.PAGE], i % R.PAGE] = rows[i]
+    run.seqs, run.tokens = [(1, n - 1)] * S, S
+    run.table, run.lens, run.starts = np.repeat(run.table, S, 0), np.repeat(run.lens, S), np.arange(S + 1, dtype=np.uint32)
+    run.q = (16 * u + 0.3 * g.standard_normal((S, hq, 128))).astype(np.float32)
+    got, _ = attend(ctx, K, run, False)
+    kk, vv = (run.rows(pool, 0, n)[0][:, 0] for pool in (run.k, run.v))
+    for t in range(0, S, 13):
+        for h in range(hq):
+            q = run.q[t, h].astype(np.float64)
+            a = kk @ q / np.sqrt(128)
+            p = np.exp(a - a.max())
+            p /= p.sum()
+            o = p @ vv
+            ds = 2.0 ** -22 * 130 * (np.abs(kk) @ np.abs(q)).max() / np.sqrt(128)
+            check(got[t, h], o, ds * (p @ np.abs(vv - o)) + (2.0 ** -19 + 2.0 ** -24 * (n / 16 + 40)) * (p @ np.abs(vv)))
+
+
+@pytest.mark.parametrize("q,k", [(1e5, 1e-4), (1e-5, 1e4), (1e-30, 1.0), (1e30, 0.0)])
+@pytest.mark.parametrize("kv", ["f16", "q8_0", "f32"])
+def test_attention_queries_of_any_size(ctx, K, kv, q, k):
+    """F32 precision: queries beyond f16's range and in its last bits."""
+    run = R.Run([(5, 130), (1, 600), (40, 20)], 4, 2, kv, seed=63, scale=q)
+    real = ~np.isnan(R.from_bytes(run.k, kv)).any(-1, keepdims=True)
+    run.k = np.where(real, R.to_bytes(np.where(real, k * R.from_bytes(run.k, kv), 0).astype(np.float32), kv), run.k)
+    run.q[1, 2, 3:] *= 1e-7  # (a row whose values lie far apart)
+    want, tol = run.attention(False)
+    check(attend(ctx, K, run, False)[0], want, tol)
+
+
 @pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("f32", False)])
 def test_attention_positions_without_pages(ctx, K, kv, half):
     """Pages that are none stand for positions that hold nothing; a row that sees nothing gives zeros."""
