@@ -561,13 +561,14 @@ __global__ void __launch_bounds__(F32_THREADS, 1) attn_packed_f32_kernel(const _
                     for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffu << (tid & 16), top, x));
                     const float now = fmaxf(m[a], top), ref = now == -INFINITY ? 0.0f : now, f = m[a] == -INFINITY ? 0.0f : exp2_approx(m[a] - ref);
                     m[a] = now;
-                    l[a] *= f;
+                    float sum = 0.0f;
 #pragma unroll
                     for (uint32_t b = 0; b < 4; ++b) {
                         const float w = exp2_approx(s[a][b] - ref);
-                        l[a] += w;
+                        sum += w;
                         ps[(4 * ty + a) * F32_P + tx + 16 * b] = w;
                     }
+                    l[a] = fmaf(l[a], f, sum);
 #pragma unroll
                     for (uint32_t e = 0; e < 8; ++e) o[a][e] *= f;
                 }
@@ -577,6 +578,11 @@ __global__ void __launch_bounds__(F32_THREADS, 1) attn_packed_f32_kernel(const _
             asm volatile("cp.async.wait_group 1;" ::: "memory");
             __syncthreads();  // V is there
             if (live) {
+                float t[4][8];  // of this tile alone: one key that outweighs all others would swallow theirs one by one
+#pragma unroll
+                for (uint32_t a = 0; a < 4; ++a)
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) t[a][e] = 0.0f;
 #pragma unroll 2
                 for (uint32_t k = 0; k < 64; k += 4) {
                     float4 w[4];
@@ -588,17 +594,21 @@ __global__ void __launch_bounds__(F32_THREADS, 1) attn_packed_f32_kernel(const _
 #pragma unroll
                         for (uint32_t a = 0; a < 4; ++a) {
                             const float f = e == 0 ? w[a].x : (e == 1 ? w[a].y : (e == 2 ? w[a].z : w[a].w));
-                            o[a][0] = fmaf(f, y0.x, o[a][0]);
-                            o[a][1] = fmaf(f, y0.y, o[a][1]);
-                            o[a][2] = fmaf(f, y0.z, o[a][2]);
-                            o[a][3] = fmaf(f, y0.w, o[a][3]);
-                            o[a][4] = fmaf(f, y1.x, o[a][4]);
-                            o[a][5] = fmaf(f, y1.y, o[a][5]);
-                            o[a][6] = fmaf(f, y1.z, o[a][6]);
-                            o[a][7] = fmaf(f, y1.w, o[a][7]);
+                            t[a][0] = fmaf(f, y0.x, t[a][0]);
+                            t[a][1] = fmaf(f, y0.y, t[a][1]);
+                            t[a][2] = fmaf(f, y0.z, t[a][2]);
+                            t[a][3] = fmaf(f, y0.w, t[a][3]);
+                            t[a][4] = fmaf(f, y1.x, t[a][4]);
+                            t[a][5] = fmaf(f, y1.y, t[a][5]);
+                            t[a][6] = fmaf(f, y1.z, t[a][6]);
+                            t[a][7] = fmaf(f, y1.w, t[a][7]);
                         }
                     }
                 }
+#pragma unroll
+                for (uint32_t a = 0; a < 4; ++a)
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) o[a][e] += t[a][e];
             }
             __syncthreads();  // V and the weights are done with
         }

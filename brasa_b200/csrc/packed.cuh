@@ -264,14 +264,16 @@ __device__ __forceinline__ PackedRowSums packed_row_again(const PackedView &v, c
         for (uint32_t e = 0; e < AT_ONCE; ++e) now = fmaxf(now, s[e]);
         const float ref = now == -INFINITY ? 0.0f : now, f = r.m == -INFINITY ? 0.0f : exp2_approx(r.m - ref);
         r.m = now;
-        r.l *= f;
-        r.o = make_float4(r.o.x * f, r.o.y * f, r.o.z * f, r.o.w * f);
+        float l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (uint32_t e = 0; e < AT_ONCE; ++e) {
             const float w = exp2_approx(s[e] - ref);
-            r.l += w;
-            r.o = make_float4(fmaf(w, y[e].x, r.o.x), fmaf(w, y[e].y, r.o.y), fmaf(w, y[e].z, r.o.z), fmaf(w, y[e].w, r.o.w));
+            l += w;
+            o = make_float4(fmaf(w, y[e].x, o.x), fmaf(w, y[e].y, o.y), fmaf(w, y[e].z, o.z), fmaf(w, y[e].w, o.w));
         }
+        r.l = fmaf(r.l, f, l);
+        r.o = make_float4(fmaf(r.o.x, f, o.x), fmaf(r.o.y, f, o.y), fmaf(r.o.z, f, o.z), fmaf(r.o.w, f, o.w));
         if (__all_sync(0xffffffffu, r.o.x != r.o.x && r.o.y != r.o.y && r.o.z != r.o.z && r.o.w != r.o.w)) break;
     }
     return r;

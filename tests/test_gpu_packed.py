@@ -111,7 +111,7 @@ def test_attention_large_scores(ctx, K, kv, half):
 
 
 @pytest.mark.parametrize("n", [6000, 32000])
-@pytest.mark.parametrize("kv", ["f16"])
+@pytest.mark.parametrize("kv", ["f16", "q8_0", "f32"])
 def test_attention_small_weights_count(ctx, K, kv, n):
     """F32 precision: one key 18 nats above all others, whose weights are near 2^-26 each and a hundredth of a percent and more together. 300 sequences over the same
     pages, so that a block has whole rows.
