@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
                         back[h] = m[h] == -INFINITY ? 0.0f : exp2_approx(m[h] - top);
                         m[h] = top;
                     }
-                    float ref = m[h] == -INFINITY ? 0.0f : m[h];
+                    float ref = m[h] == -INFINITY ? 0.0f : m[h] - (HALF ? WEIGHT_LOG2 : 0.0f);
                     if (!HALF) {
                         share_of[h] = exp2_approx(top - ref - 15.0f);
                         ref = top == -INFINITY ? 0.0f : top - 15.0f;
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
             if (tq == 0) {
-                sums[warp][0][g + 8 * h] = m[h];
+                sums[warp][0][g + 8 * h] = m[h] - (HALF ? WEIGHT_LOG2 : 0.0f);
                 sums[warp][1][g + 8 * h] = l[2 * h];
             }
 #pragma unroll

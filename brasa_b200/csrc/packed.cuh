@@ -57,6 +57,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// F16 precision forms weights as 2^(s - m + 7): with scores up to m + 8 the largest is 2^15, near f16's end, so that 2^-25, where f16 loses its last bit, is 2^-32 of
+// the weight of a score of m. (O and l carry the factor alike; a part's m is given without it.)
+constexpr float WEIGHT_LOG2 = 7.0f;
 __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
 
 // ---- the work of a run in a line, cut evenly ----

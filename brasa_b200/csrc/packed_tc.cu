@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
 #pragma unroll
                         for (int e = 0; e < 2; ++e) l[e] *= rescale;
                         m = tmax;
-                        mneg = -m * LOG2E;
+                        mneg = fmaf(-m, LOG2E, WEIGHT_LOG2);
                     }
                     if (__any_sync(0xffffffffu, move)) {  // what O holds for the row was accumulated against the old reference; the last product must have ended
                         ok = all_wait(&pv_done[x], (all_steps + k - 1) & 1);
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(Q8 ? THREADS_Q8 : THREADS, 1) attn_packed_tc_k
                 if (!share.whole) {
                     float *dst = p.part + (size_t)(2 * blockIdx.x + (j0 == 0)) * packed_part_floats(ROWS);
                     if (live) {
-                        dst[ROWS * D + r] = m * LOG2E;
+                        dst[ROWS * D + r] = fmaf(m, LOG2E, -WEIGHT_LOG2);
                         dst[ROWS * D + ROWS + r] = sum;
                     }
 #pragma unroll 1

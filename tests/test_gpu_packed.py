@@ -144,6 +144,44 @@ def test_attention_small_weights_count(ctx, K, kv, n):
             check(got[t, h], o, ds * (p @ np.abs(vv - o)) + (2.0 ** -19 + 2.0 ** -24 * (n / 16 + 40)) * (p @ np.abs(vv)))
 
 
+@pytest.mark.parametrize("new", [1, 9])
+@pytest.mark.parametrize("kv", ["f16", "q8_0"])
+def test_attention_small_weights_count_in_f16(ctx, K, kv, new):
+    """F16 precision, the same: weights near 2^-26 of the largest are off by half of f16's last step, 2^-25, under a factor of 2^7 at least, so 2^-32 of the largest each.
+    Beside that what F16 precision rounds (see Run.attention), with half a step of o below 1, 2^-12."""
+    n, S, hq = 32000, 100, 4
+    run = R.Run([(new, n - new)], hq, 1, kv, seed=64)
+    g = np.random.default_rng(65)
+    u = g.standard_normal(128)
+    u /= np.linalg.norm(u)
+    k, v = 0.05 * g.standard_normal((n, 1, 128)), 0.95 + 0.04 * g.standard_normal((n, 1, 128))
+    k[5, 0], v[5, 0] = 12.8 * u, -0.95
+    for pool, x in ((run.k, k), (run.v, v)):
+        rows = R.to_bytes(x.astype(np.float32), kv)
+        for i in range(n):
+            pool[run.table[0, i // R.PAGE], i % R.PAGE] = rows[i]
+    run.seqs, run.tokens = [(new, n - new)] * S, S * new
+    run.table, run.lens, run.starts = np.repeat(run.table, S, 0), np.repeat(run.lens, S), np.arange(0, S * new + 1, new, dtype=np.uint32)
+    run.q = (16 * u + 0.3 * g.standard_normal((S * new, hq, 128))).astype(np.float32)
+    got, _ = attend(ctx, K, run, True)
+    kk, vv = (run.rows(pool, 0, n)[0][:, 0] for pool in (run.k, run.v))
+    for t in range(0, S * new, 29):
+        for h in range(hq):
+            see = n - new + t % new + 1
+            q = run.q[t, h].astype(np.float64)
+            a = kk[:see] @ q / np.sqrt(128)
+            p = np.exp(a - a.max())
+            p /= p.sum()
+            o = p @ vv[:see]
+            off = np.abs(vv[:see] - o)
+            spread = p @ off
+            dq = 6 * 2.0 ** -11 / np.sqrt(3) * np.sqrt((kk ** 2) @ (q ** 2)).max() / np.sqrt(128) * (np.sqrt(2) if kv == "q8_0" else 1)
+            tol = (dq + 2.0 ** -11) * spread + 2.0 ** -32 * off.sum(0) + 2.0 ** -12 + 2.0 ** -22 * (see / 16 + 200)
+            if kv == "q8_0":
+                tol = tol + 2.0 ** -12  # (the dominant value's own rounding, below 1)
+            check(got[t, h], o, tol)
+
+
 @pytest.mark.parametrize("q,k", [(1e5, 1e-4), (1e-5, 1e4), (1e-30, 1.0), (1e30, 0.0)])
 @pytest.mark.parametrize("kv", ["f16", "q8_0", "f32"])
 def test_attention_queries_of_any_size(ctx, K, kv, q, k):
