@@ -34,6 +34,8 @@ __device__ __forceinline__ uint32_t cluster_word(const uint32_t *local, uint32_t
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
     return v;
 }
+// an entry of p or q; what is no positive finite number counts as 0
+__device__ __forceinline__ float probability(float x) { return __float_as_uint(x) < 0x7F800000u ? x : 0.0f; }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -67,7 +69,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 1024 
         bool take = false;
         const uint32_t x = draft0 + i < a.ndrafts ? a.drafts[draft0 + i] : UINT32_MAX;
         if (x < a.vocab) {
-            const double px = a.p[(size_t)(first + i) * a.vocab + x], qx = a.q ? a.q[(draft0 + i) * a.vocab + x] : 1.0;
+            const double px = probability(a.p[(size_t)(first + i) * a.vocab + x]), qx = a.q ? probability(a.q[(draft0 + i) * a.vocab + x]) : 1.0f;
             take = (double)a.u[first + i] * qx < px;
         }
         if (!take) atomicMin(&stop_s, i);
@@ -86,14 +88,21 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 1024 
         if (vec && i + 4 <= a.vocab) return *reinterpret_cast<const float4 *>(row + i);
         return make_float4(i < a.vocab ? row[i] : 0.0f, i + 1 < a.vocab ? row[i + 1] : 0.0f, i + 2 < a.vocab ? row[i + 2] : 0.0f, i + 3 < a.vocab ? row[i + 3] : 0.0f);
     };
-    auto masses = [&](uint32_t i, const float4 &x, const float4 &y, double m[4]) {
-        m[0] = (double)x.x - (double)y.x;
-        m[1] = (double)x.y - (double)y.y;
-        m[2] = (double)x.z - (double)y.z;
-        m[3] = (double)x.w - (double)y.w;
+    auto masses = [&](uint32_t i, const float4 &x4, const float4 &y4, double m[4], uint32_t &held) {  // held: the last of the ids that has any
+        float x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
+        auto most = [](const float z[4]) { return max(max(__float_as_uint(z[0]), __float_as_uint(z[1])), max(__float_as_uint(z[2]), __float_as_uint(z[3]))); };
+        if (max(most(x), most(y)) >= 0x7F800000u || gone - i < 4)  // (rare: looked at together)
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k)
-            if (!(m[k] > 0.0 && m[k] < INFINITY) || i + k == gone) m[k] = 0.0;
+            for (uint32_t k = 0; k < 4; ++k) {
+                x[k] = gone - i != k ? probability(x[k]) : 0.0f;
+                y[k] = probability(y[k]);
+            }
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            x[k] = fmaxf(x[k], y[k]);
+            m[k] = (double)x[k] - (double)y[k];
+            if (x[k] > y[k]) held = i + k;
+        }
     };
     const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     double total = 0.0, start = 0.0;
@@ -106,10 +115,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 1024 
 #pragma unroll 4
             for (uint32_t i = piece_at(n) + 4 * lane; i < end_id; i += UNIT) {
                 double m[4];
-                masses(i, load4(p, i), q ? load4(q, i) : none, m);
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k)
-                    if (m[k] > 0.0) last = i + k;
+                masses(i, load4(p, i), q ? load4(q, i) : none, m, last);
                 sum += (m[0] + m[1]) + (m[2] + m[3]);
             }
             for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
@@ -153,7 +159,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 1024 
         for (uint32_t i0 = piece_at(n); i0 < end_id && id == UINT32_MAX; i0 += UNIT) {
             const uint32_t i = i0 + 4 * lane;
             double m[4];
-            masses(i, x, y, m);
+            masses(i, x, y, m, held);
             x = load4(p, i + UNIT);
             y = q ? load4(q, i + UNIT) : none;
             const double sum = (m[0] + m[1]) + (m[2] + m[3]);
@@ -167,7 +173,6 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 1024 
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
                 run += m[k];
-                if (m[k] > 0.0) held = i + k;
                 if (mine == UINT32_MAX && m[k] > 0.0 && run > point) mine = i + k;
             }
             id = __reduce_min_sync(0xffffffffu, mine);

@@ -521,6 +521,31 @@ def test_verify_odd_numbers(ctx, K):
     assert (got[0] == want[0]).all()
 
 
+@pytest.mark.parametrize("vocab", [40, 4099])
+@pytest.mark.parametrize("given", [True, False])
+def test_verify_entries_that_are_no_numbers_count_as_0(ctx, K, vocab, given):
+    """Infinities, NaN and negative numbers at drafts and elsewhere, in p and in q: the result is that of the same call with zeros in their places."""
+    g = np.random.default_rng(vocab)
+    odd = np.array([np.nan, np.inf, -np.inf, -0.25, -0.0], np.float32)
+    p, q, d, u, starts = random_verify(g, 150, 4, vocab, given)
+    at = 0
+    for s in range(150):
+        for i in range(int(starts[s]), int(starts[s + 1]) - 1):
+            if g.random() < 0.5:
+                p[i, d[at]] = g.choice(odd)
+            if given and g.random() < 0.5:
+                q[at, d[at]] = g.choice(odd)
+            at += 1
+    for x in (p, q) if given else (p,):
+        x[g.random(x.shape) < 0.1] = g.choice(odd)
+        x[:, ::7] = g.choice(odd, x[:, ::7].shape)
+    zeros = lambda x: None if x is None else np.where(np.isfinite(x) & (x > 0), x, 0).astype(np.float32)
+    got, _ = run_verify(ctx, K, p, q, d, u, starts)
+    same, want = run_verify(ctx, K, zeros(p), zeros(q), d, u, starts)
+    assert (same[0] == want[0]).all() and (same[1] == want[1]).all()
+    assert (got[0] == want[0]).all() and (got[1] == want[1]).all()
+
+
 def test_verify_draws_as_the_target_does(ctx, K):
     """First tokens of 20 000 verified drafts are distributed as p: each frequency within five standard deviations."""
     g = np.random.default_rng(4)
