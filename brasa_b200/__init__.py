@@ -595,10 +595,10 @@ class Kernels:
         """All layers' pages, the rows' tables and lengths, and the pages that others hold too (pinned, may be None)."""
         return _PagePool(_arg(kpool), _arg(vpool), _arg(table), _arg(lens), _arg(pinned), rows, max_pages, num_pages, layers, hkv, int(kv))
 
-    def pages_reassign(self, cmd, pool: _PagePool, source, keep, room, table_out, lens_out, result, accepted=None):
+    def pages_reassign(self, cmd, pool: _PagePool, source, keep, room, table_out, lens_out, result, accepted=None, starts=None):
         """Every row anew from `keep` positions of an old row (None: all, with those that `accepted` adds) and pages for `room` more: forks, reorders,
-        rolls back, frees, reserves."""
-        self._k(self.L.brasa_k_pages_reassign(cmd._h, pool, _arg(source), _arg(keep), _arg(accepted), _arg(room), _arg(table_out), _arg(lens_out), _arg(result)))
+        rolls back, frees, reserves. starts: the verified step's, so that rows without tokens in it stay as they are (None: all had some)."""
+        self._k(self.L.brasa_k_pages_reassign(cmd._h, pool, _arg(source), _arg(keep), _arg(accepted), _arg(starts), _arg(room), _arg(table_out), _arg(lens_out), _arg(result)))
 
     def pages_compact(self, cmd, pool: _PagePool, table_out, moved, result):
         """Moves the pages in use to the front of the pool."""

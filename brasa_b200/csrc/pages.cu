@@ -56,7 +56,7 @@ struct NewRow {
 struct ReassignArgs {
     PagePlan p;
     const int32_t *source;
-    const uint32_t *keep, *accepted, *room;
+    const uint32_t *keep, *accepted, *starts, *room;
     uint32_t *lens_out;
 };
 __device__ __forceinline__ NewRow new_row(const ReassignArgs &a, uint32_t r) {
@@ -66,7 +66,7 @@ __device__ __forceinline__ NewRow new_row(const ReassignArgs &a, uint32_t r) {
     const uint64_t most = (uint64_t)a.p.max_pages * PAGE;
     n.source = there ? (uint32_t)s : 0u;
     uint64_t holds = 0;
-    if (there) holds = (uint64_t)a.p.lens[s] + (a.accepted ? (uint64_t)a.accepted[s] + 1 : 0);
+    if (there) holds = (uint64_t)a.p.lens[s] + (a.accepted && (!a.starts || a.starts[s + 1] > a.starts[s]) ? (uint64_t)a.accepted[s] + 1 : 0);
     if (a.keep) holds = min(holds, (uint64_t)a.keep[r]);
     n.keep = (uint32_t)min(holds, most);
     n.have = (n.keep + PAGE - 1) / PAGE;
@@ -325,17 +325,18 @@ int32_t copy_pages(brasa_cmd *cmd, const brasa_page_pool &g, const PagePlan &p) 
 
 extern "C" {
 
-int32_t brasa_k_pages_reassign(brasa_cmd *cmd, brasa_page_pool g, brasa_arg source, brasa_arg keep, brasa_arg accepted, brasa_arg room, brasa_arg table_out,
-                               brasa_arg lens_out, brasa_arg result) {
+int32_t brasa_k_pages_reassign(brasa_cmd *cmd, brasa_page_pool g, brasa_arg source, brasa_arg keep, brasa_arg accepted, brasa_arg starts, brasa_arg room,
+                               brasa_arg table_out, brasa_arg lens_out, brasa_arg result) {
     if (!cmd) return BRASA_EINVAL;
     brasa_ctx *ctx = cmd->ctx;
     BRASA_TRY(check_pool(ctx, "pages_reassign", g));
     const uint64_t nt = (uint64_t)g.rows * g.max_pages * 4, nr = (uint64_t)g.rows * 4;
-    BRASA_REQUIRE(ctx, arg_fits(source, nr) && (!keep.buf || arg_fits(keep, nr)) && (!accepted.buf || arg_fits(accepted, nr)) && arg_fits(room, nr),
-                  "pages_reassign: source, keep, accepted or room too small");
+    BRASA_REQUIRE(ctx, arg_fits(source, nr) && (!keep.buf || arg_fits(keep, nr)) && (!accepted.buf || arg_fits(accepted, nr)) && (!starts.buf || arg_fits(starts, nr + 4)) && arg_fits(room, nr),
+                  "pages_reassign: source, keep, accepted, starts or room too small");
+    BRASA_REQUIRE(ctx, accepted.buf || !starts.buf, "pages_reassign: starts without accepted");
     BRASA_REQUIRE(ctx, arg_fits(table_out, nt) && arg_fits(lens_out, nr) && arg_fits(result, 16), "pages_reassign: table_out, lens_out or result too small");
-    for (const brasa_arg *a : {&source, &keep, &accepted, &room, &table_out, &lens_out, &result}) BRASA_REQUIRE(ctx, a->offset % 4 == 0, "pages_reassign: misaligned buffer");
-    const std::pair<const brasa_arg *, uint64_t> ins[] = {{&g.table, nt}, {&g.lens, nr}, {&source, nr}, {&keep, nr}, {&accepted, nr}, {&room, nr}, {&g.pinned, (uint64_t)g.num_pages * 4}},
+    for (const brasa_arg *a : {&source, &keep, &accepted, &starts, &room, &table_out, &lens_out, &result}) BRASA_REQUIRE(ctx, a->offset % 4 == 0, "pages_reassign: misaligned buffer");
+    const std::pair<const brasa_arg *, uint64_t> ins[] = {{&g.table, nt}, {&g.lens, nr}, {&source, nr}, {&keep, nr}, {&accepted, nr}, {&starts, nr + 4}, {&room, nr}, {&g.pinned, (uint64_t)g.num_pages * 4}},
                                                  outs[] = {{&table_out, nt}, {&lens_out, nr}, {&result, 16}};
     for (const auto &i : ins)
         for (const auto &o : outs) BRASA_REQUIRE(ctx, !arg_overlap(*i.first, i.second, *o.first, o.second), "pages_reassign: table_out, lens_out and result must not overlap what is read");
@@ -346,6 +347,7 @@ int32_t brasa_k_pages_reassign(brasa_cmd *cmd, brasa_page_pool g, brasa_arg sour
     a.source = (const int32_t *)arg_ptr(source);
     a.keep = (const uint32_t *)arg_ptr(keep);
     a.accepted = (const uint32_t *)arg_ptr(accepted);
+    a.starts = (const uint32_t *)arg_ptr(starts);
     a.room = (const uint32_t *)arg_ptr(room);
     a.lens_out = (uint32_t *)arg_ptr(lens_out);
     const uint32_t words = flag_words(g.num_pages);

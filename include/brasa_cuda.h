@@ -482,7 +482,9 @@ typedef struct brasa_page_pool {
 /* Every row anew: row r takes over the first positions of the old row source[r] (i32; outside the rows: nothing), keep[r] (u32; buf NULL:
  * all) of the lens[source[r]] that it holds, and gets pages for room[r] (u32) positions more, as far as max_pages reach. With accepted
  * (u32 [rows], buf NULL: none), as brasa_k_verify_drafts leaves it, an old row s holds accepted[s] + 1 positions more than lens[s]: the token
- * that the step began with and the drafts that stood. One call forks (several rows with one source), reorders,
+ * that the step began with and the drafts that stood. starts (u32 [rows + 1], buf NULL: every row was in the step) are the step's: a row without new
+ * tokens in it, paused or free, holds what lens says, for accepted[s] 0 alone does not tell it from one whose drafts were all refused. One call forks (several rows
+ * with one source), reorders,
  * rolls back, frees (source -1 or keep 0, room 0) and reserves. Whole pages that are kept are shared. The last page of a row, when it is not
  * full, becomes its own to write into: the first row that ends in it keeps it, unless it is pinned or held as a whole page too, the
  * others get copies of it in all layers. Pages that no new row holds are free at once; free ones are handed out from the lowest
@@ -490,8 +492,8 @@ typedef struct brasa_page_pool {
  * table_out i32 [rows][max_pages] and lens_out u32 [rows] must not overlap one another or what is read. result u32[4]: pages in use (pinned ones among them), pages
  * copied, pages free, pages missing; when pages are missing nothing is copied and table_out and lens_out are table and lens (entries
  * that name no page are -1). The first call with so many rows and pages makes the workspace of this and the next call: that one must not be recorded. */
-int32_t brasa_k_pages_reassign(brasa_cmd *cmd, brasa_page_pool pool, brasa_arg source, brasa_arg keep, brasa_arg accepted, brasa_arg room, brasa_arg table_out,
-                               brasa_arg lens_out, brasa_arg result);
+int32_t brasa_k_pages_reassign(brasa_cmd *cmd, brasa_page_pool pool, brasa_arg source, brasa_arg keep, brasa_arg accepted, brasa_arg starts, brasa_arg room,
+                               brasa_arg table_out, brasa_arg lens_out, brasa_arg result);
 /* Moves pages to the front of the pool: the highest page in use that is not pinned to the lowest free one, until none lies behind a free
  * one. In use is what the table names or pinned holds. table_out i32 [rows][max_pages] (which may be table) names the new places, moved
  * i32 [num_pages] where every page went (itself if it stayed, -1 if it was not in use). result u32[4]: pages in use, pages moved, one more

@@ -639,6 +639,38 @@ def test_reassign_pages_held_more_than_once(ctx, K):
     run_reassign(ctx, K, P, [0, 0, 2, 2, 3, 5], [40, 33, 20, 17, 20, 5], [0, 30, 1, 0, 5, 17])
 
 
+def test_steps_with_paused_and_free_rows(ctx, K):
+    """Verification and reassignment in turn, with rows that have no tokens in a step, among them free ones of length 0: those keep their length, the others gain what
+    stood. Every table against the host's."""
+    g = np.random.default_rng(71)
+    rows, V = 24, 90
+    P = Pages(g, rows, 12, 400, 2, 1, "f16", 0.2)
+    P.pinned[:] = 0
+    P.lens[3], P.table[3], P.lens[9], P.table[9] = 0, -1, 0, -1
+    tables, lens = [ctx.buffer_from(P.table), ctx.buffer(P.table.nbytes)], [ctx.buffer_from(P.lens), ctx.buffer(4 * rows)]
+    pools = [ctx.buffer_from(P.k), ctx.buffer_from(P.v)]
+    result, source = ctx.buffer(16), np.arange(rows)
+    acc, now = None, 0
+    for step in range(6):
+        p, q, d, u, starts = random_verify(g, rows, 4, V, True, 0.4)
+        starts_before = ctx.buffer_from(starts)
+        out, acc = ctx.buffer(4 * len(p)), ctx.buffer(4 * rows)
+        ins = [ctx.buffer_from(x) for x in (p, q, d, u)]
+        go(ctx, lambda c: K.verify_drafts(c, *ins, starts_before, rows, len(p), V, out, acc))
+        host = acc.download(np.uint32).astype(np.int64)
+        host[np.diff(starts) == 0] = -1  # (+ 1: no position more)
+        room = np.where(g.random(rows) < 0.3, 0, 5)
+        table, length, res, copies = R.reassign(P.table, P.lens, None, P.num_pages, source, None, room, host)
+        args = [ctx.buffer_from(x) for x in (source.astype(np.int32), room.astype(np.uint32))]
+        pool = K.page_pool(*pools, tables[now], lens[now], None, rows, 12, 400, 2, 1, 1)
+        go(ctx, lambda c: K.pages_reassign(c, pool, args[0], None, args[1], tables[1 - now], lens[1 - now], result, accepted=acc, starts=starts_before))
+        now = 1 - now
+        assert (lens[now].download(np.uint32) == length).all() and list(result.download(np.uint32)) == res
+        assert (tables[now].download(np.int32).reshape(table.shape) == table).all()
+        assert (length[np.diff(starts) == 0] == P.lens[np.diff(starts) == 0]).all()
+        P.table, P.lens = table, length
+
+
 @pytest.mark.parametrize("rows,max_pages,num_pages,layers,hkv,kv", [(1, 1, 1, 1, 1, "f16"), (4, 5, 40, 2, 2, "q8_0"), (33, 9, 1500, 1, 1, "f32"), (7, 40, 200, 3, 1, "f16"),
                                                                   (20, 300, 40000, 1, 1, "q8_0")])
 @pytest.mark.parametrize("in_place", [False, True])
@@ -818,6 +850,20 @@ def test_refusals_of_outputs_over_inputs(B, ctx, K):
             call(*args)
         assert e.value.code == B.EINVAL
     assert ctx.launch_count() == before
+
+
+def test_refusals_of_starts(B, ctx, K):
+    pool = ctx.buffer(2 * 8 * 16 * 256)
+    page = K.page_pool(pool, pool, ctx.buffer(48), ctx.buffer(16), None, 4, 3, 8, 2, 1, 1)
+    src, acc, room, out, starts, lens, res, small = (ctx.buffer(n) for n in (16, 16, 16, 48, 20, 16, 16, 16))
+
+    def rea(acc=acc, starts=starts, lens_out=lens):
+        go(ctx, lambda c: K.pages_reassign(c, page, src, None, room, out, lens_out, res, accepted=acc, starts=starts))
+    rea(), rea(starts=None)
+    for kw in (dict(starts=small), dict(starts=pool.at(2)), dict(acc=None), dict(lens_out=pool, starts=pool.at(12)), dict(starts=pool, lens_out=pool.at(16))):
+        with pytest.raises(B.BrasaError) as e:
+            rea(**kw)
+        assert e.value.code == B.EINVAL, kw
 
 
 def test_refusals(B, ctx, K):
