@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <utility>
@@ -189,6 +190,17 @@ static inline bool arg_fits(const brasa_arg &a, uint64_t n) {
 }
 static inline bool arg_overlap(const brasa_arg &a, uint64_t an, const brasa_arg &b, uint64_t bn) {
     return a.buf == b.buf && an && bn && a.offset < b.offset + bn && b.offset < a.offset + an;
+}
+// A range that an operator reads or writes; whether one of the first overlaps one of the second.
+struct brasa_range {
+    brasa_arg at;
+    uint64_t bytes;
+};
+static inline bool any_overlap(std::initializer_list<brasa_range> a, std::initializer_list<brasa_range> b) {
+    for (const brasa_range &x : a)
+        for (const brasa_range &y : b)
+            if (arg_overlap(x.at, x.bytes, y.at, y.bytes)) return true;
+    return false;
 }
 static inline bool qm_fits(const brasa_qmatrix &m) {
     return arg_fits(m.data, brasa_qtype_nbytes(m.qtype, (uint64_t)m.rows * m.cols));

@@ -762,8 +762,13 @@ int32_t brasa_k_qk_norm_rope_store_packed(brasa_cmd *cmd, brasa_arg q, brasa_arg
     for (const brasa_arg *a : {&q, &k, &v, &q_norm, &k_norm, &rope_cos, &rope_sin, &q_out})
         BRASA_REQUIRE(ctx, a->offset % 16 == 0, "qk_norm_rope_store_packed: misaligned buffer");
     // (in place every warp writes the rows that it has read)
-    BRASA_REQUIRE(ctx, ((q.buf == q_out.buf && q.offset == q_out.offset) || !arg_overlap(q, nq, q_out, nq)) && !arg_overlap(k, nkv, q_out, nq) && !arg_overlap(v, nkv, q_out, nq),
-                  "qk_norm_rope_store_packed: q_out must be q or overlap none of q, k and v");
+    const uint64_t pool = brasa_kv_bytes(pg.kv, (uint64_t)pg.num_pages * PAGE * hkv * 128), table = (uint64_t)pg.seqs * pg.max_pages * 4, seqs = (uint64_t)pg.seqs * 4;
+    const bool in_place = q.buf == q_out.buf && q.offset == q_out.offset;
+    const bool over = any_overlap({{q_out, nq}, {pg.kpool, pool}, {pg.vpool, pool}}, {{k, nkv}, {v, nkv}, {q_norm, 512}, {k_norm, 512}, {rope_cos, table_bytes},
+                                                                                     {rope_sin, table_bytes}, {run.starts, seqs + 4}, {pg.table, table}, {pg.lens, seqs}}) ||
+                      any_overlap({{q, nq}, {q_out, nq}}, {{pg.kpool, pool}, {pg.vpool, pool}}) || arg_overlap(pg.kpool, pool, pg.vpool, pool) ||
+                      (!in_place && arg_overlap(q, nq, q_out, nq));
+    BRASA_REQUIRE(ctx, !over, "qk_norm_rope_store_packed: q_out (unless it is q) and the pools must overlap neither one another nor what is read");
     const uint32_t per_tok = (hq + 2 * hkv + STORE_ROWS - 1) / STORE_ROWS;
     const uint64_t warps = (uint64_t)run.tokens * per_tok;
     BRASA_REQUIRE(ctx, warps <= 1ull << 33, "qk_norm_rope_store_packed: more than 2^35 rows");
@@ -790,7 +795,9 @@ int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv pg,
     const uint64_t n = (uint64_t)run.tokens * hq * D;
     BRASA_REQUIRE(ctx, arg_fits(q, n * 4) && arg_fits(o, n * (half ? 2 : 4)), "attention_packed: q or o too small");
     BRASA_REQUIRE(ctx, q.offset % 16 == 0 && o.offset % 16 == 0, "attention_packed: misaligned buffer");
-    BRASA_REQUIRE(ctx, !arg_overlap(q, n * 4, o, n * (half ? 2 : 4)), "attention_packed: o must not overlap q");
+    const uint64_t pool = brasa_kv_bytes(pg.kv, (uint64_t)pg.num_pages * PAGE * hkv * 128), seqs = (uint64_t)pg.seqs * 4;
+    const bool over = any_overlap({{o, n * (half ? 2 : 4)}}, {{q, n * 4}, {pg.kpool, pool}, {pg.vpool, pool}, {pg.table, seqs * pg.max_pages}, {pg.lens, seqs}, {run.starts, seqs + 4}});
+    BRASA_REQUIRE(ctx, !over, "attention_packed: o must not overlap what is read");
     BRASA_REQUIRE(ctx, (uint64_t)run.tokens * (hq / hkv) < 1ull << 31, "attention_packed: more than 2^31 rows of a key head's group");
     const float scale = 1.0f / sqrtf((float)D);
     // Sequences of many rows go to the tensor-core kernel where there is one (16-bit products) and the call can have any. What is neither an f16 cache nor 16-bit

@@ -302,6 +302,7 @@ int32_t check_pool(brasa_ctx *ctx, const char *who, const brasa_page_pool &g) {
     BRASA_REQUIRE(ctx, g.kpool.offset % 16 == 0 && g.vpool.offset % 16 == 0 && g.table.offset % 4 == 0 && g.lens.offset % 4 == 0 && g.pinned.offset % 4 == 0, "%s: misaligned", who);
     return BRASA_OK;
 }
+uint64_t pool_bytes(const brasa_page_pool &g) { return brasa_kv_bytes(g.kv, (uint64_t)PAGE * g.hkv * 128) * g.num_pages * g.layers; }  // (of K or V, behind check_pool)
 // The plan's arrays in the context's workspace.
 int32_t plan_of(brasa_ctx *ctx, const brasa_page_pool &g, brasa_arg table_out, brasa_arg result, PagePlan *p) {
     const size_t pairs = std::max(g.rows, g.num_pages), words = 2 * (size_t)g.num_pages + g.rows + 4 + 2 * pairs;
@@ -336,12 +337,11 @@ int32_t brasa_k_pages_reassign(brasa_cmd *cmd, brasa_page_pool g, brasa_arg sour
     BRASA_REQUIRE(ctx, accepted.buf || !starts.buf, "pages_reassign: starts without accepted");
     BRASA_REQUIRE(ctx, arg_fits(table_out, nt) && arg_fits(lens_out, nr) && arg_fits(result, 16), "pages_reassign: table_out, lens_out or result too small");
     for (const brasa_arg *a : {&source, &keep, &accepted, &starts, &room, &table_out, &lens_out, &result}) BRASA_REQUIRE(ctx, a->offset % 4 == 0, "pages_reassign: misaligned buffer");
-    const std::pair<const brasa_arg *, uint64_t> ins[] = {{&g.table, nt}, {&g.lens, nr}, {&source, nr}, {&keep, nr}, {&accepted, nr}, {&starts, nr + 4}, {&room, nr}, {&g.pinned, (uint64_t)g.num_pages * 4}},
-                                                 outs[] = {{&table_out, nt}, {&lens_out, nr}, {&result, 16}};
-    for (const auto &i : ins)
-        for (const auto &o : outs) BRASA_REQUIRE(ctx, !arg_overlap(*i.first, i.second, *o.first, o.second), "pages_reassign: table_out, lens_out and result must not overlap what is read");
-    BRASA_REQUIRE(ctx, !arg_overlap(table_out, nt, lens_out, nr) && !arg_overlap(table_out, nt, result, 16) && !arg_overlap(lens_out, nr, result, 16),
-                  "pages_reassign: table_out, lens_out and result must not overlap");
+    const uint64_t np = (uint64_t)g.num_pages * 4, pool = pool_bytes(g);
+    const brasa_range table{table_out, nt}, lens{lens_out, nr}, counts{result, 16}, k{g.kpool, pool}, v{g.vpool, pool};
+    const bool over = any_overlap({table, lens, counts, k, v}, {{g.table, nt}, {g.lens, nr}, {source, nr}, {keep, nr}, {accepted, nr}, {starts, nr + 4}, {room, nr}, {g.pinned, np}}) ||
+                      any_overlap({table, lens, counts}, {k, v}) || any_overlap({table}, {lens, counts}) || any_overlap({lens}, {counts});
+    BRASA_REQUIRE(ctx, !over, "pages_reassign: table_out, lens_out, result and the pools must overlap neither one another nor what is read");
     ReassignArgs a;
     BRASA_TRY(plan_of(ctx, g, table_out, result, &a.p));
     a.source = (const int32_t *)arg_ptr(source);
@@ -365,10 +365,11 @@ int32_t brasa_k_pages_compact(brasa_cmd *cmd, brasa_page_pool g, brasa_arg table
     BRASA_REQUIRE(ctx, arg_fits(table_out, nt) && arg_fits(moved, np) && arg_fits(result, 16), "pages_compact: table_out, moved or result too small");
     for (const brasa_arg *a : {&table_out, &moved, &result}) BRASA_REQUIRE(ctx, a->offset % 4 == 0, "pages_compact: misaligned buffer");
     const bool in_place = table_out.buf == g.table.buf && table_out.offset == g.table.offset;
-    BRASA_REQUIRE(ctx, (in_place || !arg_overlap(table_out, nt, g.table, nt)) && !arg_overlap(moved, np, g.table, nt) && !arg_overlap(moved, np, g.pinned, np) &&
-                  !arg_overlap(result, 16, g.table, nt) && !arg_overlap(result, 16, g.pinned, np) && !arg_overlap(table_out, nt, g.pinned, np) && !arg_overlap(table_out, nt, moved, np) &&
-                  !arg_overlap(result, 16, table_out, nt) && !arg_overlap(result, 16, moved, np),
-                  "pages_compact: outputs overlap one another or what is read");
+    const uint64_t pool = pool_bytes(g);
+    const brasa_range table{table_out, nt}, where{moved, np}, counts{result, 16}, k{g.kpool, pool}, v{g.vpool, pool};
+    const bool over = (!in_place && arg_overlap(table_out, nt, g.table, nt)) || any_overlap({where, counts, k, v}, {{g.table, nt}, {g.pinned, np}}) ||
+                      any_overlap({table}, {{g.pinned, np}, where, counts, k, v}) || any_overlap({where, counts}, {k, v}) || any_overlap({where}, {counts});
+    BRASA_REQUIRE(ctx, !over, "pages_compact: outputs and the pools overlap one another or what is read");
     PagePlan p;
     BRASA_TRY(plan_of(ctx, g, table_out, result, &p));
     const uint32_t words = flag_words(g.num_pages);

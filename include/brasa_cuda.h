@@ -444,7 +444,7 @@ typedef struct brasa_packed_run {
     uint32_t tokens;  /* rows of the buffers, at least starts[seqs] */
     uint32_t longest; /* the most tokens one sequence has in this run */
 } brasa_packed_run;
-/* brasa_k_qk_norm_rope_store_paged for such a run: q f32 [tokens][hq][128] is normalised and rotated into q_out (q itself or apart from q, k and v), k and
+/* brasa_k_qk_norm_rope_store_paged for such a run: q f32 [tokens][hq][128] is normalised and rotated into q_out (q itself, or apart from all that the call reads), k and
  * v f32 [tokens][hkv][128] are read: normalised and rotated k, and v, are rounded to the cache type and stored into the pages. No two
  * tokens may share a place of the pool. Tables as for the paged call: every position that max_pages pages reach. */
 int32_t brasa_k_qk_norm_rope_store_packed(brasa_cmd *cmd, brasa_arg q, brasa_arg k, brasa_arg v, brasa_arg q_norm, brasa_arg k_norm, brasa_arg rope_cos,
@@ -454,7 +454,7 @@ int32_t brasa_k_qk_norm_rope_store_packed(brasa_cmd *cmd, brasa_arg q, brasa_arg
  * values rounded to f16, sums in 32 bits; F32: o f32, 32-bit arithmetic, over an f16 cache with q and the
  * weights as two f16 terms, scaled so that neither range nor size of either matters (2^-22 of the value, or 2^-40 of the largest of the row or of sixteen keys). Cache rows that a sequence has not reached may hold anything, infinities and NaN included. A token
  * that sees no position gives zeros. A token whose key or value is not finite counts for its own row and those behind it, never for one
- * before it. o and q must not overlap. max_pages up to 2^27 - 1. The first call of a context makes its workspace, so that it must not be one that is
+ * before it. o must not overlap what is read. max_pages up to 2^27 - 1. The first call of a context makes its workspace, so that it must not be one that is
  * recorded; lengths, tables and starts are read on the device, a recorded call follows what they hold by then. */
 int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv paged, brasa_packed_run run, brasa_arg o, uint32_t hq, uint32_t hkv, int32_t precision);
 /* Verification of drafted tokens. Sequence s has rows starts[s] .. starts[s + 1] - 1 (u32 [seqs + 1], not falling, at most `rows`) of p
@@ -489,7 +489,7 @@ typedef struct brasa_page_pool {
  * full, becomes its own to write into: the first row that ends in it keeps it, unless it is pinned or held as a whole page too, the
  * others get copies of it in all layers. Pages that no new row holds are free at once; free ones are handed out from the lowest
  * on, to the rows in order (a copy's page ahead of those for new positions). Table entries that name no page are kept as -1.
- * table_out i32 [rows][max_pages] and lens_out u32 [rows] must not overlap one another or what is read. result u32[4]: pages in use (pinned ones among them), pages
+ * table_out i32 [rows][max_pages] and lens_out u32 [rows] must not overlap one another, what is read or the pools. result u32[4]: pages in use (pinned ones among them), pages
  * copied, pages free, pages missing; when pages are missing nothing is copied and table_out and lens_out are table and lens (entries
  * that name no page are -1). The first call with so many rows and pages makes the workspace of this and the next call: that one must not be recorded. */
 int32_t brasa_k_pages_reassign(brasa_cmd *cmd, brasa_page_pool pool, brasa_arg source, brasa_arg keep, brasa_arg accepted, brasa_arg starts, brasa_arg room,

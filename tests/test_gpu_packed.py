@@ -540,7 +540,8 @@ def test_verify_entries_that_are_no_numbers_count_as_0(ctx, K, vocab, given):
         x[g.random(x.shape) < 0.1] = g.choice(odd)
         x[:, ::7] = g.choice(odd, x[:, ::7].shape)
     zeros = lambda x: None if x is None else np.where(np.isfinite(x) & (x > 0), x, 0).astype(np.float32)
-    got, _ = run_verify(ctx, K, p, q, d, u, starts)
+    with np.errstate(invalid="ignore"):
+        got, _ = run_verify(ctx, K, p, q, d, u, starts)
     same, want = run_verify(ctx, K, zeros(p), zeros(q), d, u, starts)
     assert (same[0] == want[0]).all() and (same[1] == want[1]).all()
     assert (got[0] == want[0]).all() and (got[1] == want[1]).all()
@@ -849,6 +850,50 @@ def test_refusals_of_outputs_over_inputs(B, ctx, K):
         with pytest.raises(B.BrasaError, match="overlap") as e:
             call(*args)
         assert e.value.code == B.EINVAL
+    assert ctx.launch_count() == before
+
+
+def test_refusals_of_outputs_over_pools_and_tables(B, ctx, K):
+    """Outputs over the pools, tables, norms and lengths that the same launch reads, and pools over what is read or over one another."""
+    run = R.Run([(2, 20)], 4, 2, "f16")
+    T, pages = run.tokens, run.num_pages
+    size = pages * 16 * 2 * 256
+    big = ctx.buffer(4 * size)
+    n_rope = run.max_pages * 16 * 64 * 4
+
+    class Rope:
+        cos, sin = ctx.buffer(n_rope), ctx.buffer(n_rope)
+    f = {x: ctx.buffer(4096) for x in ("q", "k", "v", "o", "qn", "kn", "table", "lens", "starts")}
+    f["starts"].upload(run.starts), f["table"].upload(run.table), f["lens"].upload(run.lens)
+
+    def calls(kpool=big, vpool=big.at(size), out=None, **over):
+        x = {**f, **over}
+        paged, packed = K.paged_kv(kpool, vpool, x["table"], x["lens"], 1, run.max_pages, pages, 1), K.packed_run(x["starts"], T, 2)
+        return (lambda c: K.qk_norm_rope_store_packed(c, x["q"], x["k"], x["v"], x["qn"], x["kn"], EPS, Rope, paged, packed, out or x["o"], 4, 2),
+                lambda c: K.attention_packed(c, x["q"], paged, packed, out or x["o"], 4, 2, 1))
+    for call in calls():
+        go(ctx, call)
+    both = [dict(out=big.at(size - 16)), dict(out=big.at(2 * size - 512)), dict(out=f["table"]), dict(out=f["lens"]), dict(out=f["starts"])]
+    store = [dict(out=f["qn"]), dict(out=f["kn"]), dict(out=Rope.cos), dict(out=Rope.sin.at(n_rope - 4096)), dict(vpool=big.at(16)), dict(vpool=big), dict(q=big), dict(k=big.at(size)), dict(v=big.at(2 * size - 2048)),
+             dict(qn=big.at(64)), dict(table=big), dict(lens=big.at(size)), dict(starts=big.at(8)), dict(q=big.at(2 * size - 16), out=big.at(2 * size - 16))]
+    pool = ctx.buffer(8 * 16 * 256)
+    small = {x: ctx.buffer(256) for x in ("table", "lens", "pinned", "src", "keep", "acc", "st", "room", "out", "lens_out", "res", "moved")}
+
+    def page_calls(**over):
+        x = {**small, **over}
+        g = K.page_pool(pool, pool, x["table"], x["lens"], x["pinned"], 4, 3, 8, 1, 1, 1)
+        return (lambda c: K.pages_reassign(c, g, x["src"], x["keep"], x["room"], x["out"], x["lens_out"], x["res"], accepted=x["acc"], starts=x["st"]),
+                lambda c: K.pages_compact(c, g, x["out"], x["moved"], x["res"]))
+    for call in page_calls():
+        go(ctx, call)
+    before = ctx.launch_count()
+    bad = [x for kw in both for x in calls(**kw)] + [calls(**kw)[0] for kw in store]
+    bad += [page_calls(**{x: pool})[0] for x in ("table", "lens", "pinned", "src", "keep", "acc", "st", "room", "out", "lens_out", "res")]
+    bad += [page_calls(**{x: pool.at(8 * 16 * 256 - 64)})[1] for x in ("table", "pinned", "out", "res", "moved")]
+    for i, call in enumerate(bad):
+        with pytest.raises(B.BrasaError) as e:
+            go(ctx, call)
+        assert e.value.code == B.EINVAL and "overlap" in str(e.value), i
     assert ctx.launch_count() == before
 
 
