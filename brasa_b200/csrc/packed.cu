@@ -13,7 +13,7 @@ constexpr int D = 128;
 // y = x / sqrt(mean x^2 + eps) * w of rows of q and k, rotated by the token's own position (pairs i, i + 64), and the store of k and v. Bound by memory: q read
 // and written, k and v read, the cache's rows written. A warp takes four rows of a token (a lane four dims of each, so that a row is one
 // request and a pair's other half lies sixteen lanes on), asks for all of them first and finds the token's sequence, position and page meanwhile. 9 prompts of
-// 7257 tokens (32 heads on 8, f16) 70 us, 4.7 TB/s (one row a warp: 92 us).
+// 7257 tokens (32 heads on 8, f16) 71 us, 4.6 TB/s (one row a warp: 92 us).
 constexpr uint32_t STORE_ROWS = 4;
 
 // four dims a lane of one row, rounded to the cache type
@@ -90,8 +90,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_store_packed_kernel(const fl
 // keys to at most 2^15. Hi + lo is then off by 2^-22 of the value, or 2^-40 of the largest, whatever the other keys weigh; a step's product is added to O in 32 bits.
 // l sums the weights as the product reads them, by a column of ones beside V.
 // Bound by the cache's bytes while an item has one row tile or two, by mma.sync and its waits beyond that, where the tcgen05 kernel takes over (PACKED_TC_MIN_ROWS). 64
-// sequences of two to five tokens behind 2600 (32 heads on 8, f16) 153 us, 4.6 TB/s; 16 of three behind 3000 with an 8-bit cache 67 us against 68 with an f16
-// one: there the conversions bound it (5 instructions for two codes), 1.6 TB/s.
+// sequences of two to five tokens behind 2600 (32 heads on 8, f16) 154 us, 4.6 TB/s, in F32 precision 204 us; behind a flush of the L2, 16 of three behind 3000 take 61 us with
+// an 8-bit cache and 63 with an f16 one: there no unit is full (DRAM 33 %, issue slots 43 %), a page's chain of reads, conversions and products is what is waited for.
 struct FewParams {
     PackedLine l;
     const float *q;
@@ -456,7 +456,8 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
 // ---- 32-bit arithmetic: an f32 cache, or an 8-bit one whose values keep all their bits -------------------------------------------------------------
 // A block has up to 64 rows and takes 64 keys at a time as f32 in shared memory, K's next tile on its way while V's is used. 256 threads in a square: scores four
 // rows by four keys each (keys 16 apart, so that a quarter warp's reads of K meet in no bank), outputs four rows by eight dims. Bound by the FMA units
-// with many rows, by the cache's bytes with few: 2100 prompt tokens (8 heads on 2) 30 TFLOP/s, two to five tokens a sequence 1.5 TB/s.
+// with many rows, by the cache's bytes with few: 2100 prompt tokens (8 heads on 2) 331 us, 27 TFLOP/s, 64 sequences of two to five tokens behind 2600 (32 on 8) 826 us, 1.7 TB/s
+// (each behind a flush of the L2).
 constexpr uint32_t F32_THREADS = 256, F32_P = 68;
 constexpr size_t F32_SMEM = (3 * 64 * (size_t)FEW_TS + 64 * F32_P) * sizeof(float);
 

@@ -9,7 +9,7 @@
 // Roles: warps 0-7 the softmax, a thread to a row, a row tile to four warps; warps 8 and 9 issue a row tile's products each, so that neither waits
 // for the other's weights; then the copies. f16: a warp each for K and V, since a warp issues a TMA copy (16 positions x 64 dims, half a page) every 80 cycles,
 // sixteen to a tile of 128 keys. 8 bit: three warps each read codes and scales, turn them into f16(d * code) and store them swizzled; a tile's codes are asked for
-// when the tile before is stored, behind the fence, which would wait for them (two warps each: 493 instead of 444 us at the 8-bit figure below). Tiles go
+// when the tile before is stored, behind the fence, which would wait for them (two warps each, at the 8-bit figure below: 493 us when three took 444). Tiles go
 // through two slots for K and two for V. The copying warp of K walks the line and hands each share on; a share's queries are fetched while the
 // share before has its last step. The row tiles take turns with the exponentials: side by side, both would hold the unit up and then leave it idle.
 //
@@ -19,9 +19,9 @@
 // likewise, the output to f16. l sums the rounded weights, so that their error largely cancels in O / l.
 //
 // Bound by the round of a step, not by one unit: a row tile's scores, exponentials (16 a clock and SM, 1024 cycles for both row tiles' 64 keys), the weights' way
-// into tensor memory and their product follow one another, with two row tiles and two steps in flight; on the prompts below the tensor core works 40 % of the
-// time and the exponential unit 41 %. Measured: 1000 new tokens behind 9000 (64 heads on 8 key heads) 360 us, 865 TFLOP/s, with an 8-bit cache 459 us, 679 TFLOP/s (the
-// conversions take issue slots and registers from the softmax); 14 prompts of 16 138 tokens (32 on 8) 577 us, 642 TFLOP/s.
+// into tensor memory and their product follow one another, with two row tiles and two steps in flight; with 1024 tokens behind 5000 the tensor core works 39 % of the
+// time and the exponential unit 40 %. Measured: 1000 new tokens behind 9000 (64 heads on 8 key heads, behind a flush of the L2) 357 us, 871 TFLOP/s, with an 8-bit cache 445 us,
+// 699 TFLOP/s (the conversions take issue slots and registers from the softmax); 14 prompts of 16 138 tokens (32 on 8) 569 us, 651 TFLOP/s.
 #include <math.h>
 #include <string.h>
 

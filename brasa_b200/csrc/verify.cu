@@ -5,7 +5,8 @@
 // One row of p (and of q) per sequence is all that has to be read: 2 x 0.6 MB for a vocabulary of 151 936, so a cluster of eight blocks
 // takes a sequence, each with an eighth of the ids. Masses and their sums are 64-bit: p - q of two f32 numbers is exact up to the last
 // bits, and where the running sum passes the drawn point is decided far below the smallest mass. The sums' order depends on the vocabulary alone.
-// 64 sequences of 151 936 ids with q 23 us (3.4 TB/s), bound by two passes of a cluster whose second waits for the first; one sequence without q 9.3 us, latency.
+// 64 sequences of 151 936 ids with q 23.5 us among calls that leave the 78 MB in the L2, 32 us behind a flush (2.5 TB/s): two passes of a cluster whose second waits for the first;
+// one sequence without q 9 us and 18 us, latency.
 #include "brasa_internal.h"
 
 namespace {
@@ -226,7 +227,7 @@ extern "C" int32_t brasa_k_verify_drafts(brasa_cmd *cmd, brasa_arg p, brasa_arg 
                    (uint32_t *)arg_ptr(tokens), (uint32_t *)arg_ptr(accepted), seqs, rows, vocab, drafts.buf ? (drafts.buf->bytes - drafts.offset) / 4 : 0};
     if (q.buf) a.ndrafts = std::min(a.ndrafts, (q.buf->bytes - q.offset) / 4 / vocab);
     // 16 warps a block while all blocks are resident at once (clusters of eight fill 128 of the SMs, two blocks to each), eight warps where there are more sequences. 151 936 ids
-    // with q, 16 | 8 warps: 1 sequence 23.4 | 28.9 us, 32 sequences 27.7 | 34.4, 34 sequences 37.6 | 34.1, 64 sequences 42 | 35 (each behind a flush of the L2).
+    // with q, 16 | 8 warps: 1 sequence 18.4 | 23.6 us, 32 sequences 22.6 | 28.7, 34 sequences 32.8 | 28.7, 64 sequences 38.9 | 31.7 (each behind a flush of the L2).
     const bool wide = seqs <= 32;
     BRASA_CUDA(ctx, brasa_launch_dependent(ctx, wide ? verify_drafts_kernel<512> : verify_drafts_kernel<256>, dim3(seqs * CLUSTER), dim3(wide ? 512 : 256), 0, a));
     return brasa_post_launch(cmd, "verify_drafts");

@@ -451,11 +451,13 @@ int32_t brasa_k_qk_norm_rope_store_packed(brasa_cmd *cmd, brasa_arg q, brasa_arg
                                           brasa_arg rope_sin, float eps, brasa_paged_kv paged, brasa_packed_run run, brasa_arg q_out, uint32_t hq, uint32_t hkv);
 /* Causal attention of the run's tokens: a token attends to the positions of its sequence up to its own, which the call before it has
  * stored. q f32 [tokens][hq][128]; precision F16: o f16 [tokens][hq][128], q * scale, the weights and an 8-bit cache's
- * values rounded to f16, sums in 32 bits; F32: o f32, 32-bit arithmetic, over an f16 cache with q and the
- * weights as two f16 terms, scaled so that neither range nor size of either matters (2^-22 of the value, or 2^-40 of the largest of the row or of sixteen keys). Cache rows that a sequence has not reached may hold anything, infinities and NaN included. A token
- * that sees no position gives zeros. A token whose key or value is not finite counts for its own row and those behind it, never for one
- * before it. o must not overlap what is read. max_pages up to 2^27 - 1. The first call of a context makes its workspace, so that it must not be one that is
- * recorded; lengths, tables and starts are read on the device, a recorded call follows what they hold by then. */
+ * values rounded to f16 (2^-11 of each, weights below 2^-21 of the row's largest 2^-32 of that), sums in 32 bits. That is less than
+ * brasa_k_flash_attention_with keeps under the same name, which rounds q * scale alone. F32: o f32, 32-bit arithmetic, over an f16 cache
+ * with q and the weights as two f16 terms under powers of two of their own (2^-22 of the value, or 2^-40 of the largest of the row or of
+ * sixteen keys). Cache rows that a sequence has not reached may hold anything, infinities and NaN included. A token that sees no position
+ * gives zeros. A token whose key or value is not finite counts for its own row and those behind it, never for one
+ * before it. o must not overlap what is read. max_pages up to 2^27 - 1. The first call of a context makes its workspace, 59 MB on 148 SMs
+ * whatever the call, so that it must not be one that is recorded; lengths, tables and starts are read on the device, a recorded call follows what they hold by then. */
 int32_t brasa_k_attention_packed(brasa_cmd *cmd, brasa_arg q, brasa_paged_kv paged, brasa_packed_run run, brasa_arg o, uint32_t hq, uint32_t hkv, int32_t precision);
 /* Verification of drafted tokens. Sequence s has rows starts[s] .. starts[s + 1] - 1 (u32 [seqs + 1], not falling, at most `rows`) of p
  * f32 [rows][vocab], the target model's probabilities behind its last token and behind each of its drafted ones, so one row more
@@ -483,9 +485,8 @@ typedef struct brasa_page_pool {
  * all) of the lens[source[r]] that it holds, and gets pages for room[r] (u32) positions more, as far as max_pages reach. With accepted
  * (u32 [rows], buf NULL: none), as brasa_k_verify_drafts leaves it, an old row s holds accepted[s] + 1 positions more than lens[s]: the token
  * that the step began with and the drafts that stood. starts (u32 [rows + 1], buf NULL: every row was in the step) are the step's: a row without new
- * tokens in it, paused or free, holds what lens says, for accepted[s] 0 alone does not tell it from one whose drafts were all refused. One call forks (several rows
- * with one source), reorders,
- * rolls back, frees (source -1 or keep 0, room 0) and reserves. Whole pages that are kept are shared. The last page of a row, when it is not
+ * tokens in it, paused or free, holds what lens says, for accepted[s] 0 alone does not tell it from one whose drafts were all refused. One call
+ * forks (several rows with one source), reorders, rolls back, frees (source -1 or keep 0, room 0) and reserves. Whole pages that are kept are shared. The last page of a row, when it is not
  * full, becomes its own to write into: the first row that ends in it keeps it, unless it is pinned or held as a whole page too, the
  * others get copies of it in all layers. Pages that no new row holds are free at once; free ones are handed out from the lowest
  * on, to the rows in order (a copy's page ahead of those for new positions). Table entries that name no page are kept as -1.
