@@ -212,9 +212,9 @@ __device__ __forceinline__ bool line_next(const PackedLine &l, PackedItem &it) {
 // ---- rows before a value that is not finite ----
 // A weight of zero times an infinity or NaN of V is NaN, so that in a matrix product a key behind a row's own position, new in the same run, reaches the row. A kernel
 // that finds a row not finite although keys of its share lie behind it comes here with all its threads, at a place where no other warp waits for them.
-// Dim by dim, V of the share's new positions says where the last value is that is not finite and where the first NaN: a row is taken again when it has a dim
-// that a value behind it spoiled and that no NaN at or before it makes NaN anyway. What the row's older positions hold is not looked at: a value there costs
-// this one look at up to 256 positions. An 8-bit value that the products round to an f16 infinity spoils like one.
+// V of the share is looked at once, dim by dim: where the first NaN and the first infinity of either sign are, and the last of them. That says of a dim which a value behind
+// the row reached what it has to be when the row sees such values itself: NaN, or the infinity. Only where it sees none the row is taken again, key by key. An
+// overflowing channel or a prompt of NaN so costs the one look. An 8-bit value that the products round to an f16 infinity is one.
 struct PackedAgain {
     const float *q;
     const uint8_t *kpool, *vpool;
@@ -283,15 +283,16 @@ __device__ __forceinline__ PackedRowSums packed_row_again(const PackedView &v, c
 }
 template <int KV, bool HALF>
 __device__ __noinline__ void packed_rows_again(const PackedLine &l, const PackedAgain &a) {
-    __shared__ uint32_t first_nan[128], past_bad[128];  // by dim: positions, the second one further on
+    __shared__ uint32_t first_nan[128], first_up[128], first_down[128], past_bad[128];  // by dim: positions, the last one further on
     constexpr float LIMIT = KV == BRASA_KV_Q8_0 && HALF ? 65520.0f : INFINITY;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     for (uint32_t i = threadIdx.x; i < 128; i += blockDim.x) {
-        first_nan[i] = UINT32_MAX;
+        first_nan[i] = first_up[i] = first_down[i] = UINT32_MAX;
         past_bad[i] = 0;
     }
     __syncthreads();
-    for (uint32_t p = max(a.past, a.from) + warp; p < a.upto; p += warps) {
+#pragma unroll 4
+    for (uint32_t p = a.from + warp; p < a.upto; p += warps) {
         const int32_t page = packed_page(l.v, a.seq, p);
         if (page < 0) continue;
         const float4 y = packed_row4<KV>(a.vpool + (((size_t)page * BRASA_KV_PAGE + p % BRASA_KV_PAGE) * l.v.hkv + a.kh) * KvRow<KV>::BYTES, lane);
@@ -300,14 +301,20 @@ __device__ __noinline__ void packed_rows_again(const PackedLine &l, const Packed
         for (uint32_t e = 0; e < 4; ++e)
             if (!(fabsf(ys[e]) < LIMIT)) {
                 atomicMax(&past_bad[4 * lane + e], p + 1);
-                if (ys[e] != ys[e]) atomicMin(&first_nan[4 * lane + e], p);
+                atomicMin(&(ys[e] != ys[e] ? first_nan : ys[e] > 0.0f ? first_up : first_down)[4 * lane + e], p);
             }
     }
     __syncthreads();
-    const uint4 nan = reinterpret_cast<const uint4 *>(first_nan)[lane], bad = reinterpret_cast<const uint4 *>(past_bad)[lane];
     for (uint32_t r = warp; r < a.rows; r += warps) {
         const uint32_t token = row_token(l, r), own = a.past + token;
         const size_t at = ((size_t)(a.t0 + token) * a.hq + a.kh * l.group + r - token * l.group) * 128 + 4 * lane;
+        auto put = [&](const float4 &v) {
+            if (!a.whole) reinterpret_cast<float4 *>(a.part + (size_t)r * 128)[lane] = v;
+            else if (HALF) {
+                const __half2 lo = __floats2half2_rn(v.x, v.y), hi = __floats2half2_rn(v.z, v.w);
+                *reinterpret_cast<uint2 *>(static_cast<__half *>(a.o) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+            } else *reinterpret_cast<float4 *>(static_cast<float *>(a.o) + at) = v;
+        };
         float4 y;
         if (!a.whole) y = reinterpret_cast<const float4 *>(a.part + (size_t)r * 128)[lane];
         else if (HALF) {
@@ -315,22 +322,34 @@ __device__ __noinline__ void packed_rows_again(const PackedLine &l, const Packed
             const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
             y = make_float4(lo.x, lo.y, hi.x, hi.y);
         } else y = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.o) + at);
-        auto spoiled = [&](float v, uint32_t upto, uint32_t first) { return not_finite(v) && upto > own + 1 && first > own; };
-        if (!__any_sync(0xffffffffu, spoiled(y.x, bad.x, nan.x) || spoiled(y.y, bad.y, nan.y) || spoiled(y.z, bad.z, nan.z) || spoiled(y.w, bad.w, nan.w))) continue;
-        const PackedRowSums x = packed_row_again<KV>(l.v, a.kpool, a.vpool, a.q + at - 4 * lane, a.scale, a.seq, a.kh, a.from, min(a.upto, own + 1));
-        if (a.whole) {
-            const float inv = x.l == 0.0f ? 0.0f : 1.0f / x.l;
-            const float4 v = make_float4(x.o.x * inv, x.o.y * inv, x.o.z * inv, x.o.w * inv);
-            if (HALF) {
-                const __half2 lo = __floats2half2_rn(v.x, v.y), hi = __floats2half2_rn(v.z, v.w);
-                *reinterpret_cast<uint2 *>(static_cast<__half *>(a.o) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-            } else *reinterpret_cast<float4 *>(static_cast<float *>(a.o) + at) = v;
-        } else {
-            reinterpret_cast<float4 *>(a.part + (size_t)r * 128)[lane] = x.o;
-            if (lane == 0) {
-                a.part[(size_t)a.rows_item * 128 + r] = x.m;
-                a.part[(size_t)a.rows_item * 129 + r] = x.l;
+        float ys[4] = {y.x, y.y, y.z, y.w};
+        bool clean = false, dead = false, known = false, taken = false;  // a dim without such values; one that is NaN, so that a score is; a dim known to be an infinity; one not known
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            const uint32_t d = 4 * lane + e, bad = past_bad[d];
+            if (bad == 0) {
+                clean = true;
+                dead = dead || ys[e] != ys[e];
+            } else if (not_finite(ys[e]) && bad > own + 1 && first_nan[d] > own) {
+                const bool up = first_up[d] <= own, down = first_down[d] <= own;
+                if (up != down) {
+                    ys[e] = up ? INFINITY : -INFINITY;
+                    known = true;
+                } else if (!up) taken = true;
             }
+        }
+        if (__any_sync(0xffffffffu, dead)) continue;
+        const bool some = __any_sync(0xffffffffu, known);
+        if (!__any_sync(0xffffffffu, taken) && (!some || __any_sync(0xffffffffu, clean))) {  // (with no dim clean a NaN of a score would not show)
+            if (some) put(make_float4(ys[0], ys[1], ys[2], ys[3]));
+            continue;
+        }
+        const PackedRowSums x = packed_row_again<KV>(l.v, a.kpool, a.vpool, a.q + at - 4 * lane, a.scale, a.seq, a.kh, a.from, min(a.upto, own + 1));
+        const float inv = !a.whole ? 1.0f : x.l == 0.0f ? 0.0f : 1.0f / x.l;
+        put(make_float4(x.o.x * inv, x.o.y * inv, x.o.z * inv, x.o.w * inv));
+        if (!a.whole && lane == 0) {
+            a.part[(size_t)a.rows_item * 128 + r] = x.m;
+            a.part[(size_t)a.rows_item * 129 + r] = x.l;
         }
     }
     __syncthreads();

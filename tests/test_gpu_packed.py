@@ -327,6 +327,44 @@ def test_attention_bad_values_dim_by_dim(ctx, K, kv, half):
         assert not np.isfinite(got[a + then:a + n, :, 64:96]).any()
 
 
+@pytest.mark.parametrize("seqs", [[(500, 6000), (2, 50)], [(1200, 0), (1, 700)], [(7, 900)]])
+@pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("q8_0", False), ("f32", False)])
+def test_attention_a_channel_that_overflows(ctx, K, kv, half, seqs):
+    """Infinities in the last 32 dims of every new token of the first sequence, of the other sign from the fifth on, and a NaN key in its second but last: the rows are
+    infinite there, then NaN, the last two NaN throughout, all else as without. The call takes no longer for it than a call takes."""
+    run = R.Run(seqs, 4, 2, kv, seed=55)
+    n, past = seqs[0]
+    times = []
+    for bad in (False, True):
+        if bad:
+            for j in range(n):
+                raw = run.v[run.table[0, (past + j) // R.PAGE], (past + j) % R.PAGE]
+                value = np.inf if j < 4 else -np.inf
+                if kv == "q8_0":
+                    raw[:, 96:128] = 1
+                    raw[:, 128:].view(np.float16)[:, 3] = value
+                else:
+                    raw.view(np.float16 if kv == "f16" else np.float32)[:, 96:] = value
+            put_row(run, run.k, 0, past + n - 2, np.full((2, R.D), np.nan, np.float32))
+        dev = OnDevice(ctx, K, run)
+        o = ctx.buffer(run.tokens * 4 * 512)
+        took = []
+        for _ in range(4):
+            cmd = ctx.command()
+            K.attention_packed(cmd, dev.q, dev.paged, dev.packed, o, 4, 2, 0 if half else 1)
+            took.append(cmd.wait())
+        times.append(min(took))
+        got = o.download(np.float16 if half else np.float32)[:run.tokens * 4 * 128].astype(np.float64).reshape(run.tokens, 4, 128)
+        if not bad:
+            clean = got
+        o.free()
+        dev.free()
+    rest = np.delete(np.arange(run.tokens), [n - 2, n - 1])
+    assert (got[rest, :, :96] == clean[rest, :, :96]).all() and (got[n:] == clean[n:]).all()
+    assert (got[:4, :, 96:] == np.inf).all() and np.isnan(got[4:n, :, 96:]).all() and np.isnan(got[n - 2:n]).all()
+    assert times[1] < 2 * times[0] + 2e-4, times
+
+
 @pytest.mark.parametrize("shape", [[(6, 40)], [(60, 900)]])
 def test_attention_8_bit_values_past_f16(ctx, K, shape):
     """A new token's value that is finite in 8 bits and infinite in f16, as the products of F16 precision round it, does not reach the rows before it."""
