@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PackedPieces pieces;
     __shared__ float sums[4][2][16];
-    __shared__ uint32_t again;  // a row is not finite although keys lie behind it
+    __shared__ uint32_t again;  // a row is not finite and may have to be otherwise (packed_rows_again)
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem), hkv = p.l.v.hkv, G = p.l.group;
     PackedNote note{};
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
                 L = fmaf(sums[w][1][x], f, L);
                 acc = fmaf(reinterpret_cast<float *>(smem)[(w * 16 + x) * FEW_TS + tid], f, acc);
             }
-            if (not_finite(acc) && it.past + token0 + row_token(p.l, r) + 1 < upto) again = 1;
+            if (not_finite(acc) && (!HALF || it.past + token0 + row_token(p.l, r) + 1 < upto)) again = 1;
             if (whole) {
                 const uint32_t token = row_token(p.l, r);
                 const size_t at = ((size_t)(t0 + token) * p.hq + it.kh * G + r - token * G) * D + tid;
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(F32_THREADS, 1) attn_packed_f32_kernel(const _
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(16) float fs[];
     __shared__ PackedPieces pieces;
-    __shared__ uint32_t again;  // a row is not finite although keys lie behind it
+    __shared__ uint32_t again;  // a row is not finite and may have to be otherwise (packed_rows_again)
     float *qs = fs, *ks = qs + 64 * FEW_TS, *vs = ks + 64 * FEW_TS, *ps = vs + 64 * FEW_TS;
     const uint32_t tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, hkv = p.l.v.hkv, G = p.l.group;
     PackedNote note{};

@@ -214,7 +214,10 @@ __device__ __forceinline__ bool line_next(const PackedLine &l, PackedItem &it) {
 // that finds a row not finite although keys of its share lie behind it comes here with all its threads, at a place where no other warp waits for them.
 // V of the share is looked at once, dim by dim: where the first NaN and the first infinity of either sign are, and the last of them. That says of a dim which a value behind
 // the row reached what it has to be when the row sees such values itself: NaN, or the infinity. Only where it sees none the row is taken again, key by key. An
-// overflowing channel or a prompt of NaN so costs the one look. An 8-bit value that the products round to an f16 infinity is one.
+// overflowing channel or a prompt of NaN so costs the one look. An 8-bit value that the products round to an f16 infinity is one. Weights in two terms make NaN of an
+// infinity that the row does see, since the second term is 0 or negative: such a kernel comes here with every row that is not finite.
+template <int KV, bool HALF>
+constexpr bool two_terms() { return KV == BRASA_KV_F16 && !HALF; }
 struct PackedAgain {
     const float *q;
     const uint8_t *kpool, *vpool;
@@ -285,6 +288,7 @@ template <int KV, bool HALF>
 __device__ __noinline__ void packed_rows_again(const PackedLine &l, const PackedAgain &a) {
     __shared__ uint32_t first_nan[128], first_up[128], first_down[128], past_bad[128];  // by dim: positions, the last one further on
     constexpr float LIMIT = KV == BRASA_KV_Q8_0 && HALF ? 65520.0f : INFINITY;
+    constexpr bool TERMS = two_terms<KV, HALF>();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     for (uint32_t i = threadIdx.x; i < 128; i += blockDim.x) {
         first_nan[i] = first_up[i] = first_down[i] = UINT32_MAX;
@@ -330,7 +334,7 @@ __device__ __noinline__ void packed_rows_again(const PackedLine &l, const Packed
             if (bad == 0) {
                 clean = true;
                 dead = dead || ys[e] != ys[e];
-            } else if (not_finite(ys[e]) && bad > own + 1 && first_nan[d] > own) {
+            } else if (not_finite(ys[e]) && (TERMS || bad > own + 1) && first_nan[d] > own) {
                 const bool up = first_up[d] <= own, down = first_down[d] <= own;
                 if (up != down) {
                     ys[e] = up ? INFINITY : -INFINITY;

@@ -327,6 +327,31 @@ def test_attention_bad_values_dim_by_dim(ctx, K, kv, half):
         assert not np.isfinite(got[a + then:a + n, :, 64:96]).any()
 
 
+@pytest.mark.parametrize("seqs", [[(1, 300)], [(6, 90), (1, 2000)], [(70, 30)]])
+@pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("q8_0", False), ("f32", False), ("f32", True)])
+def test_attention_infinities_that_a_row_sees(ctx, K, kv, half, seqs):
+    """An infinity of V at an old position makes its dims that infinity, of both signs NaN; in 8 bits a block of 32 dims."""
+    run = R.Run(seqs, 6, 2, kv, seed=59)
+    want, tol = run.attention(half)
+    at = seqs[0][1] // 2
+    for j, dims, values in ((at, slice(32, 64), (np.inf, -np.inf)), (at + 1, slice(64, 96), (-np.inf, np.inf)), (at + 2, slice(64, 96), (-np.inf, -np.inf))):
+        for h in range(2):
+            raw = run.v[run.table[0, j // R.PAGE], j % R.PAGE, h]
+            if kv == "q8_0":
+                raw[dims] = 1
+                raw[128:].view(np.float16)[dims.start // 32] = values[h]
+            else:
+                raw.view(np.float16 if kv == "f16" else np.float32)[dims] = values[h]
+    got, _ = attend(ctx, K, run, half)
+    n = seqs[0][0]
+    for d in (slice(0, 32), slice(96, 128)):
+        check(got[:n, :, d], want[:n, :, d], tol[:n, :, d])
+    assert (got[:n, :3, 32:64] == np.inf).all() and (got[:n, 3:, 32:64] == -np.inf).all()
+    assert (got[:n, :3, 64:96] == -np.inf).all() and np.isnan(got[:n, 3:, 64:96]).all()
+    if len(seqs) > 1:
+        check(got[n:], want[n:], tol[n:])
+
+
 @pytest.mark.parametrize("seqs", [[(500, 6000), (2, 50)], [(1200, 0), (1, 700)], [(7, 900)]])
 @pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("q8_0", False), ("f32", False)])
 def test_attention_a_channel_that_overflows(ctx, K, kv, half, seqs):
