@@ -445,6 +445,44 @@ def test_attention_long_cache(ctx, K):
         check(attend(ctx, K, run, half)[0], want, tol)
 
 
+@pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("f32", False)])
+def test_pages_behind_4_gib(B, ctx, K, kv, half):
+    """The store, the attention and the page operators on pages whose offsets pass 32 bits: the bits of the same run in a small pool."""
+    run = R.Run([(40, 30), (3, 200), (1, 0)], 16, 8, kv, seed=57)
+    page = 16 * 8 * R.ROW[kv]
+    num = 2 ** 32 // page + 2 * run.num_pages
+    first = num - run.num_pages
+    small = OnDevice(ctx, K, run)
+    kpool, vpool = ctx.buffer(num * page), ctx.buffer(num * page)
+    kpool.upload(run.k, first * page), vpool.upload(run.v, first * page)
+    table = ctx.buffer_from((run.table + first).astype(np.int32))
+    far = K.paged_kv(kpool, vpool, table, small.bufs[3], 3, run.max_pages, num, KV[kv])
+    g = np.random.default_rng(58)
+    k, v = (ctx.buffer_from(g.standard_normal((run.tokens, 8, 128)).astype(np.float32)) for _ in range(2))
+    norm, rope = ctx.buffer_from(np.ones(128, np.float32)), B.RopeTable(ctx, THETA, 128, run.max_pages * 16)
+    n = run.tokens * 16 * 128
+    got = []
+    for paged, pools, at in ((small.paged, (small.kpool, small.vpool), 0), (far, (kpool, vpool), first * page)):
+        q, o = ctx.buffer(n * 4), ctx.buffer(n * 4)
+        go(ctx, lambda c: K.qk_norm_rope_store_packed(c, small.q, k, v, norm, norm, EPS, rope, paged, small.packed, q, 16, 8))
+        go(ctx, lambda c: K.attention_packed(c, q, paged, small.packed, o, 16, 8, 0 if half else 1))
+        got.append([q.download(np.uint32), o.download(np.uint32)] + [p.download(np.uint8, run.k.size, at) for p in pools])
+        q.free(), o.free()
+    assert all((a == b).all() for a, b in zip(*got))
+    result, moved, out = ctx.buffer(16), ctx.buffer(num * 4), ctx.buffer(run.table.nbytes)
+    pool = K.page_pool(kpool, vpool, table, small.bufs[3], None, 3, run.max_pages, num, 1, 8, KV[kv])
+    go(ctx, lambda c: K.pages_compact(c, pool, out, moved, result))  # (pages that the table names are entries of any page: those of no sequence too)
+    want, to, counts, moves = R.compact(run.table + first, None, num)
+    assert (out.download(np.int32).reshape(want.shape) == want).all() and list(result.download(np.uint32)) == counts and len(moves) == counts[1] > 0
+    for p, was in zip((kpool, vpool), got[0][2:]):
+        was = was.reshape(run.k.shape)
+        for a, b in moves:
+            assert (p.download(np.uint8, page, b * page) == was[a - first].reshape(-1)).all()
+    for b in (kpool, vpool, table, k, v, norm, result, moved, out):
+        b.free()
+    small.free()
+
+
 def test_attention_many_sequences(ctx, K):
     """More sequences than a warp has lanes, most without new tokens."""
     g = np.random.default_rng(2)
