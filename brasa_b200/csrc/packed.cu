@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_store_packed_kernel(const fl
 // keys to at most 2^15. Hi + lo is then off by 2^-22 of the value, or 2^-40 of the largest, whatever the other keys weigh; a step's product is added to O in 32 bits.
 // l sums the weights as the product reads them, by a column of ones beside V.
 // Bound by the cache's bytes while an item has one row tile or two, by mma.sync and its waits beyond that, where the tcgen05 kernel takes over (PACKED_TC_MIN_ROWS). 64
-// sequences of two to five tokens behind 2600 (32 heads on 8, f16) 154 us, 4.6 TB/s, in F32 precision 204 us; behind a flush of the L2, 16 of three behind 3000 take 61 us with
+// sequences of two to five tokens behind 2600 (32 heads on 8, f16) 154 us, 4.6 TB/s, in F32 precision 198 us; behind a flush of the L2, 16 of three behind 3000 take 61 us with
 // an 8-bit cache and 63 with an f16 one: there no unit is full (DRAM 33 %, issue slots 43 %), a page's chain of reads, conversions and products is what is waited for.
 struct FewParams {
     PackedLine l;
@@ -287,15 +287,19 @@ __global__ void __launch_bounds__(128, FEW_BLOCKS) attn_packed_few_kernel(const 
                     s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
                     if (!Q8) {
                         const uint32_t row = 16 * u + 8 * t + (lane & 7);
+                        float low[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of the second terms: 0 or of either sign, so that an infinite key's score is what the first ones make it
 #pragma unroll
                         for (uint32_t ks = 0; ks < 8; ks += 2) {
                             uint32_t b[4];
                             ldsm_x4(b, kt + row * 256 + (((2 * ks + (lane >> 3)) ^ (row & 7)) << 4));
                             mma_f16(s[t], qh[ks], b[0], b[1]);
-                            if (!HALF) mma_f16(s[t], ql[ks], b[0], b[1]);
+                            if (!HALF) mma_f16(low, ql[ks], b[0], b[1]);
                             mma_f16(s[t], qh[ks + 1], b[2], b[3]);
-                            if (!HALF) mma_f16(s[t], ql[ks + 1], b[2], b[3]);
+                            if (!HALF) mma_f16(low, ql[ks + 1], b[2], b[3]);
                         }
+                        if (!HALF)
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e) s[t][e] += not_finite(s[t][e]) ? 0.0f : low[e];
                     } else {
                         const uint8_t *row = smem + (kt - ring) + (16 * u + 8 * t + g) * S::K_PITCH;
                         const uint2 sc = *reinterpret_cast<const uint2 *>(row + 128);

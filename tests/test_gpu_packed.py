@@ -352,6 +352,22 @@ def test_attention_infinities_that_a_row_sees(ctx, K, kv, half, seqs):
         check(got[n:], want[n:], tol[n:])
 
 
+@pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("f32", False), ("f32", True)])
+def test_attention_infinite_keys(ctx, K, kv, half):
+    """An infinity in one dim of old keys: a row whose query is negative there has scores of minus infinity and attends to the others, any other row is NaN."""
+    run = R.Run([(3, 200), (40, 60), (1, 1500)], 8, 2, kv, seed=60)
+    for s in range(3):
+        run.k[run.table[s, 2]].reshape(16, 2, -1).view(np.float16 if kv == "f16" else np.float32)[:, :, 7] = np.inf
+    table = run.table.copy()
+    run.table[:, 2] = -1
+    want, tol = run.attention(half)
+    run.table = table
+    got, _ = attend(ctx, K, run, half)
+    down = run.q[:, :, 7] < 0
+    check(got[down], want[down], tol[down])
+    assert np.isnan(got[~down]).all()
+
+
 @pytest.mark.parametrize("seqs", [[(500, 6000), (2, 50)], [(1200, 0), (1, 700)], [(7, 900)]])
 @pytest.mark.parametrize("kv,half", [("f16", True), ("f16", False), ("q8_0", True), ("q8_0", False), ("f32", False)])
 def test_attention_a_channel_that_overflows(ctx, K, kv, half, seqs):
